@@ -15,10 +15,18 @@ from .sampler import NeighborSampler, ParallelBatchSampler, SampledSubgraph, Sam
 
 __version__ = "0.1.0"
 
+
+def __getattr__(name):
+    if name == "ops":  # needs torch, which the rest of the package imports only where it is used
+        import importlib
+
+        return importlib.import_module(".ops", __name__)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
 __all__ = [
     "CsrGraph", "FeatureStore", "Graph", "GraphLoadError", "HeteroCsrGraph", "HeteroNeighborLoader",
     "HeteroNeighborSampler", "HeteroSampledSubgraph", "HeteroSamplingConfig", "NeighborLoader", "NeighborSampler",
     "ParallelBatchSampler", "PrefetchStats",
-    "SampledSubgraph", "Sampler", "SamplingConfig", "SamplingError", "__version__", "partition_aligned_batches",
+    "SampledSubgraph", "Sampler", "SamplingConfig", "SamplingError", "__version__", "ops", "partition_aligned_batches",
     "release_kept_memory", "save_features",
 ]

@@ -15,8 +15,8 @@ LIB_PATH = os.path.join(_HERE, "libaethergpu.so")
 AG_OK, AG_ERR_VALUE, AG_ERR_LOAD, AG_ERR_SAMPLING, AG_ERR_TIMEOUT, AG_ERR_WORKER, AG_ERR_CUDA, \
     AG_ERR_SHUTDOWN = range(8)
 AG_MEM_HOST, AG_MEM_DEVICE = 0, 1
-AG_F32, AG_F16, AG_BF16, AG_I8 = 0, 1, 2, 3
-DTYPE_TAG = {"f32": AG_F32, "f16": AG_F16, "bf16": AG_BF16, "i8": AG_I8}
+AG_F32, AG_F16, AG_BF16, AG_I8, AG_F8 = 0, 1, 2, 3, 4
+DTYPE_TAG = {"f32": AG_F32, "f16": AG_F16, "bf16": AG_BF16, "i8": AG_I8, "f8": AG_F8}
 DTYPE_NAME = {v: k for k, v in DTYPE_TAG.items()}
 VALIDATION = {"auto": 0, "header_only": 1, "offsets_only": 2, "full": 3}
 AG_RNG_WYRAND_EXACT, AG_RNG_PHILOX = 0, 1
@@ -99,6 +99,25 @@ class HeteroBatch(C.Structure):
     _fields_ = [("batch_idx", C.c_int64), ("seq", C.c_uint64), ("bufs", HeteroBuffers), ("counts", HeteroCounts)]
 
 
+class Norm(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "residual", "weight", "y", "h", "rstd", "codes", "scales")] + \
+               [(n, C.c_uint64) for n in ("rows", "dim", "x_stride", "residual_stride", "y_stride", "h_stride", "code_stride", "seed",
+                                          "offset")] + \
+               [("p", C.c_double), ("eps", C.c_float), ("dtype", C.c_int32), ("weight_dtype", C.c_int32), ("encode_only", C.c_int32)]
+
+
+class NormGrad(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "dh", "h", "weight", "rstd", "dx", "dresidual", "dw", "scratch")] + \
+               [(n, C.c_uint64) for n in ("scratch_bytes", "rows", "dim", "dy_stride", "dh_stride", "h_stride", "seed", "offset")] + \
+               [("p", C.c_double), ("dtype", C.c_int32), ("weight_dtype", C.c_int32)]
+
+
+class Product(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("codes", "scales", "weight", "weight_scales", "ids", "bias", "out")] + \
+               [(n, C.c_uint64) for n in ("rows", "held", "dim", "out_dim", "code_stride", "weight_stride", "out_stride")] + \
+               [("ids_are_i64", C.c_int32), ("out_dtype", C.c_int32)]
+
+
 _P = C.c_void_p
 _PP = C.POINTER(C.c_void_p)
 _U64P = C.POINTER(C.c_uint64)
@@ -137,6 +156,8 @@ SIGNATURES = {
     "ag_features_from_memory": (C.c_int32, [_P, C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, C.c_int32, _PP]),
     "ag_features_from_f32": (C.c_int32, [_P, C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, C.c_int32, _PP]),
     "ag_features_adopt_device": (C.c_int32, [_P, C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, _PP]),
+    "ag_features_from_f8": (C.c_int32, [_P, _P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_int32, _PP]),
+    "ag_features_f8_rows": (C.c_int32, [_P, _PP, _PP, _U64P]),
     "ag_features_info": (C.c_int32, [_P, _U64P, _U64P, _I32P, _I32P, _U64P]),
     "ag_features_device_ptr": (C.c_int32, [_P, _PP]),
     "ag_features_get_batch": (C.c_int32, [_P, _P, C.c_uint64, _P]),
@@ -205,6 +226,14 @@ SIGNATURES = {
     "ag_hetero_loader_stats_get": (C.c_int32, [_P, C.POINTER(LoaderStats)]),
     "ag_hetero_loader_shutdown": (C.c_int32, [_P]),
     "ag_hetero_loader_free": (None, [_P]),
+    "ag_rows_dropout": (C.c_int32, [_P, _P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_int32, C.c_double, C.c_uint64,
+                                    C.c_uint64, C.c_int32, _P]),
+    "ag_rows_norm": (C.c_int32, [_P, C.c_int32, _P]),
+    "ag_rows_norm_backward_scratch": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_int32, _U64P]),
+    "ag_rows_norm_backward": (C.c_int32, [_P, C.c_int32, _P]),
+    "ag_rows_encode_weight": (C.c_int32, [_P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_int32, _P, C.c_uint64, _P, C.c_int32, _P]),
+    "ag_rows_product": (C.c_int32, [_P, C.c_int32, _P]),
+    "ag_rows_check": (C.c_int32, [C.c_int32]),
     "ag_synth_rmat_graph": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_float, C.c_float, C.c_float, C.c_uint64,
                                         C.c_float, C.c_int32, _PP]),
     "ag_synth_rmat_csr": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_uint64, C.c_float, C.c_float, C.c_float,

@@ -991,8 +991,9 @@ extern "C" int32_t ag_features_copy_to_host(const ag_features *f, void *payload)
     if (f->shards) return fail(AG_ERR_VALUE, "ag_features_copy_to_host: a sharded view holds no rows of its own; copy each shard");
     DeviceGuard guard(f->device);
     if (!guard.ok) return AG_ERR_CUDA;
-    const uint64_t bytes = f->rows * f->dim * elem_size(f->dtype);
-    if (bytes) AG_CUDA(cudaMemcpy(payload, f->payload, bytes, cudaMemcpyDeviceToHost));
+    const uint64_t row = f->dim * elem_size(f->dtype), bytes = f->rows * row;
+    if (bytes && f->pitch) AG_CUDA(cudaMemcpy2D(payload, row, f->payload, f->pitch, row, f->rows, cudaMemcpyDeviceToHost));
+    else if (bytes) AG_CUDA(cudaMemcpy(payload, f->payload, bytes, cudaMemcpyDeviceToHost));
     return AG_OK;
 }
 
@@ -1076,11 +1077,11 @@ ag_features *new_features(int device, uint64_t n, uint64_t begin, uint64_t rows,
 int32_t alloc_features(ag_features *f, bool alloc_payload) {
     if (alloc_payload) {
         // a block peers can map with large pages, should the store become a shard of a view
-        AG_TRY(alloc_feature_payload(f->device, std::max<uint64_t>(f->rows * f->dim * elem_size(f->dtype), 16), &f->payload,
+        AG_TRY(alloc_feature_payload(f->device, std::max<uint64_t>(f->rows * row_pitch(f), 16), &f->payload,
                                      &f->block));
     }
-    if (alloc_payload && f->dtype == AG_I8)
-        AG_CUDA(device_malloc(&f->scales, std::max<uint64_t>(f->rows * ((f->dim + kQuantBlock - 1) / kQuantBlock) * 4, 16)));
+    if (alloc_payload && scales_per_row(f->dtype, f->dim))
+        AG_CUDA(device_malloc(&f->scales, std::max<uint64_t>(f->rows * scales_per_row(f->dtype, f->dim) * 4, 16)));
     AG_CUDA(device_malloc(&f->err, 32));  // error bits, then the gather counters (internal.h)
     AG_CUDA(cudaMemset(f->err, 0, 32));
     return AG_OK;
@@ -1263,11 +1264,13 @@ extern "C" int32_t ag_features_from_memory(const void *payload, uint64_t num_nod
 extern "C" int32_t ag_features_from_f32(const float *features, uint64_t num_nodes, uint64_t dim, int32_t dtype,
                                         int32_t mem_kind, int32_t device, ag_features **out) {
     if ((!features && num_nodes * dim) || !out) return fail(AG_ERR_VALUE, "ag_features_from_f32: null argument");
-    if (dtype < 0 || dtype > AG_I8) return fail(AG_ERR_VALUE, "unknown feature dtype tag: %d", dtype);
-    if (dtype == AG_I8 && dim == 0) return fail(AG_ERR_VALUE, "feature_dim must be non-zero");  // FeatureCodecError::ZeroDim
+    if (dtype < 0 || dtype > AG_F8) return fail(AG_ERR_VALUE, "unknown feature dtype tag: %d", dtype);
+    if (dtype == AG_F8 && dim > 0x7FFFFFF0ull) return fail(AG_ERR_VALUE, "8-bit float rows hold fewer than 2^31 columns");
+    if ((dtype == AG_I8 || dtype == AG_F8) && dim == 0) return fail(AG_ERR_VALUE, "feature_dim must be non-zero");  // FeatureCodecError::ZeroDim
     DeviceGuard guard(device);
     if (!guard.ok) return AG_ERR_CUDA;
     ag_features *f = new_features(device, num_nodes, 0, num_nodes, dim, dtype);
+    if (dtype == AG_F8) f->pitch = (dim + 15) / 16 * 16;
     int32_t st = alloc_features(f, true);
     const uint64_t count = num_nodes * dim;
     float *staged = nullptr;
@@ -1284,11 +1287,13 @@ extern "C" int32_t ag_features_from_f32(const float *features, uint64_t num_node
             src = staged;
         }
         cudaError_t e;
-        if (dtype == AG_I8) {
+        if (dtype == AG_I8 || dtype == AG_F8) {
             uint32_t hbad = 0;
             e = device_malloc(&bad, 4);
             if (e == cudaSuccess) e = cudaMemset(bad, 0, 4);
-            if (e == cudaSuccess) e = launch_encode_i8(src, num_nodes, dim, (int8_t *)f->payload, f->scales, bad, 0);
+            if (e == cudaSuccess)
+                e = dtype == AG_F8 ? launch_encode_f8(src, num_nodes, dim, f->pitch, f->payload, f->scales, bad, 0)
+                                   : launch_encode_i8(src, num_nodes, dim, (int8_t *)f->payload, f->scales, bad, 0);
             if (e == cudaSuccess) e = cudaMemcpy(&hbad, bad, 4, cudaMemcpyDeviceToHost);
             if (e == cudaSuccess && hbad) { st = fail(AG_ERR_VALUE, "feature values must be finite"); break; }  // FeatureCodecError::NotFinite
         } else {
@@ -1314,6 +1319,30 @@ extern "C" int32_t ag_features_adopt_device(void *payload_dev, uint64_t num_node
     const int32_t st = alloc_features(f, false);
     if (st != AG_OK) { f->owns_payload = false; ag_features_free(f); return st; }
     *out = f;
+    return AG_OK;
+}
+
+extern "C" int32_t ag_features_from_f8(const void *codes, const float *scales, uint64_t num_nodes, uint64_t dim, uint64_t code_stride,
+                                       int32_t device, ag_features **out) {
+    if (((!codes || !scales) && num_nodes) || !out) return fail(AG_ERR_VALUE, "ag_features_from_f8: null argument");
+    if (dim == 0 || dim > 0x7FFFFFF0ull) return fail(AG_ERR_VALUE, "8-bit float rows hold 1 to 2^31 - 16 columns, got %llu", (unsigned long long)dim);
+    if (code_stride % 16 || code_stride < dim || code_stride > 0xFFFFFFFFull || (uintptr_t)codes % 16)
+        return fail(AG_ERR_VALUE, "8-bit float rows start on multiples of 16 bytes and do not overlap");
+    DeviceGuard guard(device);
+    if (!guard.ok) return AG_ERR_CUDA;
+    ag_features *f = new_features(device, num_nodes, 0, num_nodes, dim, AG_F8);
+    f->payload = (uint8_t *)codes; f->scales = (float *)scales; f->pitch = code_stride;
+    f->owns_payload = false;
+    const int32_t st = alloc_features(f, false);
+    if (st != AG_OK) { ag_features_free(f); return st; }
+    *out = f;
+    return AG_OK;
+}
+
+extern "C" int32_t ag_features_f8_rows(const ag_features *f, const void **codes, const float **scales, uint64_t *code_stride) {
+    if (!f || !codes || !scales || !code_stride) return fail(AG_ERR_VALUE, "ag_features_f8_rows: null argument");
+    if (f->dtype != AG_F8) return fail(AG_ERR_VALUE, "the store does not hold 8-bit float rows");
+    *codes = f->payload; *scales = f->scales; *code_stride = f->pitch;
     return AG_OK;
 }
 
@@ -1372,10 +1401,10 @@ extern "C" int32_t ag_gather(const ag_features *f, const void *ids_dev, int32_t 
 
 extern "C" int32_t ag_features_scales_to_host(const ag_features *f, float *scales) {
     if (!f || !scales) return fail(AG_ERR_VALUE, "ag_features_scales_to_host: null argument");
-    if (f->dtype != AG_I8 || !f->scales) return fail(AG_ERR_VALUE, "only the int8 payload carries scales");
+    if ((f->dtype != AG_I8 && f->dtype != AG_F8) || !f->scales) return fail(AG_ERR_VALUE, "only 8-bit payloads carry scales");
     DeviceGuard guard(f->device);
     if (!guard.ok) return AG_ERR_CUDA;
-    AG_CUDA(cudaMemcpy(scales, f->scales, f->rows * ((f->dim + kQuantBlock - 1) / kQuantBlock) * 4, cudaMemcpyDeviceToHost));
+    AG_CUDA(cudaMemcpy(scales, f->scales, f->rows * scales_per_row(f->dtype, f->dim) * 4, cudaMemcpyDeviceToHost));
     return AG_OK;
 }
 

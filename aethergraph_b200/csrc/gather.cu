@@ -22,6 +22,7 @@
 
 #include <cub/device/device_radix_sort.cuh>
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 
 #include "common.cuh"
 #include "internal.h"
@@ -371,6 +372,73 @@ cudaError_t launch_i8(const GatherArgs &a, const GatherArgs *group, uint32_t row
     else if (vecs <= 8) k_gather_i8<8><<<grid, kThreads, 0, st>>>(a, group, first);
     else if (vecs <= 16) k_gather_i8<16><<<grid, kThreads, 0, st>>>(a, group, first);
     else k_gather_i8<32><<<grid, kThreads, 0, st>>>(a, group, first);
+    return cudaGetLastError();
+}
+
+// 8-bit float rows: e4m3 codes at a pitch of row_bytes (a multiple of 16) and one scale per 128
+// columns; value = code * scale, one multiplication, as ops.product_f8 reads them.  The lanes of a
+// row take its 4-byte words in turn, as above, for loads and 16-byte stores that lie side by side.
+// VEC: output rows start on 16 bytes; else the four floats of a word are stored one by one.
+template <int LPR, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+k_gather_f8(GatherArgs a, const GatherArgs *group) {
+    constexpr int kRowsPerBlock = kThreads / LPR;
+    constexpr int kWordsPerLane = 4;
+    if (group) a = group[blockIdx.y];
+    if (!a.payload) return;
+    const uint64_t n = a.n_dev ? min((uint64_t)*a.n_dev, a.n) : a.n;
+    if (a.ids_off) a.ids = (const uint32_t *)a.ids + *a.ids_off;
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const uint32_t words = (a.dim + 3) / 4, scales_per_row = (a.dim + kF8Block - 1) / kF8Block;
+    constexpr uint64_t kRows = (uint64_t)kRowsPerBlock * kInFlight;  // the grid is sized for this many rows per block
+    for (uint64_t base = (uint64_t)blockIdx.x * kRows + sub; base < n; base += (uint64_t)gridDim.x * kRows)
+        for (int u = 0; u < kInFlight; ++u) {
+            const uint64_t r = base + (uint64_t)u * kRowsPerBlock;
+            if (r >= n) break;
+            const uint64_t id = load_id(a.ids, a.ids64, r), local = id - a.row_begin;
+            const bool ok = id >= a.row_begin && local < a.rows;
+            if (!ok && lane == 0) atomicOr(a.err, kErrBadId);
+            const uint32_t *row = (const uint32_t *)(a.payload + local * a.row_bytes);
+            const float *scales = a.scales + local * scales_per_row;
+            float *dst = a.out + r * a.dim;
+            for (uint32_t w0 = lane; w0 < words; w0 += LPR * kWordsPerLane) {
+                uint32_t val[kWordsPerLane];
+                float scale[kWordsPerLane];
+#pragma unroll
+                for (int q = 0; q < kWordsPerLane; ++q) {
+                    const uint32_t w = w0 + q * LPR;
+                    val[q] = 0; scale[q] = 0.f;  // a row outside the store decodes to zeros
+                    if (ok && w < words) {
+                        val[q] = __ldg(row + w);
+                        scale[q] = __ldg(scales + w / (kF8Block / 4));
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < kWordsPerLane; ++q) {
+                    const uint32_t w = w0 + q * LPR;
+                    if (w >= words) continue;
+                    const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)val[q], __NV_E4M3)));
+                    const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(val[q] >> 16), __NV_E4M3)));
+                    const uint32_t f[4] = {__float_as_uint(lo.x * scale[q]), __float_as_uint(lo.y * scale[q]),
+                                           __float_as_uint(hi.x * scale[q]), __float_as_uint(hi.y * scale[q])};
+                    if (VEC) {
+                        st_stream_v4(dst + (uint64_t)w * 4, make_uint4(f[0], f[1], f[2], f[3]));
+                    } else {
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e)
+                            if (w * 4 + e < a.dim) st_stream_u32(dst + (uint64_t)w * 4 + e, f[e]);
+                    }
+                }
+            }
+        }
+}
+
+template <bool VEC> cudaError_t launch_f8(const GatherArgs &a, const GatherArgs *group, uint32_t row_bytes, dim3 grid, cudaStream_t st) {
+    const uint32_t vecs = row_bytes >> 4;
+    if (vecs <= 4) k_gather_f8<4, VEC><<<grid, kThreads, 0, st>>>(a, group);
+    else if (vecs <= 8) k_gather_f8<8, VEC><<<grid, kThreads, 0, st>>>(a, group);
+    else if (vecs <= 16) k_gather_f8<16, VEC><<<grid, kThreads, 0, st>>>(a, group);
+    else k_gather_f8<32, VEC><<<grid, kThreads, 0, st>>>(a, group);
     return cudaGetLastError();
 }
 
@@ -1090,6 +1158,11 @@ int gather_grid_blocks(uint64_t n, uint32_t row_bytes) {
 
 cudaError_t launch_gather(const GatherArgs &a, int dtype, cudaStream_t st) {
     if (a.n == 0) return cudaSuccess;
+    if (dtype == AG_F8) {
+        const dim3 grid(gather_grid_blocks(a.n, a.row_bytes), 1);
+        return a.dim % 4 == 0 && (uintptr_t)a.out % 16 == 0 ? launch_f8<true>(a, nullptr, a.row_bytes, grid, st)
+                                                            : launch_f8<false>(a, nullptr, a.row_bytes, grid, st);
+    }
     const bool vec_ok = (a.row_bytes % 16 == 0) && (((uintptr_t)a.payload) % 16 == 0) &&
                         (((uintptr_t)a.out) % 16 == 0);
     if (vec_ok) {
@@ -1115,6 +1188,11 @@ cudaError_t launch_gather_group(const GatherArgs *group_dev, uint32_t n_batches,
                                 cudaStream_t st, bool chained) {
     if (n_batches == 0 || n_bound == 0) return cudaSuccess;
     GatherArgs none{};
+    if (dtype == AG_F8) {
+        const dim3 grid(std::min(gather_grid_blocks(n_bound, row_bytes), std::max(1, (kSMs * 64 + (int)n_batches - 1) / (int)n_batches)), n_batches);
+        return dim % 4 == 0 && aligned ? launch_f8<true>(none, group_dev, row_bytes, grid, st)
+                                       : launch_f8<false>(none, group_dev, row_bytes, grid, st);
+    }
     if (row_bytes % 16 == 0 && aligned) {
         // n_bound is the caller's estimate of the rows per batch (the true count is
         // read on the device); a batch with more rows strides over extra chunks.

@@ -1075,8 +1075,9 @@ int32_t hetero_group_into(ag_hetero_sampler *s, uint32_t n_batches, uint32_t see
             if (!any[t]) continue;
             const uint64_t bound = std::min<uint64_t>(s->max_nodes, m.type_nodes[t]);
             rows[t] = std::max<uint64_t>(s->est_nodes ? std::min(bound, s->est_type[t]) : bound / 4, 1);
-            row_bytes[t] = (uint32_t)(feats[t]->dim * elem_size(feats[t]->dtype));
+            row_bytes[t] = (uint32_t)row_pitch(feats[t]);
             together = together && aligned[t] && row_bytes[t] % 16 == 0 && !feats[t]->shards && feats[t]->dtype != AG_I8 &&
+                       feats[t]->dtype != AG_F8 &&
                        (dtype < 0 || dtype == feats[t]->dtype);
             dtype = feats[t]->dtype;
         }

@@ -80,7 +80,8 @@ struct ag_features {
     uint64_t dim = 0;
     int dtype = AG_F32;
     uint8_t *payload = nullptr;  // device, rows * dim * elem_size
-    float *scales = nullptr;     // device, AG_I8 only: rows * ceil(dim / 32) per-block scales
+    float *scales = nullptr;     // device, AG_I8 / AG_F8 only: scales_per_row() per row
+    uint64_t pitch = 0;          // bytes from row to row where that is not dim * elem_size (AG_F8: a multiple of 16)
     uint32_t *err = nullptr;     // device, 32 bytes: sticky error bits; at +8 / +16 two u64 counters of the
                                  // address-ordered gather (rows asked for, rows actually loaded)
     bool owns_payload = true;
@@ -136,8 +137,13 @@ struct ag_shard_table {
 
 namespace ag {
 
-inline uint32_t elem_size(int dtype) { return dtype == AG_F32 ? 4u : dtype == AG_I8 ? 1u : 2u; }
+inline uint32_t elem_size(int dtype) { return dtype == AG_F32 ? 4u : dtype == AG_I8 || dtype == AG_F8 ? 1u : 2u; }
 constexpr uint32_t kQuantBlock = 32;  // elements per scale of the int8 payload (feature_codec.rs: BlockScaledI8::BLOCK)
+constexpr uint32_t kF8Block = 128;    // columns per scale of 8-bit float rows; weights: 128 x 128
+inline uint64_t row_pitch(const ag_features *f) { return f->pitch ? f->pitch : f->dim * elem_size(f->dtype); }
+inline uint64_t scales_per_row(int dtype, uint64_t dim) {
+    return dtype == AG_I8 ? (dim + kQuantBlock - 1) / kQuantBlock : dtype == AG_F8 ? (dim + kF8Block - 1) / kF8Block : 0;
+}
 
 struct GatherArgs {
     const uint8_t *payload;
@@ -151,13 +157,13 @@ struct GatherArgs {
     uint32_t *err;
     const ag_shard_table *shards;  // non-null: rows are looked up through the shard table
     const uint32_t *ids_off;       // non-null (u32 ids only): the ids start at ids + *ids_off (device value)
-    const float *scales;           // AG_I8 stores: per-block scales
+    const float *scales;           // AG_I8 / AG_F8 stores: per-block scales
 };
 
 // The source half of a gather's arguments, from a feature store handle.
 inline void set_gather_source(GatherArgs &a, const ag_features *f) {
     a.payload = f->payload; a.row_begin = f->row_begin; a.rows = f->rows;
-    a.row_bytes = (uint32_t)(f->dim * elem_size(f->dtype)); a.dim = (uint32_t)f->dim;
+    a.row_bytes = (uint32_t)row_pitch(f); a.dim = (uint32_t)f->dim;
     a.err = f->err; a.shards = f->shards; a.scales = f->scales;
 }
 
@@ -181,6 +187,9 @@ cudaError_t launch_encode(const float *src, void *dst, uint64_t count, int dtype
 // f32 rows -> block-scaled int8 codes + scales; *bad_dev is set when a value is not finite.
 cudaError_t launch_encode_i8(const float *src, uint64_t rows, uint64_t dim, int8_t *codes, float *scales, uint32_t *bad_dev,
                              cudaStream_t st);
+// f32 rows -> e4m3 codes at a pitch of row_pitch bytes + scales; *bad_dev is set when a value is not finite.
+cudaError_t launch_encode_f8(const float *src, uint64_t rows, uint64_t dim, uint64_t pitch, uint8_t *codes, float *scales,
+                             uint32_t *bad_dev, cudaStream_t st);
 int gather_grid_blocks(uint64_t n, uint32_t row_bytes);
 void sampler_set_pipelined(ag_sampler *s);  // other chains run beside this handle's: it gathers on a stream of its own
 int32_t sampler_set_yielding_wait(ag_sampler *s, bool on);  // poll + yield instead of spinning in ag_sample_group_wait

@@ -1,0 +1,669 @@
+// Row operators of a layer over a batch's feature rows: dropout, the root-mean-square norm
+// with the residual's addition (forward and backward), rows and weights in 8-bit floats.
+// No counterpart in the reference, which hands its rows to PyTorch.
+//
+// A row is cut into chunks of eight consecutive columns.  A thread owns a chunk: 16 bytes of
+// f16 / bf16 or 32 bytes of f32 in one load, and exactly the eight 16-bit lots of one Philox4x32-10
+// call, whose counter is (chunk, row, offset) — so a mask is a function of (seed, offset, row,
+// column) alone, whatever the row pitch, launch shape or type, and is made again wherever it is
+// needed instead of being stored.  All sums, statistics and products are held in f32; the one
+// rounding to the rows' type is the store's.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "internal.h"
+
+namespace ag {
+
+namespace {
+
+constexpr uint32_t kChunk = 8;
+constexpr float kE4M3Max = 448.0f;
+constexpr uint32_t kMaxNormDim = 16384;  // 512 threads x 4 chunks
+
+// ------------------------------------------------------------ row access --
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Eight stored elements, before conversion.
+template <typename T> struct Raw { uint32_t w[sizeof(T) * 2]; };
+
+// Plain loads: an in-place call writes what it has read.
+__device__ __forceinline__ void load_words(Raw<float> &r, const void *p) {
+    asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+                 : "l"(p) : "memory");
+}
+template <typename T> __device__ __forceinline__ void load_words(Raw<T> &r, const void *p) {
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void store_words(const Raw<float> &r, void *p) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" :: "l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]),
+                 "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7]) : "memory");
+}
+template <typename T> __device__ __forceinline__ void store_words(const Raw<T> &r, void *p) {
+    asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};" :: "l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]) : "memory");
+}
+
+// Columns c .. c + 7 of a row of `dim`; what lies past its end reads as zeros.  VEC: rows start on
+// multiples of eight elements' bytes.
+template <typename T, bool VEC> __device__ __forceinline__ Raw<T> load_chunk(const T *row, uint32_t c, uint32_t dim) {
+    Raw<T> r;
+    if (VEC && c + kChunk <= dim) {
+        load_words(r, row + c);
+    } else {
+        T e[kChunk];
+#pragma unroll
+        for (uint32_t i = 0; i < kChunk; ++i) e[i] = c + i < dim ? row[c + i] : from_f32<T>(0.f);
+        memcpy(&r, e, sizeof r);
+    }
+    return r;
+}
+template <typename T> __device__ __forceinline__ void unpack(const Raw<T> &r, float v[kChunk]) {
+    T e[kChunk];
+    memcpy(e, &r, sizeof r);
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk; ++i) v[i] = to_f32(e[i]);
+}
+template <typename T, bool VEC> __device__ __forceinline__ void store_chunk(T *row, uint32_t c, uint32_t dim, const float v[kChunk]) {
+    T e[kChunk];
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk; ++i) e[i] = from_f32<T>(v[i]);
+    if (VEC && c + kChunk <= dim) {
+        Raw<T> r;
+        memcpy(&r, e, sizeof r);
+        store_words(r, row + c);
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kChunk; ++i)
+            if (c + i < dim) row[c + i] = e[i];
+    }
+}
+// The norm's weights: the rows' type or f32, any alignment, the same few for every row (L1).
+template <typename T> __device__ __forceinline__ void load_weight(const void *w, int w_f32, uint32_t c, uint32_t dim, float v[kChunk]) {
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk; ++i)
+        v[i] = !w ? 1.f : c + i >= dim ? 0.f : w_f32 ? __ldg((const float *)w + c + i) : to_f32(((const T *)w)[c + i]);
+}
+
+// ---------------------------------------------------------------- dropout --
+struct Drop {
+    uint32_t threshold;  // an element stays iff its 16 random bits are at least this; 0: no dropout, 65536: nothing stays
+    float scale;
+    uint64_t seed, offset;
+};
+
+__device__ __forceinline__ void drop_chunk(const Drop &d, uint64_t row, uint32_t chunk, float v[kChunk]) {
+    const uint4 r = philox4x32_10(d.seed, (uint32_t)d.offset, row << 32 | chunk, (uint32_t)(d.offset >> 32));
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk; ++i) {
+        const uint32_t u = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu;
+        v[i] = u >= d.threshold ? v[i] * d.scale : 0.f;  // a select: a dropped infinity or NaN is gone
+    }
+}
+
+constexpr int kThreads = 256;
+
+// A thread per chunk.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads)
+k_dropout(const T *x, T *y, uint64_t rows, uint32_t dim, uint64_t x_stride, uint64_t y_stride, Drop d) {
+    const uint32_t chunks = (dim + kChunk - 1) / kChunk;
+    const uint64_t total = rows * chunks;
+    for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < total; i += (uint64_t)gridDim.x * kThreads) {
+        const uint64_t row = i / chunks;
+        const uint32_t chunk = (uint32_t)(i - row * chunks);
+        float v[kChunk];
+        unpack(load_chunk<T, VEC>(x + row * x_stride, chunk * kChunk, dim), v);
+        drop_chunk(d, row, chunk, v);
+        store_chunk<T, VEC>(y + row * y_stride, chunk * kChunk, dim, v);
+    }
+}
+
+// ------------------------------------------------------------------- norm --
+struct NormArgs {
+    const void *x, *res, *weight;
+    void *y, *h;
+    float *rstd;
+    uint8_t *codes;  // 8-bit output instead of y
+    float *scales;
+    uint64_t rows, x_stride, res_stride, y_stride, h_stride, code_stride;
+    uint32_t dim;
+    int w_f32, plain;  // plain: no norm, the rows themselves are encoded
+    float eps;
+    Drop drop;
+};
+
+// Sum over the `lanes` (power of two, at most 32) of a row's group, or over the whole block.
+template <bool BLOCK> __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float *shared) {
+    for (uint32_t o = (BLOCK ? 32 : lanes) / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (BLOCK) {
+        __syncthreads();  // the previous row's sum has been read
+        if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.f;
+        for (uint32_t i = 0; i < blockDim.x / 32; ++i) v += shared[i];
+    }
+    return v;
+}
+
+// e4m3 codes and scale of a row's block of 128 columns: the 16 chunks that hold it are the
+// consecutive lanes `lanes` wide.  The scale puts the block's largest magnitude on 448; a block
+// with an infinity or NaN gets a NaN scale, so that every value read from it is NaN.  Magnitudes
+// are compared as bits: NaN above infinity above every number.
+__device__ __forceinline__ void encode_chunk(const float v[kChunk], uint32_t lanes, uint32_t c, uint32_t dim, uint8_t *row_codes,
+                                             float *row_scales) {
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    for (uint32_t o = min(lanes, kF8Block / kChunk) / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (c >= dim) return;
+    const bool bad = top >= 0x7F800000u;
+    // The least normal f32 at least, so that its reciprocal is finite.  The reciprocal is rounded
+    // once and the product once more: a code is off by half a step and 2^-23 of the value.
+    const float scale = bad ? __uint_as_float(0x7FC00000u) : fmaxf(__uint_as_float(top) / kE4M3Max, 1.17549435e-38f);
+    const float inv = bad ? 0.f : 1.f / scale;
+    if (c % kF8Block == 0) row_scales[c / kF8Block] = scale;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk; i += 2)
+        w[i >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[i] * inv, v[i + 1] * inv), __NV_SATFINITE, __NV_E4M3) << (8 * (i & 3));
+    if (bad) w[0] = w[1] = 0;
+    // The pitch is a multiple of 16 bytes, so the padding takes what a last chunk writes past the row.
+    *(uint2 *)(row_codes + c) = make_uint2(w[0], w[1]);
+}
+
+// h = res + dropout(x); y = h rsqrt(mean(h^2) + eps) w.  `lanes` lanes a row (BLOCK: the whole
+// block), C chunks each; the row stays in registers between the sum and the output.
+template <typename T, bool VEC, int C, bool BLOCK, bool F8>
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads)
+k_norm(NormArgs a, uint32_t lanes) {
+    __shared__ float shared[32];
+    const uint32_t lane = BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
+    const uint32_t width = BLOCK ? blockDim.x : lanes;
+    const uint64_t per_block = blockDim.x / width;
+    for (uint64_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block) {
+        const uint64_t row = base + (BLOCK ? 0 : threadIdx.x / lanes);
+        const bool in = row < a.rows;  // the others still take part in the shuffles
+        float v[C][kChunk];
+        Raw<T> rx[C], rr[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const uint32_t c = (lane + j * width) * kChunk;
+            const uint32_t end = in ? a.dim : 0;
+            if (c < end) {
+                rx[j] = load_chunk<T, VEC>((const T *)a.x + row * a.x_stride, c, end);
+                if (a.res) rr[j] = load_chunk<T, VEC>((const T *)a.res + row * a.res_stride, c, end);
+            }
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const uint32_t chunk = lane + j * width, c = chunk * kChunk;
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i) v[j][i] = 0.f;
+            if (in && c < a.dim) {
+                unpack(rx[j], v[j]);
+                if (a.drop.threshold) drop_chunk(a.drop, row, chunk, v[j]);
+                if (a.res) {
+                    float r[kChunk];
+                    unpack(rr[j], r);
+#pragma unroll
+                    for (uint32_t i = 0; i < kChunk; ++i) v[j][i] += r[i];
+                }
+                if (a.h) store_chunk<T, VEC>((T *)a.h + row * a.h_stride, c, a.dim, v[j]);
+#pragma unroll
+                for (uint32_t i = 0; i < kChunk; ++i) sum += v[j][i] * v[j][i];
+            }
+        }
+        if (!a.plain) {
+            const float rstd = rsqrtf(row_sum<BLOCK>(sum, lanes, shared) / (float)a.dim + a.eps);
+            if (a.rstd && in && lane == 0) a.rstd[row] = rstd;
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                float w[kChunk];
+                load_weight<T>(a.weight, a.w_f32, (lane + j * width) * kChunk, a.dim, w);
+#pragma unroll
+                for (uint32_t i = 0; i < kChunk; ++i) v[j][i] *= rstd * w[i];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const uint32_t c = (lane + j * width) * kChunk, end = in ? a.dim : 0;
+            if (F8) {
+                encode_chunk(v[j], lanes, c, end, a.codes + row * a.code_stride, a.scales + row * ((a.dim + kF8Block - 1) / kF8Block));
+            } else if (c < end) {
+                store_chunk<T, VEC>((T *)a.y + row * a.y_stride, c, end, v[j]);
+            }
+        }
+    }
+}
+
+struct NormBackArgs {
+    const void *dy, *dh, *h, *weight;
+    const float *rstd;
+    void *dx, *dres;
+    float *partial;  // [blocks, dim] sums of dy h rstd over a block's rows, or null
+    uint64_t rows, dy_stride, dh_stride, h_stride;
+    uint32_t dim;
+    int w_f32;
+    Drop drop;
+};
+
+// g = dy w; t = dh + rstd g - h rstd^3 / dim sum(g h): the gradient of h and of the residual; dx = dropout(t).
+// dw = sum over rows of dy h rstd: a thread's columns are the same in every row, so it keeps their
+// sums; a block adds its lane groups in order into its row of `partial`, and k_norm_dw adds those.
+// No atomics: the same bits every time on the same GPU.
+template <typename T, bool VEC, int C, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads)
+k_norm_back(NormBackArgs a, uint32_t lanes) {
+    __shared__ float shared[32];
+    extern __shared__ float sums[];  // [groups of the block][dim], not BLOCK
+    const uint32_t lane = BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
+    const uint32_t width = BLOCK ? blockDim.x : lanes;
+    const uint64_t per_block = blockDim.x / width;
+    float dw[C][kChunk];
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < kChunk; ++i) dw[j][i] = 0.f;
+    for (uint64_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block) {
+        const uint64_t row = base + (BLOCK ? 0 : threadIdx.x / lanes);
+        const bool in = row < a.rows;
+        const uint32_t end = in ? a.dim : 0;
+        Raw<T> ry[C], rh[C], rd[C];
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const uint32_t c = (lane + j * width) * kChunk;
+            if (c < end) {
+                rh[j] = load_chunk<T, VEC>((const T *)a.h + row * a.h_stride, c, end);
+                if (a.dy) ry[j] = load_chunk<T, VEC>((const T *)a.dy + row * a.dy_stride, c, end);
+                if (a.dh) rd[j] = load_chunk<T, VEC>((const T *)a.dh + row * a.dh_stride, c, end);
+            }
+        }
+        const float rstd = in ? a.rstd[row] : 0.f;
+        float g[C][kChunk], h[C][kChunk], sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const uint32_t c = (lane + j * width) * kChunk;
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i) g[j][i] = h[j][i] = 0.f;
+            if (c < end) {
+                unpack(rh[j], h[j]);
+                if (a.dy) {
+                    float w[kChunk];
+                    unpack(ry[j], g[j]);
+                    load_weight<T>(a.weight, a.w_f32, c, end, w);
+#pragma unroll
+                    for (uint32_t i = 0; i < kChunk; ++i) {
+                        dw[j][i] += g[j][i] * (h[j][i] * rstd);
+                        g[j][i] *= w[i];
+                        sum += g[j][i] * h[j][i];
+                    }
+                }
+            }
+        }
+        const float coef = row_sum<BLOCK>(sum, lanes, shared) * rstd * rstd * rstd / (float)a.dim;
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+            const uint32_t chunk = lane + j * width, c = chunk * kChunk;
+            if (c >= end) continue;
+            float t[kChunk];
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i) t[i] = rstd * g[j][i] - h[j][i] * coef;
+            if (a.dh) {
+                float d[kChunk];
+                unpack(rd[j], d);
+#pragma unroll
+                for (uint32_t i = 0; i < kChunk; ++i) t[i] += d[i];
+            }
+            if (a.dres) store_chunk<T, VEC>((T *)a.dres + row * a.dim, c, end, t);
+            if (a.dx) {
+                if (a.drop.threshold) drop_chunk(a.drop, row, chunk, t);
+                store_chunk<T, VEC>((T *)a.dx + row * a.dim, c, end, t);
+            }
+        }
+    }
+    if (!a.partial) return;
+    float *mine = a.partial + (uint64_t)blockIdx.x * a.dim;
+    if (BLOCK) {
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i) {
+                const uint32_t c = (lane + j * width) * kChunk + i;
+                if (c < a.dim) mine[c] = dw[j][i];
+            }
+    } else {
+        const uint32_t group = threadIdx.x / lanes;
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i) {
+                const uint32_t c = (lane + j * width) * kChunk + i;
+                if (c < a.dim) sums[group * a.dim + c] = dw[j][i];
+            }
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
+            float s = 0.f;
+            for (uint32_t q = 0; q < per_block; ++q) s += sums[q * a.dim + c];
+            mine[c] = s;
+        }
+    }
+}
+
+// dw[c] = sum of the blocks' partial sums, 32 columns a block, 16 slices of blocks each.
+template <typename T>
+__global__ void __launch_bounds__(512)
+k_norm_dw(const float *partial, uint32_t blocks, uint32_t dim, T *dw) {
+    __shared__ float sums[16][32];
+    const uint32_t c = blockIdx.x * 32 + threadIdx.x;
+    float s = 0.f;
+    if (c < dim)
+        for (uint32_t b = threadIdx.y; b < blocks; b += 16) s += partial[(uint64_t)b * dim + c];
+    sums[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < dim) {
+        s = 0.f;
+        for (int q = 0; q < 16; ++q) s += sums[q][threadIdx.x];
+        dw[c] = from_f32<T>(s);
+    }
+}
+
+// ---------------------------------------------------- weights in 8 bits --
+// A block of 128 x 128 weights per thread block: its largest magnitude, then the codes.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+k_encode_weight(const T *w, uint64_t out, uint32_t dim, uint64_t stride, uint8_t *codes, uint64_t code_stride, float *scales) {
+    __shared__ uint32_t peak;
+    if (threadIdx.x == 0) peak = 0;
+    __syncthreads();
+    const uint32_t blocks_per_row = (dim + kF8Block - 1) / kF8Block;
+    const uint32_t bk = blockIdx.x % blocks_per_row;
+    const uint64_t bn = blockIdx.x / blocks_per_row;
+    uint32_t top = 0;
+    for (uint32_t i = threadIdx.x; i < kF8Block * kF8Block; i += kThreads) {
+        const uint64_t n = bn * kF8Block + i / kF8Block;
+        const uint32_t c = bk * kF8Block + i % kF8Block;
+        if (n < out && c < dim) top = max(top, __float_as_uint(to_f32(w[n * stride + c])) & 0x7FFFFFFFu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) atomicMax(&peak, top);
+    __syncthreads();
+    top = peak;
+    const bool bad = top >= 0x7F800000u;
+    const float scale = bad ? __uint_as_float(0x7FC00000u) : fmaxf(__uint_as_float(top) / kE4M3Max, 1.17549435e-38f);
+    const float inv = bad ? 0.f : 1.f / scale;
+    if (threadIdx.x == 0) scales[blockIdx.x] = scale;
+    for (uint32_t i = threadIdx.x; i < kF8Block * kF8Block; i += kThreads) {
+        const uint64_t n = bn * kF8Block + i / kF8Block;
+        const uint32_t c = bk * kF8Block + i % kF8Block;
+        if (n < out && c < dim)
+            codes[n * code_stride + c] = bad ? 0 : (uint8_t)__nv_cvt_float_to_fp8(to_f32(w[n * stride + c]) * inv, __NV_SATFINITE, __NV_E4M3);
+    }
+}
+
+// --------------------------------------------------------------- launches --
+// Whether every row of a tensor starts on a multiple of eight elements' bytes.
+bool vec_rows(const void *p, uint64_t stride, uint32_t elem) {
+    return !p || ((uintptr_t)p % (kChunk * elem) == 0 && stride % kChunk == 0);
+}
+
+template <typename F> void with_type(int dtype, F f) {
+    if (dtype == AG_F32) f((float *)nullptr);
+    else if (dtype == AG_F16) f((__half *)nullptr);
+    else f((__nv_bfloat16 *)nullptr);
+}
+
+int32_t make_drop(double p, uint64_t seed, uint64_t offset, Drop *d) {
+    if (!(p >= 0.0 && p <= 1.0)) return fail(AG_ERR_VALUE, "dropout probability must be in [0, 1], got %g", p);
+    d->threshold = (uint32_t)std::floor(p * 65536.0 + 0.5);
+    d->scale = d->threshold < 65536 ? 65536.0f / (65536 - d->threshold) : 0.0f;
+    d->seed = seed; d->offset = offset;
+    return AG_OK;
+}
+
+int32_t check_rows(const char *who, uint64_t rows, uint64_t dim, int32_t dtype) {
+    if (dtype < AG_F32 || dtype > AG_BF16) return fail(AG_ERR_VALUE, "%s: rows are f32, f16 or bf16, got dtype tag %d", who, dtype);
+    if (rows > 0xFFFFFFFFull) return fail(AG_ERR_VALUE, "%s: at most 2^32 - 1 rows, got %llu", who, (unsigned long long)rows);
+    if (dim == 0 || dim > 0xFFFFFFF0ull) return fail(AG_ERR_VALUE, "%s: rows of 1 to 2^32 - 16 columns, got %llu", who, (unsigned long long)dim);
+    return AG_OK;
+}
+
+// How a row of `dim` columns is shared out: lanes (0: a whole block of `threads`) and chunks a lane.
+struct Split { uint32_t lanes, threads; int chunks; };
+Split split_row(uint32_t dim) {
+    const uint32_t n = (dim + kChunk - 1) / kChunk;
+    Split s{1, kThreads, 1};
+    if (n <= 128) {
+        while (s.lanes < 32 && s.lanes < n) s.lanes *= 2;
+        while ((uint32_t)s.chunks * s.lanes < n) s.chunks *= 2;
+    } else {
+        s.lanes = 0;
+        s.threads = 128;
+        while (s.threads < 512 && s.threads * 2 < n) s.threads *= 2;
+        while ((uint32_t)s.chunks * s.threads < n) s.chunks *= 2;
+    }
+    return s;
+}
+
+template <typename T, bool VEC, bool F8>
+cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
+    const Split s = split_row(a.dim);
+    const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>((a.rows + per - 1) / per, 1u << 30), lanes = s.lanes ? s.lanes : 32;
+    if (s.lanes) {
+        if (s.chunks == 1) k_norm<T, VEC, 1, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+        else if (s.chunks == 2) k_norm<T, VEC, 2, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+        else k_norm<T, VEC, 4, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+    } else {
+        if (s.chunks == 1) k_norm<T, VEC, 1, true, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+        else if (s.chunks == 2) k_norm<T, VEC, 2, true, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+        else k_norm<T, VEC, 4, true, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+    }
+    return cudaGetLastError();
+}
+
+uint32_t back_blocks(uint64_t rows, uint32_t dim) {
+    const Split s = split_row(dim);
+    const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
+    return (uint32_t)std::min<uint64_t>((rows + per - 1) / per, (uint64_t)kSMs * (2048 / s.threads) / 2);
+}
+
+template <typename T, bool VEC, int C, bool BLOCK>
+cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t grid, cudaStream_t st) {
+    const size_t shared = BLOCK || !a.partial ? 0 : (size_t)(s.threads / s.lanes) * a.dim * 4;
+    k_norm_back<T, VEC, C, BLOCK><<<grid, s.threads, shared, st>>>(a, s.lanes ? s.lanes : 32);
+    return cudaGetLastError();
+}
+
+template <typename T, bool VEC>
+cudaError_t launch_back(const NormBackArgs &a, uint32_t grid, cudaStream_t st) {
+    const Split s = split_row(a.dim);
+    if (s.lanes) {
+        if (s.chunks == 1) return launch_back<T, VEC, 1, false>(a, s, grid, st);
+        if (s.chunks == 2) return launch_back<T, VEC, 2, false>(a, s, grid, st);
+        return launch_back<T, VEC, 4, false>(a, s, grid, st);
+    }
+    if (s.chunks == 1) return launch_back<T, VEC, 1, true>(a, s, grid, st);
+    if (s.chunks == 2) return launch_back<T, VEC, 2, true>(a, s, grid, st);
+    return launch_back<T, VEC, 4, true>(a, s, grid, st);
+}
+
+}  // namespace
+
+}  // namespace ag
+
+namespace ag {
+
+namespace {
+__global__ void k_scales_bad(const float *scales, uint64_t n, uint32_t *bad) {
+    for (uint64_t i = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x; i < n; i += (uint64_t)gridDim.x * blockDim.x)
+        if (isnan(scales[i])) *bad = 1;
+}
+
+// A row a block, for rows of any length; encode_chunk does the work.
+__global__ void __launch_bounds__(kThreads)
+k_encode_rows(const float *src, uint64_t rows, uint32_t dim, uint64_t pitch, uint8_t *codes, float *scales) {
+    const uint64_t per_row = (dim + kF8Block - 1) / kF8Block;
+    for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x)
+        for (uint32_t c0 = 0; c0 < dim; c0 += kThreads * kChunk) {
+            const uint32_t c = c0 + threadIdx.x * kChunk;
+            float v[kChunk];
+            unpack(load_chunk<float, false>(src + row * dim, c, dim), v);
+            encode_chunk(v, 32, c, dim, codes + row * pitch, scales + row * per_row);
+        }
+}
+}  // namespace
+
+cudaError_t launch_encode_f8(const float *src, uint64_t rows, uint64_t dim, uint64_t pitch, uint8_t *codes, float *scales,
+                             uint32_t *bad_dev, cudaStream_t st) {
+    k_encode_rows<<<(uint32_t)std::min<uint64_t>(rows, 1u << 20), kThreads, 0, st>>>(src, rows, (uint32_t)dim, pitch, codes, scales);
+    k_scales_bad<<<(uint32_t)kSMs * 4, kThreads, 0, st>>>(scales, rows * ((dim + kF8Block - 1) / kF8Block), bad_dev);
+    return cudaGetLastError();
+}
+
+}  // namespace ag
+
+using namespace ag;
+
+extern "C" int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64_t dim, uint64_t x_stride, uint64_t y_stride,
+                                   int32_t dtype, double p, uint64_t seed, uint64_t offset, int32_t device, void *stream) {
+    AG_TRY(check_rows("ag_rows_dropout", rows, dim, dtype));
+    Drop d;
+    AG_TRY(make_drop(p, seed, offset, &d));
+    if (rows == 0) return AG_OK;
+    if (!x || !y) return fail(AG_ERR_VALUE, "ag_rows_dropout: null argument");
+    if (y_stride < dim) return fail(AG_ERR_VALUE, "ag_rows_dropout: rows of the output overlap");
+    DeviceGuard guard(device);
+    if (!guard.ok) return AG_ERR_CUDA;
+    const uint64_t chunks = rows * ((dim + kChunk - 1) / kChunk);
+    const uint32_t grid = (uint32_t)std::min<uint64_t>((chunks + kThreads - 1) / kThreads, 1u << 30);
+    const bool vec = vec_rows(x, x_stride, elem_size(dtype)) && vec_rows(y, y_stride, elem_size(dtype));
+    with_type(dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (vec) k_dropout<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, rows, (uint32_t)dim, x_stride, y_stride, d);
+        else k_dropout<T, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, rows, (uint32_t)dim, x_stride, y_stride, d);
+    });
+    AG_CUDA(cudaGetLastError());
+    return AG_OK;
+}
+
+extern "C" int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream) {
+    if (!n) return fail(AG_ERR_VALUE, "ag_rows_norm: null argument");
+    AG_TRY(check_rows("ag_rows_norm", n->rows, n->dim, n->dtype));
+    if (n->dim > kMaxNormDim) return fail(AG_ERR_VALUE, "ag_rows_norm: at most %u columns, got %llu", kMaxNormDim, (unsigned long long)n->dim);
+    if (n->weight && n->weight_dtype != n->dtype && n->weight_dtype != AG_F32)
+        return fail(AG_ERR_VALUE, "ag_rows_norm: the weights are f32 or of the rows' type");
+    NormArgs a{};
+    AG_TRY(make_drop(n->p, n->seed, n->offset, &a.drop));
+    if (n->rows == 0) return AG_OK;
+    if (!n->x || (!n->y && !n->codes) || (n->codes && !n->scales)) return fail(AG_ERR_VALUE, "ag_rows_norm: null argument");
+    if (n->y && n->codes) return fail(AG_ERR_VALUE, "ag_rows_norm: either rows of their own type or 8-bit rows come out");
+    if (n->encode_only && (!n->codes || n->residual || n->weight || n->h || a.drop.threshold))
+        return fail(AG_ERR_VALUE, "ag_rows_norm: encoding alone takes rows and gives 8-bit rows");
+    if (n->codes && (n->code_stride % 16 != 0 || n->code_stride < n->dim || (uintptr_t)n->codes % 16 != 0))
+        return fail(AG_ERR_VALUE, "ag_rows_norm: 8-bit rows start on multiples of 16 bytes and do not overlap");
+    if ((n->y && n->y_stride < n->dim) || (n->h && n->h_stride < n->dim)) return fail(AG_ERR_VALUE, "ag_rows_norm: rows of the output overlap");
+    DeviceGuard guard(device);
+    if (!guard.ok) return AG_ERR_CUDA;
+    a.x = n->x; a.res = n->residual; a.weight = n->weight; a.y = n->y; a.h = n->h; a.rstd = n->rstd;
+    a.codes = (uint8_t *)n->codes; a.scales = n->scales; a.rows = n->rows; a.x_stride = n->x_stride; a.res_stride = n->residual_stride;
+    a.y_stride = n->y_stride; a.h_stride = n->h_stride; a.code_stride = n->code_stride; a.dim = (uint32_t)n->dim;
+    a.w_f32 = n->weight_dtype == AG_F32; a.plain = n->encode_only; a.eps = n->eps;
+    const uint32_t e = elem_size(n->dtype);
+    const bool vec = vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.y, a.y_stride, e) && vec_rows(a.h, a.h_stride, e);
+    cudaError_t err = cudaSuccess;
+    with_type(n->dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        cudaStream_t st = (cudaStream_t)stream;
+        if (a.codes) err = vec ? launch_norm<T, true, true>(a, st) : launch_norm<T, false, true>(a, st);
+        else err = vec ? launch_norm<T, true, false>(a, st) : launch_norm<T, false, false>(a, st);
+    });
+    AG_CUDA(err);
+    return AG_OK;
+}
+
+extern "C" int32_t ag_rows_norm_backward_scratch(uint64_t rows, uint64_t dim, int32_t device, uint64_t *bytes) {
+    if (!bytes) return fail(AG_ERR_VALUE, "ag_rows_norm_backward_scratch: null argument");
+    *bytes = 0;
+    if (rows == 0 || dim == 0 || dim > kMaxNormDim) return AG_OK;
+    DeviceGuard guard(device);
+    if (!guard.ok) return AG_ERR_CUDA;
+    *bytes = (uint64_t)back_blocks(rows, (uint32_t)dim) * dim * 4;
+    return AG_OK;
+}
+
+extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, void *stream) {
+    if (!n) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: null argument");
+    AG_TRY(check_rows("ag_rows_norm_backward", n->rows, n->dim, n->dtype));
+    if (n->dim > kMaxNormDim) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: at most %u columns, got %llu", kMaxNormDim, (unsigned long long)n->dim);
+    if (n->weight && n->weight_dtype != n->dtype && n->weight_dtype != AG_F32)
+        return fail(AG_ERR_VALUE, "ag_rows_norm_backward: the weights are f32 or of the rows' type");
+    NormBackArgs a{};
+    AG_TRY(make_drop(n->p, n->seed, n->offset, &a.drop));
+    DeviceGuard guard(device);
+    if (!guard.ok) return AG_ERR_CUDA;
+    if (n->rows == 0) {
+        if (n->dw) AG_CUDA(cudaMemsetAsync(n->dw, 0, n->dim * elem_size(n->weight_dtype), (cudaStream_t)stream));
+        return AG_OK;
+    }
+    if (!n->h || !n->rstd || (n->dw && !n->scratch)) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: null argument");
+    const uint32_t grid = back_blocks(n->rows, (uint32_t)n->dim);
+    if (n->dw && n->scratch_bytes < (uint64_t)grid * n->dim * 4)
+        return fail(AG_ERR_VALUE, "ag_rows_norm_backward: %llu bytes of scratch, %llu are needed", (unsigned long long)n->scratch_bytes,
+                    (unsigned long long)grid * n->dim * 4);
+    a.dy = n->dy; a.dh = n->dh; a.h = n->h; a.weight = n->weight; a.rstd = n->rstd; a.dx = n->dx; a.dres = n->dresidual;
+    a.partial = n->dw ? (float *)n->scratch : nullptr;
+    a.rows = n->rows; a.dim = (uint32_t)n->dim; a.dy_stride = n->dy_stride; a.dh_stride = n->dh_stride; a.h_stride = n->h_stride;
+    a.w_f32 = n->weight_dtype == AG_F32;
+    const uint32_t e = elem_size(n->dtype);
+    const bool vec = vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
+                     vec_rows(a.dx, a.dim, e) && vec_rows(a.dres, a.dim, e);
+    cudaError_t err = cudaSuccess;
+    with_type(n->dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        err = vec ? launch_back<T, true>(a, grid, (cudaStream_t)stream) : launch_back<T, false>(a, grid, (cudaStream_t)stream);
+    });
+    AG_CUDA(err);
+    if (n->dw)
+        with_type(n->weight_dtype, [&](auto *t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            k_norm_dw<T><<<((uint32_t)n->dim + 31) / 32, dim3(32, 16), 0, (cudaStream_t)stream>>>((const float *)n->scratch, grid, (uint32_t)n->dim, (T *)n->dw);
+        });
+    AG_CUDA(cudaGetLastError());
+    return AG_OK;
+}
+
+extern "C" int32_t ag_rows_encode_weight(const void *w, uint64_t out, uint64_t dim, uint64_t stride, int32_t dtype, void *codes,
+                                         uint64_t code_stride, float *scales, int32_t device, void *stream) {
+    AG_TRY(check_rows("ag_rows_encode_weight", out, dim, dtype));
+    if (out == 0) return AG_OK;
+    if (!w || !codes || !scales) return fail(AG_ERR_VALUE, "ag_rows_encode_weight: null argument");
+    if (code_stride % 16 != 0 || code_stride < dim || (uintptr_t)codes % 16 != 0)
+        return fail(AG_ERR_VALUE, "ag_rows_encode_weight: 8-bit rows start on multiples of 16 bytes and do not overlap");
+    const uint64_t blocks = (out + kF8Block - 1) / kF8Block * ((dim + kF8Block - 1) / kF8Block);
+    if (blocks > 0x7FFFFFFFull) return fail(AG_ERR_VALUE, "ag_rows_encode_weight: too many weights");
+    DeviceGuard guard(device);
+    if (!guard.ok) return AG_ERR_CUDA;
+    with_type(dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        k_encode_weight<T><<<(uint32_t)blocks, kThreads, 0, (cudaStream_t)stream>>>((const T *)w, out, (uint32_t)dim, stride, (uint8_t *)codes,
+                                                                                      code_stride, scales);
+    });
+    AG_CUDA(cudaGetLastError());
+    return AG_OK;
+}

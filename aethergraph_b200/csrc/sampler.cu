@@ -1814,7 +1814,7 @@ int32_t launch_saved_impl(ag_sampler *s, bool relaunch) {
         bool aligned = ((uintptr_t)feats->payload % 16) == 0;
         for (uint32_t b = 0; b < n_batches; ++b) aligned = aligned && ((uintptr_t)bufs[b].x % 16) == 0;
         const uint64_t rows = s->est_nodes ? std::min(b_nodes, s->est_nodes) : b_nodes;
-        const uint32_t row_bytes = (uint32_t)(feats->dim * elem_size(feats->dtype));
+        const uint32_t row_bytes = (uint32_t)row_pitch(feats);
         const bool sorted = sorted_gather_applies(feats, row_bytes, aligned);
         // Rows of a sharded store are fetched in address order, each distinct row of the chain
         // once.  Making and sorting the keys is small, latency-bound work like the sampling

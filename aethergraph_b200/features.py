@@ -80,11 +80,12 @@ class FeatureStore:
         `"i8"` is the reference's block-scaled int8 codec (one byte per element and one f32
         scale per 32 elements of a row, crates/aethergraph-core/src/internal/feature_codec.rs):
         lossy, a quarter of f32's bytes; gathers decode to exactly what the reference's
-        `BlockScaledI8::decode` gives."""
+        `BlockScaledI8::decode` gives.  `"f8"` keeps 8-bit floats (e4m3, one f32 scale per 128
+        elements of a row), which `project` multiplies without decoding them first."""
         import torch
 
         if dtype not in _lib.DTYPE_TAG:
-            raise ValueError(f"Invalid dtype '{dtype}'. Must be 'f32', 'f16', 'bf16', or 'i8'")
+            raise ValueError(f"Invalid dtype '{dtype}'. Must be 'f32', 'f16', 'bf16', 'i8' or 'f8'")
         out = C.c_void_p()
         dev = FeatureStore._dev(device)
         if isinstance(features, torch.Tensor):
@@ -114,6 +115,24 @@ class FeatureStore:
                                                       _lib.DTYPE_TAG[dtype], _lib.AG_MEM_HOST,
                                                       FeatureStore._dev(device), C.byref(out)))
         return FeatureStore(out.value)
+
+    @staticmethod
+    def from_f8(codes, scales) -> "FeatureStore":
+        """A store over 8-bit rows (`ops.encode_f8`, `ops.add_rms_norm_f8`) where they are: what a
+        layer has written becomes the next layer's features.  The store keeps both tensors; waits
+        for the current stream, on which they were written."""
+        import torch
+
+        from . import ops
+
+        ops._check_f8(codes, scales, "codes", 1)
+        torch.cuda.current_stream(codes.device).synchronize()
+        out = C.c_void_p()
+        _lib.check(_lib.lib().ag_features_from_f8(codes.data_ptr() or None, scales.data_ptr() or None, codes.shape[0], codes.shape[1],
+                                                  codes.stride(0), codes.device.index, C.byref(out)))
+        store = FeatureStore(out.value)
+        store._keep = (codes, scales)
+        return store
 
     # -- shards over the GPUs of one node --------------------------------------
     @staticmethod
@@ -188,16 +207,17 @@ class FeatureStore:
 
     def payload_to_host(self) -> np.ndarray:
         """The stored (encoded) rows held by this handle as a flat host array
-        (float32 for f32 stores, uint16 bit patterns for f16 / bf16)."""
-        kind = {_lib.AG_F32: np.float32, _lib.AG_I8: np.int8}.get(self._dtype, np.uint16)
+        (float32 for f32 stores, uint16 bit patterns for f16 / bf16, int8 and uint8 codes for i8 / f8)."""
+        kind = {_lib.AG_F32: np.float32, _lib.AG_I8: np.int8, _lib.AG_F8: np.uint8}.get(self._dtype, np.uint16)
         out = np.empty(self._rows * self._dim, dtype=kind)
         if out.size:
             _lib.check(_lib.lib().ag_features_copy_to_host(self._h, out.ctypes.data))
         return out
 
     def scales_to_host(self) -> np.ndarray:
-        """`"i8"` stores: the per-block scales, f32 [rows, ceil(dim / 32)]."""
-        out = np.empty((self._rows, (self._dim + 31) // 32), dtype=np.float32)
+        """`"i8"` / `"f8"` stores: the per-block scales, f32 [rows, ceil(dim / 32)] or [rows, ceil(dim / 128)]."""
+        block = 128 if self._dtype == _lib.AG_F8 else 32
+        out = np.empty((self._rows, (self._dim + block - 1) // block), dtype=np.float32)
         if out.size:
             _lib.check(_lib.lib().ag_features_scales_to_host(self._h, out.ctypes.data))
         return out
@@ -216,6 +236,23 @@ class FeatureStore:
         _lib.check(_lib.lib().ag_gather(self._h, ids.data_ptr() if n else None, int(ids.dtype == torch.int64), n,
                                         None, out.data_ptr() if n else None, st))
         return out
+
+    def project(self, ids, weight, weight_scales, bias=None, dtype=None):
+        """Rows `ids` of an `"f8"` store times 8-bit weights (`ops.encode_weight_f8`), plus `bias`:
+        [len(ids), out] in `dtype` (bfloat16 by default).  What `gather` followed by a linear layer
+        computes, without writing the decoded rows: a kernel reads the stored codes by id and multiplies
+        them.  `ids` is a CUDA tensor (int64, or int32 holding u32 ids); one outside the store gives a
+        zero row and an error that `check` raises."""
+        import torch
+
+        from . import ops
+
+        return ops._product(self._f8_rows(), weight, weight_scales, ids, bias, torch.bfloat16 if dtype is None else dtype)
+
+    def _f8_rows(self):
+        codes, scales, pitch = C.c_void_p(), C.c_void_p(), C.c_uint64()
+        _lib.check(_lib.lib().ag_features_f8_rows(self._h, C.byref(codes), C.byref(scales), C.byref(pitch)))
+        return codes.value, scales.value, pitch.value, self._n, self._dim, self._device
 
     def gather_stats(self) -> tuple[int, int, int]:
         """Sharded views: `(rows requested, rows loaded, rows loaded from the local copy of
@@ -251,8 +288,11 @@ class FeatureStore:
         return n.value
 
     def check(self) -> None:
-        """Raise ValueError if a device gather since the last check saw an out-of-range id."""
+        """Raise ValueError if a device gather (or, on the store's GPU, a product) since the last check saw
+        an out-of-range id."""
         _lib.check(_lib.lib().ag_features_check(self._h))
+        if self._dtype == _lib.AG_F8:
+            _lib.check(_lib.lib().ag_rows_check(self._device))
 
     def telemetry(self):
         return None

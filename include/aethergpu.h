@@ -144,7 +144,11 @@ enum { AG_F32 = 0, AG_F16 = 1, AG_BF16 = 2,
         * decode = code * scale (one IEEE multiply: the gather's rows are bit-identical to
         * the reference's BlockScaledI8::decode).  In-memory only (the reference defines no
         * file layout for it): ag_features_from_f32, ag_synth_features.  Not shardable. */
-       AG_I8 = 3 };
+       AG_I8 = 3,
+       /* 8-bit float rows (see "row operators"): e4m3 codes at a pitch that is a multiple of 16 bytes
+        * and one f32 scale per 128 columns; gathers decode code * scale.  In-memory only:
+        * ag_features_from_f32, ag_features_from_f8.  Not shardable. */
+       AG_F8 = 4 };
 
 int32_t ag_features_save(const char *path, const float *features, uint64_t num_nodes,
                          uint64_t dim, int32_t dtype);
@@ -162,6 +166,14 @@ int32_t ag_features_from_f32(const float *features, uint64_t num_nodes, uint64_t
                              int32_t dtype, int32_t mem_kind, int32_t device, ag_features **out);
 int32_t ag_features_adopt_device(void *payload_dev, uint64_t num_nodes, uint64_t dim,
                                  int32_t dtype, int32_t device, ag_features **out);
+/* A store over 8-bit float rows in the caller's device memory (codes at a pitch of code_stride
+ * bytes, scales [num_nodes, ceil(dim / 128)]), which must outlive it; what a layer has written
+ * becomes the next layer's features without a copy.  ag_features_f8_rows: where a store of this
+ * kind keeps its rows, for ag_rows_product. */
+int32_t ag_features_from_f8(const void *codes, const float *scales, uint64_t num_nodes, uint64_t dim,
+                            uint64_t code_stride, int32_t device, ag_features **out);
+int32_t ag_features_f8_rows(const ag_features *f, const void **codes, const float **scales,
+                            uint64_t *code_stride);
 int32_t ag_features_info(const ag_features *f, uint64_t *num_nodes, uint64_t *dim,
                          int32_t *dtype, int32_t *device, uint64_t *row_begin);
 /* The vertex range [row_begin, row_begin + rows) this handle holds. */
@@ -242,7 +254,7 @@ int32_t ag_features_set_gather_order(ag_features *view, int32_t order);
 int32_t ag_graph_hot_vertices(const ag_graph *g, uint64_t max_rows, uint32_t **ids_dev,
                               uint64_t *n_out);
 int32_t ag_features_cache_rows(ag_features *view, const uint32_t *ids_dev, uint64_t n);
-/* AG_I8 stores: the per-block scales (rows x ceil(dim / 32) f32) to host memory. */
+/* AG_I8 / AG_F8 stores: the per-block scales (rows x ceil(dim / 32) or ceil(dim / 128) f32) to host memory. */
 int32_t ag_features_scales_to_host(const ag_features *f, float *scales);
 /* Copies the stored (encoded) rows held by this handle back to host memory. */
 int32_t ag_features_copy_to_host(const ag_features *f, void *payload);
@@ -668,6 +680,89 @@ int32_t ag_hetero_loader_release_batch(ag_hetero_loader *l, ag_hetero_batch *bat
 int32_t ag_hetero_loader_stats_get(const ag_hetero_loader *l, ag_loader_stats *stats);
 int32_t ag_hetero_loader_shutdown(ag_hetero_loader *l);
 void ag_hetero_loader_free(ag_hetero_loader *l);
+
+/* -------------------------------------------------------- row operators --
+ * No counterpart in the reference, which hands its gathered rows to PyTorch: what a
+ * model's layers do to the rows of a batch.  All tensors are device memory of `device`,
+ * rows of `dim` consecutive elements at a pitch of `*_stride` elements; nothing is
+ * allocated, copied to the host or waited for, so every call can be captured into a graph.
+ *
+ * Dropout.  With T = round(65536 p), element (r, c) stays iff 16 random bits u(r, c) >= T and
+ * is then scaled by 65536 / (65536 - T); a dropped one becomes 0, whatever it was.  u comes from
+ * Philox4x32-10 with the counter (c / 8, r, offset's lower, upper 32 bits) and the key `seed`:
+ * of the four words the one numbered (c % 8) / 2, its lower half for even c.  The mask is a
+ * function of (seed, offset, r, c): it is never stored, and the gradient of a dropout is the
+ * same call on the gradient.  x == y is allowed.  At most 2^32 - 1 rows. */
+int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64_t dim, uint64_t x_stride,
+                        uint64_t y_stride, int32_t dtype, double p, uint64_t seed, uint64_t offset,
+                        int32_t device, void *stream);
+/* h = residual + dropout(x);  y = h / sqrt(mean(h^2) + eps) * weight, the mean over the row's
+ * columns (at most 16384), in f32 and rounded once to the rows' type.  Out come y, or codes and
+ * scales (8-bit rows, below), and where not NULL h and 1 / sqrt(..) per row (f32, what the
+ * backward pass needs).  residual and weight may be NULL.  encode_only: no norm, x itself
+ * becomes 8-bit rows.
+ *
+ * 8-bit rows: e4m3 codes, a scale (f32) per 128 columns of a row, value = code * scale; the scale
+ * is max(largest magnitude / 448, 2^-126), NaN for a block that holds an infinity or NaN.
+ * codes: [rows] at a pitch of code_stride bytes, a multiple of 16, base 16-byte aligned; the
+ * bytes between dim and the pitch are undefined.  scales: f32 [rows, ceil(dim / 128)]. */
+typedef struct {
+    const void *x, *residual, *weight;
+    void *y, *h;
+    float *rstd;
+    void *codes;
+    float *scales;
+    uint64_t rows, dim, x_stride, residual_stride, y_stride, h_stride, code_stride;
+    uint64_t seed, offset;
+    double p;
+    float eps;
+    int32_t dtype, weight_dtype; /* weight: f32 or the rows' type */
+    int32_t encode_only;
+} ag_norm;
+int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream);
+/* Gradients of the norm, from dy and dh (the gradients of y and h, either may be NULL), h and
+ * rstd: dresidual = dh + d(norm); dx = dropout(dresidual) with the forward call's mask; dw, of
+ * weight_dtype, the sum over the rows of dy h rstd.  Any of the three may be NULL; dx and
+ * dresidual are contiguous.  dw needs scratch of ag_rows_norm_backward_scratch bytes, which
+ * belongs to the call until it is done; its summation order is fixed. */
+typedef struct {
+    const void *dy, *dh, *h, *weight;
+    const float *rstd;
+    void *dx, *dresidual, *dw, *scratch;
+    uint64_t scratch_bytes;
+    uint64_t rows, dim, dy_stride, dh_stride, h_stride;
+    uint64_t seed, offset;
+    double p;
+    int32_t dtype, weight_dtype;
+} ag_norm_grad;
+int32_t ag_rows_norm_backward_scratch(uint64_t rows, uint64_t dim, int32_t device, uint64_t *bytes);
+int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, void *stream);
+/* Weights [out, dim] as e4m3 codes (pitch as above) with one scale per 128 x 128 block, f32
+ * [ceil(out / 128), ceil(dim / 128)]. */
+int32_t ag_rows_encode_weight(const void *w, uint64_t out, uint64_t dim, uint64_t stride,
+                              int32_t dtype, void *codes, uint64_t code_stride, float *scales,
+                              int32_t device, void *stream);
+/* Product of 8-bit rows with 8-bit weights: out[m, n] = sum over the blocks of 128 columns of
+ * scales[i, block] * weight_scales[n / 128, block] * (codes[i] . weight[n] within the block), plus
+ * bias[n] (f32, may be NULL), in f32, rounded once to out_dtype (f32, f16, bf16).  i = m, or
+ * ids[m] (int64, or u32 ids where ids_are_i64 == 0): the rows of a feature store by id.  An id
+ * outside [0, held) gives a zero row and raises a sticky error that ag_rows_check reports, per
+ * device.  held, out_dim < 2^31. */
+typedef struct {
+    const void *codes;
+    const float *scales;
+    const void *weight;
+    const float *weight_scales;
+    const void *ids;
+    const float *bias;
+    void *out;
+    uint64_t rows, held, dim, out_dim, code_stride, weight_stride, out_stride;
+    int32_t ids_are_i64, out_dtype;
+} ag_product;
+int32_t ag_rows_product(const ag_product *p, int32_t device, void *stream);
+/* AG_ERR_VALUE if any product since the last check saw an id outside its rows
+ * (synchronises the device). */
+int32_t ag_rows_check(int32_t device);
 
 /* ------------------------------------------------------ synthetic inputs --
  * Seeded generators that build test and benchmark inputs directly in HBM
