@@ -1,11 +1,13 @@
 // Product of 8-bit rows (e4m3, a scale per 128 columns of a row) with 8-bit weights (a scale per
 // 128 x 128 block), the rows in order or by id: the gather of a feature store that multiplies
 // what it reads.  No counterpart in the reference.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "common.cuh"
 #include "internal.h"
@@ -61,6 +63,7 @@ __device__ __forceinline__ void load_codes(const uint8_t *row, uint32_t c, uint3
 }
 
 constexpr int kDotThreads = 256, kDotRows = 4;
+constexpr uint64_t kFewRows = 8;
 
 // Few rows: a warp per column of the output and up to kDotRows rows.
 __global__ void __launch_bounds__(kDotThreads)
@@ -97,6 +100,348 @@ k_product_dot(ProductArgs a) {
     }
 }
 
+// ------------------------------------------------------ tensor-core tiles --
+// A tile of 128 rows x BN output columns per turn of a persistent block, K in steps of 128 bytes,
+// which is one scale block: the tensor cores add up the 128 products of a step in f32 in TMEM, and
+// the epilogue warps fold each step into their sums in registers, times the row's and the weights'
+// scale.  Roles: warp 0 loads (TMA, rows by id through tile::gather4), one thread of warp 1 issues
+// tcgen05.mma (K = 32 each) and the commits, warps 4 - 11 read TMEM (a warp can reach only the 32 lanes
+// of its number mod 4, so two warps share a quarter of the rows and split the columns).
+//
+// Every wait is bounded.  A role whose wait runs out marks the block dead and the sticky error
+// word; all roles then leave their loops, copies and multiplications in flight are waited for
+// (bounded too) and TMEM is freed.
+constexpr int kBM = 128, kBK = 128, kAccStages = 4, kTileThreads = 384;
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+
+constexpr int load_stages(int bn) { return bn >= 128 ? 6 : 8; }
+constexpr int stage_bytes(int bn) { return (kBM + bn) * kBK; }
+constexpr int tile_shared(int bn) { return load_stages(bn) * stage_bytes(bn) + 1024 + 256; }
+
+struct TileArgs {
+    ProductArgs p;
+    uint32_t m_tiles, n_tiles;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// Waits for the barrier's phase; false when the block is dead or the time ran out (which marks it dead).
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *dead) {
+    if (mbar_try(bar, parity)) return true;
+    const uint64_t until = now_ns() + kWaitLimitNs;
+    for (;;) {
+        if (mbar_try(bar, parity)) return true;
+        if (*dead) return false;
+        if (now_ns() > until) {
+            *dead = 1;
+            atomicOr(&g_rows_error, kErrSpinTimeout);
+            return false;
+        }
+    }
+}
+// The same for what is already in flight when a dead block ends.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+    const uint64_t until = now_ns() + kWaitLimitNs;
+    while (!mbar_try(bar, parity) && now_ns() < until) {}
+}
+__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t x, int32_t y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t x, int4 rows) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+                 :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+// Shared-memory matrix descriptor: rows of 128 bytes, 128-byte swizzle, eight rows (1024 bytes) to the next group.
+__device__ __forceinline__ uint64_t matrix_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// 32 columns of this warp's 32 TMEM lanes, a lane a thread.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+                   "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+                   "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(addr));
+}
+
+// Waits for this thread's TMEM loads.  The registers pass through, so that no use of theirs moves ahead of it.
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) :: "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
+    uint32_t (&lo)[16] = *(uint32_t (*)[16])&v[0];
+    uint32_t (&hi)[16] = *(uint32_t (*)[16])&v[16];
+    tmem_wait(lo);
+    tmem_wait(hi);
+}
+
+template <typename T> __device__ __forceinline__ T round_to(float v);
+template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// COLS sums of one output row from column n on.
+template <typename T, int COLS>
+__device__ __forceinline__ void store_row(const ProductArgs &a, uint64_t m, uint32_t n, const float (&acc)[COLS], bool valid) {
+    constexpr uint32_t kPer = 16 / sizeof(T);
+    T *row = (T *)a.out + m * a.out_stride + n;
+    const bool vec = (uintptr_t)row % 16 == 0;
+#pragma unroll
+    for (uint32_t j = 0; j < COLS; j += kPer) {
+        T e[kPer];
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) {
+            float v = acc[j + i];
+            if (a.bias && n + j + i < a.out_dim) v += __ldg(a.bias + n + j + i);
+            e[i] = round_to<T>(valid ? v : 0.f);
+        }
+        if (vec && n + j + kPer <= a.out_dim) {
+            uint4 q;
+            memcpy(&q, e, 16);
+            *(uint4 *)(row + j) = q;
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i)
+                if (n + j + i < a.out_dim) row[j + i] = e[i];
+        }
+    }
+}
+
+template <int BN, bool IDS, typename T>
+__global__ void __launch_bounds__(kTileThreads, 1)
+k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const TileArgs t) {
+    constexpr int kStages = load_stages(BN), kHalf = BN / 2;
+    extern __shared__ uint8_t raw_shared[];
+    uint8_t *shared = (uint8_t *)(((uintptr_t)raw_shared + 1023) & ~(uintptr_t)1023);  // the swizzle's period
+    uint64_t *bars = (uint64_t *)(shared + kStages * stage_bytes(BN));
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 8 * kAccStages,
+                   done = acc_empty + 8 * kAccStages;
+    uint32_t *words = (uint32_t *)(bars + 2 * kStages + 2 * kAccStages + 1);
+    volatile uint32_t *dead = words + 1;
+    const ProductArgs &a = t.p;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+        for (int i = 0; i < kAccStages; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, 8); }
+        mbar_init(done, 1);
+        *dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(words)), "r"(kAccStages * BN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *(volatile uint32_t *)words;
+    const uint32_t tiles = t.m_tiles * t.n_tiles, steps = a.blocks;
+
+    if (warp == 0) {
+        uint32_t issued = 0;
+        bool alive = true;
+        for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+            const uint32_t m0 = tile / t.n_tiles * kBM, n0 = tile % t.n_tiles * BN;
+            int4 rows = make_int4(0, 0, 0, 0);
+            if (IDS) {  // rows without one, and ids outside, load row 0: the epilogue leaves its zeros
+                int r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint64_t m = m0 + lane * 4 + i;
+                    r[i] = 0;
+                    if (m < a.rows) {
+                        const uint64_t id = source_row(a, m);
+                        if (id < a.held) r[i] = (int)id;
+                    }
+                }
+                rows = make_int4(r[0], r[1], r[2], r[3]);
+            }
+            for (uint32_t k = 0; k < steps; ++k, ++issued) {
+                const uint32_t s = issued % kStages;
+                alive = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, (issued / kStages & 1) ^ 1, dead));
+                if (!alive) break;
+                const uint32_t at = smem_u32(shared + s * stage_bytes(BN));
+                if (lane == 0) mbar_expect(full + 8 * s, stage_bytes(BN));
+                __syncwarp();
+                if (IDS) tma_gather4(at + lane * 4 * kBK, &map_a, full + 8 * s, k * kBK, rows);
+                if (lane == 0) {
+                    if (!IDS) tma_tile(at, &map_a, full + 8 * s, k * kBK, m0);
+                    tma_tile(at + kBM * kBK, &map_w, full + 8 * s, k * kBK, n0);
+                }
+            }
+        }
+        if (!alive)
+            for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_drain(full + 8 * (i % kStages), i / kStages & 1);
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);  // e4m3 x e4m3 -> f32
+            uint32_t n = 0;
+            bool alive = true;
+            for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x)
+                for (uint32_t k = 0; k < steps; ++k, ++n) {
+                    const uint32_t s = n % kStages, c = n % kAccStages;
+                    alive = mbar_wait(acc_empty + 8 * c, (n / kAccStages & 1) ^ 1, dead) && mbar_wait(full + 8 * s, n / kStages & 1, dead);
+                    if (!alive) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = smem_u32(shared + s * stage_bytes(BN));
+                    const uint64_t da = matrix_desc(at), db = matrix_desc(at + kBM * kBK);
+#pragma unroll
+                    for (int q = 0; q < kBK / 32; ++q) mma_f8(tmem + c * BN, da + q * 2, db + q * 2, kIdesc, q > 0);
+                    mma_commit(empty + 8 * s);
+                    mma_commit(acc_full + 8 * c);
+                }
+            if (!alive) {
+                mma_commit(done);
+                mbar_drain(done, 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
+        uint32_t n = 0;
+        bool alive = true;
+        for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+            const uint32_t m0 = tile / t.n_tiles * kBM, n0 = tile % t.n_tiles * BN;
+            const uint64_t m = m0 + quarter * 32 + lane;
+            uint64_t src = m;
+            bool valid = m < a.rows;
+            if (IDS && valid) {
+                src = a.ids64 ? (uint64_t)((const int64_t *)a.ids)[m] : (uint64_t)((const uint32_t *)a.ids)[m];
+                valid = src < a.held;
+            }
+            const float *sa = a.scales + (valid ? src : 0) * a.blocks;
+            const float *sw = a.weight_scales + (uint64_t)(n0 / kF8Block) * a.blocks;
+            float acc[kHalf];
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) acc[i] = 0.f;
+            for (uint32_t k = 0; k < steps; ++k, ++n) {
+                const uint32_t c = n % kAccStages;
+                const float scale = __ldg(sa + k) * __ldg(sw + k);
+                alive = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * c, n / kAccStages & 1, dead));
+                if (!alive) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t from = tmem + c * BN + half * kHalf + (quarter << 21);
+                if constexpr (kHalf >= 32) {
+                    uint32_t v[kHalf / 32][32];
+#pragma unroll
+                    for (int j = 0; j < kHalf / 32; ++j) tmem_load32(from + j * 32, v[j]);
+#pragma unroll
+                    for (int j = 0; j < kHalf / 32; ++j) tmem_wait(v[j]);
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    if (lane == 0) mbar_arrive(acc_empty + 8 * c);
+#pragma unroll
+                    for (int j = 0; j < kHalf; ++j) acc[j] += scale * __uint_as_float(v[j / 32][j % 32]);
+                } else {
+                    uint32_t v[16];
+                    tmem_load16(from, v);
+                    tmem_wait(v);
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    if (lane == 0) mbar_arrive(acc_empty + 8 * c);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[j] += scale * __uint_as_float(v[j]);
+                }
+            }
+            if (alive && m < a.rows && n0 + half * kHalf < a.out_dim) store_row<T, kHalf>(a, m, n0 + half * kHalf, acc, valid);
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(kAccStages * BN));
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult status;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &status) == cudaSuccess && status == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiled)p;
+        else cudaGetLastError();
+    });
+    return fn;
+}
+
+// Rows of bytes as a tensor map: 128 columns x `box` rows a load, what lies outside reads as zeros.
+int32_t rows_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t dim, uint64_t pitch, uint32_t box) {
+    if (!encode_tiled()) return fail(AG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[2] = {dim, rows}, strides[1] = {pitch};
+    const cuuint32_t boxes[2] = {kBK, box}, steps[2] = {1, 1};
+    const CUresult r = encode_tiled()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, boxes, steps,
+                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(AG_ERR_CUDA, "cannot describe %llu rows of %llu bytes at a pitch of %llu (driver error %d)", (unsigned long long)rows,
+                    (unsigned long long)dim, (unsigned long long)pitch, (int)r);
+    return AG_OK;
+}
+
+template <int BN, bool IDS, typename T>
+int32_t launch_tile(const ProductArgs &a, cudaStream_t st) {
+    TileArgs t{a, (uint32_t)((a.rows + kBM - 1) / kBM), (a.out_dim + BN - 1) / BN};
+    CUtensorMap map_a, map_w;
+    AG_TRY(rows_map(&map_a, a.codes, IDS ? a.held : a.rows, a.dim, a.code_stride, IDS ? 1 : kBM));
+    AG_TRY(rows_map(&map_w, a.weight, a.out_dim, a.dim, a.weight_stride, BN));
+    AG_CUDA(cudaFuncSetAttribute(k_product_tile<BN, IDS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_shared(BN)));
+    const uint64_t tiles = (uint64_t)t.m_tiles * t.n_tiles;
+    if (tiles > 0x7FFFFFFFull) return fail(AG_ERR_VALUE, "ag_rows_product: the output is too large");
+    k_product_tile<BN, IDS, T><<<(uint32_t)std::min<uint64_t>(tiles, kSMs), kTileThreads, tile_shared(BN), st>>>(map_a, map_w, t);
+    return AG_OK;
+}
+
+template <bool IDS, typename T> int32_t launch_tile(const ProductArgs &a, cudaStream_t st) {
+    // The widest tile that no half of is empty and that still gives every SM one.
+    const uint64_t m_tiles = (a.rows + kBM - 1) / kBM;
+    uint32_t bn = 128;
+    while (bn > 32 && (bn / 2 >= a.out_dim || m_tiles * ((a.out_dim + bn - 1) / bn) < (uint64_t)kSMs)) bn /= 2;
+    if (bn == 128) return launch_tile<128, IDS, T>(a, st);
+    if (bn == 64) return launch_tile<64, IDS, T>(a, st);
+    return launch_tile<32, IDS, T>(a, st);
+}
+
+template <typename T> int32_t launch_tile(const ProductArgs &a, cudaStream_t st) {
+    return a.ids ? launch_tile<true, T>(a, st) : launch_tile<false, T>(a, st);
+}
+
 }  // namespace
 
 }  // namespace ag
@@ -125,15 +470,15 @@ extern "C" int32_t ag_rows_product(const ag_product *p, int32_t device, void *st
     a.dim = (uint32_t)p->dim; a.out_dim = (uint32_t)p->out_dim; a.blocks = (uint32_t)((p->dim + kF8Block - 1) / kF8Block);
     a.ids64 = p->ids_are_i64; a.out_dtype = p->out_dtype;
     cudaStream_t st = (cudaStream_t)stream;
-    const uint64_t slabs = (a.rows + kDotRows - 1) / kDotRows;
-    for (uint64_t s0 = 0; s0 < slabs; s0 += 65535) {  // the grid's y ends there
-        ProductArgs b = a;
-        b.rows = std::min<uint64_t>(a.rows - s0 * kDotRows, 65535ull * kDotRows);
-        if (a.ids) b.ids = (const uint8_t *)a.ids + s0 * kDotRows * (a.ids64 ? 8 : 4);
-        else { b.codes += s0 * kDotRows * a.code_stride; b.scales += s0 * kDotRows * a.blocks; }
-        b.out = (uint8_t *)a.out + s0 * kDotRows * a.out_stride * elem_size(a.out_dtype);
-        const uint32_t y = (uint32_t)std::min<uint64_t>(slabs - s0, 65535);
-        k_product_dot<<<dim3((a.out_dim + kDotThreads / 32 - 1) / (kDotThreads / 32), y), kDotThreads, 0, st>>>(b);
+    if (a.rows <= kFewRows) {
+        const dim3 grid((a.out_dim + kDotThreads / 32 - 1) / (kDotThreads / 32), (uint32_t)((a.rows + kDotRows - 1) / kDotRows));
+        k_product_dot<<<grid, kDotThreads, 0, st>>>(a);
+    } else if (a.out_dtype == AG_F32) {
+        AG_TRY(launch_tile<float>(a, st));
+    } else if (a.out_dtype == AG_F16) {
+        AG_TRY(launch_tile<__half>(a, st));
+    } else {
+        AG_TRY(launch_tile<__nv_bfloat16>(a, st));
     }
     AG_CUDA(cudaGetLastError());
     return AG_OK;
@@ -148,5 +493,6 @@ extern "C" int32_t ag_rows_check(int32_t device) {
     if (!h) return AG_OK;
     const uint32_t zero = 0;
     AG_CUDA(cudaMemcpyToSymbol(g_rows_error, &zero, 4));
+    if (h & kErrSpinTimeout) return fail(AG_ERR_CUDA, "a product gave up waiting for its loads or multiplications; its output is incomplete");
     return fail(AG_ERR_VALUE, "a row id of a product is out of bounds");
 }
