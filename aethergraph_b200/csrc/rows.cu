@@ -57,16 +57,28 @@ template <typename T> __device__ __forceinline__ void store_words(const Raw<T> &
     asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};" :: "l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]) : "memory");
 }
 
-// Columns c .. c + 7 of a row of `dim`; what lies past its end reads as zeros.  VEC: rows start on
-// multiples of eight elements' bytes.
-template <typename T, bool VEC> __device__ __forceinline__ Raw<T> load_chunk(const T *row, uint32_t c, uint32_t dim) {
+// Which eight columns of a row a thread holds in its step j.  Aligned rows (VEC: every row starts on a
+// multiple of eight elements' bytes): a chunk, one vector load.  Others: the lanes of a group take
+// consecutive columns, so that its eight loads of one element each are coalesced: the thread's
+// columns lie `stride` apart, and the group still covers whole chunks together.
+template <bool VEC> struct Columns {
+    uint32_t first, stride;
+    __device__ __forceinline__ Columns(uint32_t lane, uint32_t lanes, uint32_t step_chunk) {  // lanes: of the group, at most 32
+        stride = VEC ? 1 : lanes;
+        first = VEC ? (step_chunk + lane) * kChunk : step_chunk * kChunk + lane;
+    }
+    __device__ __forceinline__ uint32_t at(uint32_t i) const { return first + i * stride; }
+};
+
+// A thread's eight columns; what lies past the row's end reads as zeros.
+template <typename T, bool VEC> __device__ __forceinline__ Raw<T> load_chunk(const T *row, const Columns<VEC> &c, uint32_t dim) {
     Raw<T> r;
-    if (VEC && c + kChunk <= dim) {
-        load_words(r, row + c);
+    if (VEC && c.first + kChunk <= dim) {
+        load_words(r, row + c.first);
     } else {
         T e[kChunk];
 #pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) e[i] = c + i < dim ? row[c + i] : from_f32<T>(0.f);
+        for (uint32_t i = 0; i < kChunk; ++i) e[i] = c.at(i) < dim ? row[c.at(i)] : from_f32<T>(0.f);
         memcpy(&r, e, sizeof r);
     }
     return r;
@@ -77,25 +89,43 @@ template <typename T> __device__ __forceinline__ void unpack(const Raw<T> &r, fl
 #pragma unroll
     for (uint32_t i = 0; i < kChunk; ++i) v[i] = to_f32(e[i]);
 }
-template <typename T, bool VEC> __device__ __forceinline__ void store_chunk(T *row, uint32_t c, uint32_t dim, const float v[kChunk]) {
+template <typename T> __device__ __forceinline__ Raw<T> pack(const float v[kChunk]) {
     T e[kChunk];
 #pragma unroll
     for (uint32_t i = 0; i < kChunk; ++i) e[i] = from_f32<T>(v[i]);
-    if (VEC && c + kChunk <= dim) {
-        Raw<T> r;
-        memcpy(&r, e, sizeof r);
-        store_words(r, row + c);
+    Raw<T> r;
+    memcpy(&r, e, sizeof r);
+    return r;
+}
+template <typename T, bool VEC> __device__ __forceinline__ void store_chunk(T *row, const Columns<VEC> &c, uint32_t dim, const float v[kChunk]) {
+    if (VEC && c.first + kChunk <= dim) {
+        store_words(pack<T>(v), row + c.first);
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
-            if (c + i < dim) row[c + i] = e[i];
+            if (c.at(i) < dim) row[c.at(i)] = from_f32<T>(v[i]);
     }
 }
-// The norm's weights: the rows' type or f32, any alignment, the same few for every row (L1).
-template <typename T> __device__ __forceinline__ void load_weight(const void *w, int w_f32, uint32_t c, uint32_t dim, float v[kChunk]) {
+// The norm's weights, of the rows' type or f32: the same few for every row (L1).
+template <typename T, bool VEC> __device__ __forceinline__ void load_weight(const void *w, int w_f32, const Columns<VEC> &c, uint32_t dim, float v[kChunk]) {
+    if (!w) {
 #pragma unroll
-    for (uint32_t i = 0; i < kChunk; ++i)
-        v[i] = !w ? 1.f : c + i >= dim ? 0.f : w_f32 ? __ldg((const float *)w + c + i) : to_f32(((const T *)w)[c + i]);
+        for (uint32_t i = 0; i < kChunk; ++i) v[i] = 1.f;
+    } else if (VEC && c.first + kChunk <= dim) {
+        if (w_f32) {
+            const float4 lo = __ldg((const float4 *)((const float *)w + c.first)), hi = __ldg((const float4 *)((const float *)w + c.first) + 1);
+            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+        } else if constexpr (sizeof(T) == 2) {
+            const uint4 q = __ldg((const uint4 *)((const T *)w + c.first));
+            Raw<T> r;
+            memcpy(&r, &q, sizeof q);
+            unpack(r, v);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kChunk; ++i)
+            v[i] = c.at(i) >= dim ? 0.f : w_f32 ? __ldg((const float *)w + c.at(i)) : to_f32(((const T *)w)[c.at(i)]);
+    }
 }
 
 // ---------------------------------------------------------------- dropout --
@@ -105,13 +135,31 @@ struct Drop {
     uint64_t seed, offset;
 };
 
-__device__ __forceinline__ void drop_chunk(const Drop &d, uint64_t row, uint32_t chunk, float v[kChunk]) {
-    const uint4 r = philox4x32_10(d.seed, (uint32_t)d.offset, row << 32 | chunk, (uint32_t)(d.offset >> 32));
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+__device__ __forceinline__ uint4 lots_of(const Drop &d, uint64_t row, uint32_t chunk) {
+    return philox4x32_10(d.seed, (uint32_t)d.offset, row << 32 | chunk, (uint32_t)(d.offset >> 32));
+}
+__device__ __forceinline__ uint32_t lot(const uint4 &r, uint32_t i) {  // i is a constant where this is used
+    const uint32_t w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
+    return i & 1 ? w >> 16 : w & 0xFFFFu;
+}
+// A select: a dropped infinity or NaN is gone.
+__device__ __forceinline__ float kept(const Drop &d, uint32_t u, float v) { return u >= d.threshold ? v * d.scale : 0.f; }
+
+// Dropout of a thread's eight columns.  Unless they are a chunk, the group's lanes make the lots of one
+// chunk each and pass them around in shared memory (16 bytes a lane); the whole warp calls this.
+template <bool VEC>
+__device__ __forceinline__ void drop_columns(const Drop &d, uint64_t row, uint32_t lane, uint32_t lanes, uint32_t step_chunk, uint4 *warp_lots, float v[kChunk]) {
+    const uint4 r = lots_of(d, row, step_chunk + lane);
+    if (VEC) {
 #pragma unroll
-    for (uint32_t i = 0; i < kChunk; ++i) {
-        const uint32_t u = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xFFFFu;
-        v[i] = u >= d.threshold ? v[i] * d.scale : 0.f;  // a select: a dropped infinity or NaN is gone
+        for (uint32_t i = 0; i < kChunk; ++i) v[i] = kept(d, lot(r, i), v[i]);
+    } else {
+        __syncwarp();
+        warp_lots[threadIdx.x & 31] = r;
+        __syncwarp();
+        const uint16_t *group = (const uint16_t *)(warp_lots + ((threadIdx.x & 31) - lane));
+#pragma unroll
+        for (uint32_t i = 0; i < kChunk; ++i) v[i] = kept(d, group[lane + i * lanes], v[i]);
     }
 }
 
@@ -125,11 +173,69 @@ k_dropout(const T *x, T *y, uint64_t rows, uint32_t dim, uint64_t x_stride, uint
     const uint64_t total = rows * chunks;
     for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < total; i += (uint64_t)gridDim.x * kThreads) {
         const uint64_t row = i / chunks;
-        const uint32_t chunk = (uint32_t)(i - row * chunks);
+        const uint32_t chunk = (uint32_t)(i - row * chunks), c = chunk * kChunk;
         float v[kChunk];
-        unpack(load_chunk<T, VEC>(x + row * x_stride, chunk * kChunk, dim), v);
-        drop_chunk(d, row, chunk, v);
-        store_chunk<T, VEC>(y + row * y_stride, chunk * kChunk, dim, v);
+        if (VEC && c + kChunk <= dim) {
+            Raw<T> r;
+            load_words(r, x + row * x_stride + c);
+            unpack(r, v);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < kChunk; ++e) v[e] = c + e < dim ? to_f32(x[row * x_stride + c + e]) : 0.f;
+        }
+        const uint4 r = lots_of(d, row, chunk);
+#pragma unroll
+        for (uint32_t e = 0; e < kChunk; ++e) v[e] = kept(d, lot(r, e), v[e]);
+        if (VEC && c + kChunk <= dim) {
+            store_words(pack<T>(v), y + row * y_stride + c);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < kChunk; ++e)
+                if (c + e < dim) y[row * y_stride + c + e] = from_f32<T>(v[e]);
+        }
+    }
+}
+
+// Contiguous rows whose length is no multiple of eight: the lots belong to chunks, the memory is walked
+// in aligned vectors of eight elements, whatever row they are in.  A block's 256 chunks cover one
+// run of elements; the threads leave a byte per element that says whether it stays, and read
+// eight of them back for their vector.  The vectors at the run's ends belong to two blocks, element by element.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+k_dropout_flat(const T *x, T *y, uint64_t total, uint32_t dim, Drop d) {
+    __shared__ __align__(16) uint8_t stays[kThreads * kChunk + 16];
+    const uint32_t chunks = (dim + kChunk - 1) / kChunk;
+    const uint64_t i0 = blockIdx.x * (uint64_t)kThreads, i1 = min(i0 + kThreads, total);
+    auto element = [&](uint64_t i) { return i / chunks * dim + (uint32_t)(i % chunks) * kChunk; };
+    const uint64_t from = element(i0), to = element(i1), origin = from & ~(uint64_t)(kChunk - 1);
+    const uint64_t mine = origin + threadIdx.x * kChunk;
+    Raw<T> r{};
+    if (mine >= from && mine + kChunk <= to) load_words(r, x + mine);
+    const uint32_t rest = (uint32_t)(i0 % chunks) + threadIdx.x, over = rest / chunks, chunk = rest - over * chunks;
+    const uint64_t row = i0 / chunks + over;
+    if (i0 + threadIdx.x < i1) {
+        const uint4 lots = lots_of(d, row, chunk);
+        uint8_t *at = stays + (uint32_t)(row * dim + chunk * kChunk - origin);
+        const uint32_t len = min(kChunk, dim - chunk * kChunk);
+#pragma unroll
+        for (uint32_t e = 0; e < kChunk; ++e)
+            if (e < len) at[e] = lot(lots, e) >= d.threshold;
+    }
+    __syncthreads();
+    for (uint64_t f = mine; f < to; f += kThreads * kChunk) {
+        const uint8_t *at = stays + (uint32_t)(f - origin);
+        if (f >= from && f + kChunk <= to) {
+            if (f != mine) load_words(r, x + f);
+            const uint2 flags = *(const uint2 *)at;
+            float v[kChunk];
+            unpack(r, v);
+#pragma unroll
+            for (uint32_t e = 0; e < kChunk; ++e) v[e] = (e < 4 ? flags.x : flags.y) >> (8 * (e & 3)) & 1 ? v[e] * d.scale : 0.f;
+            store_words(pack<T>(v), y + f);
+        } else {
+            for (uint32_t e = 0; e < kChunk; ++e)
+                if (f + e >= from && f + e < to) y[f + e] = at[e] ? from_f32<T>(to_f32(x[f + e]) * d.scale) : from_f32<T>(0.f);
+        }
     }
 }
 
@@ -160,95 +266,120 @@ template <bool BLOCK> __device__ __forceinline__ float row_sum(float v, uint32_t
     return v;
 }
 
-// e4m3 codes and scale of a row's block of 128 columns: the 16 chunks that hold it are the
-// consecutive lanes `lanes` wide.  The scale puts the block's largest magnitude on 448; a block
-// with an infinity or NaN gets a NaN scale, so that every value read from it is NaN.  Magnitudes
-// are compared as bits: NaN above infinity above every number.
-__device__ __forceinline__ void encode_chunk(const float v[kChunk], uint32_t lanes, uint32_t c, uint32_t dim, uint8_t *row_codes,
-                                             float *row_scales) {
-    uint32_t top = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kChunk; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    for (uint32_t o = min(lanes, kF8Block / kChunk) / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (c >= dim) return;
+// Scale of a block of 128 columns whose largest magnitude has the bits `top` (as bits NaN lies above
+// infinity above every number), and its reciprocal.  The scale puts that magnitude on 448; a block with an infinity or
+// NaN gets a NaN scale, so that every value read from it is NaN.  At least the least normal
+// f32, so that the reciprocal is finite.  Reciprocal and product are rounded once each: a code is
+// off by half a step and 2^-23 of the value.
+__device__ __forceinline__ float scale_of(uint32_t top, float &inv) {
     const bool bad = top >= 0x7F800000u;
-    // The least normal f32 at least, so that its reciprocal is finite.  The reciprocal is rounded
-    // once and the product once more: a code is off by half a step and 2^-23 of the value.
     const float scale = bad ? __uint_as_float(0x7FC00000u) : fmaxf(__uint_as_float(top) / kE4M3Max, 1.17549435e-38f);
-    const float inv = bad ? 0.f : 1.f / scale;
-    if (c % kF8Block == 0) row_scales[c / kF8Block] = scale;
-    uint32_t w[2] = {0, 0};
+    inv = bad ? 0.f : 1.f / scale;
+    return scale;
+}
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ uint32_t code2(float a, float b, float inv) {  // a reciprocal of 0: a block that is not finite
+    return inv == 0.f ? 0u : (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+}
+
+// e4m3 codes and scales of a group's step; the whole warp calls this.
+template <bool VEC>
+__device__ __forceinline__ void encode_columns(const float v[kChunk], const Columns<VEC> &c, uint32_t lane, uint32_t lanes, uint32_t dim, uint8_t *codes, float *scales) {
+    if (VEC) {  // the 16 lanes of a block reduce; a chunk lies in one block
+        uint32_t top = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kChunk; i += 2)
-        w[i >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[i] * inv, v[i + 1] * inv), __NV_SATFINITE, __NV_E4M3) << (8 * (i & 3));
-    if (bad) w[0] = w[1] = 0;
-    // The pitch is a multiple of 16 bytes, so the padding takes what a last chunk writes past the row.
-    *(uint2 *)(row_codes + c) = make_uint2(w[0], w[1]);
+        for (uint32_t i = 0; i < kChunk; ++i) top = max(top, magnitude(v[i]));
+        for (uint32_t o = min(lanes, kF8Block / kChunk) / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (c.first >= dim) return;
+        float inv;
+        const float scale = scale_of(top, inv);
+        if (c.first % kF8Block == 0) scales[c.first / kF8Block] = scale;
+        // the pitch is a multiple of 16 bytes, so its padding takes what a last chunk writes past the row
+        *(uint2 *)(codes + c.first) = make_uint2(code2(v[0], v[1], inv) | code2(v[2], v[3], inv) << 16, code2(v[4], v[5], inv) | code2(v[6], v[7], inv) << 16);
+    } else {  // 32 lanes: columns 0 - 3 of each thread are one block, 4 - 7 the next; fewer lanes have at most one block
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kChunk / 2; ++i) { lo = max(lo, magnitude(v[i])); hi = max(hi, magnitude(v[i + kChunk / 2])); }
+        if (lanes < 32) lo = hi = max(lo, hi);
+        for (uint32_t o = lanes / 2; o > 0; o /= 2) {
+            lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        }
+        float inv_lo, inv_hi;
+        const float scale_lo = scale_of(lo, inv_lo), scale_hi = scale_of(hi, inv_hi);
+        if (lane == 0) {
+            if (c.first < dim) scales[c.first / kF8Block] = scale_lo;
+            if (lanes == 32 && c.first + kF8Block < dim) scales[c.first / kF8Block + 1] = scale_hi;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kChunk; ++i)
+            if (c.at(i) < dim) codes[c.at(i)] = (uint8_t)code2(v[i], 0.f, i < kChunk / 2 ? inv_lo : inv_hi);
+    }
 }
 
 // h = res + dropout(x); y = h rsqrt(mean(h^2) + eps) w.  `lanes` lanes a row (BLOCK: the whole
 // block), C chunks each; the row stays in registers between the sum and the output.
 template <typename T, bool VEC, int C, bool BLOCK, bool F8>
-__global__ void __launch_bounds__(BLOCK ? 512 : kThreads)
-k_norm(NormArgs a, uint32_t lanes) {
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : C == 1 ? 5 : C == 2 ? 4 : 2)
+k_norm(const NormArgs a, uint32_t lanes) {
     __shared__ float shared[32];
-    const uint32_t lane = BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
-    const uint32_t width = BLOCK ? blockDim.x : lanes;
-    const uint64_t per_block = blockDim.x / width;
-    for (uint64_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block) {
-        const uint64_t row = base + (BLOCK ? 0 : threadIdx.x / lanes);
-        const bool in = row < a.rows;  // the others still take part in the shuffles
-        float v[C][kChunk];
+    __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
+    uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
+    const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
+    const uint64_t row = BLOCK ? blockIdx.x : (uint64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+    const uint32_t dim = row < a.rows ? a.dim : 0;  // lanes without a row still take part in the exchanges
+    float v[C][kChunk];
+    {
         Raw<T> rx[C], rr[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const uint32_t c = (lane + j * width) * kChunk;
-            const uint32_t end = in ? a.dim : 0;
-            if (c < end) {
-                rx[j] = load_chunk<T, VEC>((const T *)a.x + row * a.x_stride, c, end);
-                if (a.res) rr[j] = load_chunk<T, VEC>((const T *)a.res + row * a.res_stride, c, end);
-            }
+            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+            if (c.first >= dim) continue;
+            rx[j] = load_chunk<T, VEC>((const T *)a.x + row * a.x_stride, c, dim);
+            if (a.res) rr[j] = load_chunk<T, VEC>((const T *)a.res + row * a.res_stride, c, dim);
         }
-        float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const uint32_t chunk = lane + j * width, c = chunk * kChunk;
+            const uint32_t step = j * width + group_chunk;
+            const Columns<VEC> c(lane, lanes, step);
 #pragma unroll
             for (uint32_t i = 0; i < kChunk; ++i) v[j][i] = 0.f;
-            if (in && c < a.dim) {
-                unpack(rx[j], v[j]);
-                if (a.drop.threshold) drop_chunk(a.drop, row, chunk, v[j]);
-                if (a.res) {
-                    float r[kChunk];
-                    unpack(rr[j], r);
+            if (c.first < dim) unpack(rx[j], v[j]);
+            if (a.drop.threshold) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, v[j]);
+            if (a.res && c.first < dim) {
+                float r[kChunk];
+                unpack(rr[j], r);
 #pragma unroll
-                    for (uint32_t i = 0; i < kChunk; ++i) v[j][i] += r[i];
-                }
-                if (a.h) store_chunk<T, VEC>((T *)a.h + row * a.h_stride, c, a.dim, v[j]);
-#pragma unroll
-                for (uint32_t i = 0; i < kChunk; ++i) sum += v[j][i] * v[j][i];
+                for (uint32_t i = 0; i < kChunk; ++i) v[j][i] += r[i];
             }
         }
-        if (!a.plain) {
-            const float rstd = rsqrtf(row_sum<BLOCK>(sum, lanes, shared) / (float)a.dim + a.eps);
-            if (a.rstd && in && lane == 0) a.rstd[row] = rstd;
+    }
+    float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < C; ++j) {
-                float w[kChunk];
-                load_weight<T>(a.weight, a.w_f32, (lane + j * width) * kChunk, a.dim, w);
+    for (int j = 0; j < C; ++j) {
+        const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+        if (a.h && c.first < dim) store_chunk<T, VEC>((T *)a.h + row * a.h_stride, c, dim, v[j]);
 #pragma unroll
-                for (uint32_t i = 0; i < kChunk; ++i) v[j][i] *= rstd * w[i];
-            }
-        }
+        for (uint32_t i = 0; i < kChunk; ++i) sum += v[j][i] * v[j][i];
+    }
+    if (!a.plain) {
+        const float rstd = rsqrtf(row_sum<BLOCK>(sum, lanes, shared) / (float)a.dim + a.eps);
+        if (a.rstd && dim && (BLOCK ? threadIdx.x : lane) == 0) a.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const uint32_t c = (lane + j * width) * kChunk, end = in ? a.dim : 0;
-            if (F8) {
-                encode_chunk(v[j], lanes, c, end, a.codes + row * a.code_stride, a.scales + row * ((a.dim + kF8Block - 1) / kF8Block));
-            } else if (c < end) {
-                store_chunk<T, VEC>((T *)a.y + row * a.y_stride, c, end, v[j]);
-            }
+            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+            if (c.first >= dim) continue;
+            float w[kChunk];
+            load_weight<T, VEC>(a.weight, a.w_f32, c, dim, w);
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i) v[j][i] *= rstd * w[i];
         }
+    }
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+        const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+        if (F8) encode_columns<VEC>(v[j], c, lane, lanes, dim, a.codes + row * a.code_stride, a.scales + row * ((a.dim + kF8Block - 1) / kF8Block));
+        else if (c.first < dim) store_chunk<T, VEC>((T *)a.y + row * a.y_stride, c, dim, v[j]);
     }
 }
 
@@ -268,13 +399,14 @@ struct NormBackArgs {
 // sums; a block adds its lane groups in order into its row of `partial`, and k_norm_dw adds those.
 // No atomics: the same bits every time on the same GPU.
 template <typename T, bool VEC, int C, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : kThreads)
-k_norm_back(NormBackArgs a, uint32_t lanes) {
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : C == 1 ? 4 : 2)
+k_norm_back(const NormBackArgs a, uint32_t lanes) {
     __shared__ float shared[32];
+    __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
     extern __shared__ float sums[];  // [groups of the block][dim], not BLOCK
-    const uint32_t lane = BLOCK ? threadIdx.x : threadIdx.x & (lanes - 1);
-    const uint32_t width = BLOCK ? blockDim.x : lanes;
-    const uint64_t per_block = blockDim.x / width;
+    uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
+    const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
+    const uint64_t per_block = BLOCK ? 1 : blockDim.x / lanes;
     float dw[C][kChunk];
 #pragma unroll
     for (int j = 0; j < C; ++j)
@@ -282,86 +414,69 @@ k_norm_back(NormBackArgs a, uint32_t lanes) {
         for (uint32_t i = 0; i < kChunk; ++i) dw[j][i] = 0.f;
     for (uint64_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block) {
         const uint64_t row = base + (BLOCK ? 0 : threadIdx.x / lanes);
-        const bool in = row < a.rows;
-        const uint32_t end = in ? a.dim : 0;
+        const uint32_t dim = row < a.rows ? a.dim : 0;
         Raw<T> ry[C], rh[C], rd[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const uint32_t c = (lane + j * width) * kChunk;
-            if (c < end) {
-                rh[j] = load_chunk<T, VEC>((const T *)a.h + row * a.h_stride, c, end);
-                if (a.dy) ry[j] = load_chunk<T, VEC>((const T *)a.dy + row * a.dy_stride, c, end);
-                if (a.dh) rd[j] = load_chunk<T, VEC>((const T *)a.dh + row * a.dh_stride, c, end);
-            }
+            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+            ry[j] = rh[j] = rd[j] = Raw<T>{};
+            if (c.first >= dim) continue;
+            rh[j] = load_chunk<T, VEC>((const T *)a.h + row * a.h_stride, c, dim);
+            if (a.dy) ry[j] = load_chunk<T, VEC>((const T *)a.dy + row * a.dy_stride, c, dim);
+            if (a.dh) rd[j] = load_chunk<T, VEC>((const T *)a.dh + row * a.dh_stride, c, dim);
         }
-        const float rstd = in ? a.rstd[row] : 0.f;
-        float g[C][kChunk], h[C][kChunk], sum = 0.f;
+        const float rstd = dim ? a.rstd[row] : 0.f;
+        float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const uint32_t c = (lane + j * width) * kChunk;
+            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+            if (c.first >= dim) continue;
+            float g[kChunk], h[kChunk], w[kChunk];
+            unpack(rh[j], h);
+            unpack(ry[j], g);
+            load_weight<T, VEC>(a.weight, a.w_f32, c, dim, w);
 #pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) g[j][i] = h[j][i] = 0.f;
-            if (c < end) {
-                unpack(rh[j], h[j]);
-                if (a.dy) {
-                    float w[kChunk];
-                    unpack(ry[j], g[j]);
-                    load_weight<T>(a.weight, a.w_f32, c, end, w);
-#pragma unroll
-                    for (uint32_t i = 0; i < kChunk; ++i) {
-                        dw[j][i] += g[j][i] * (h[j][i] * rstd);
-                        g[j][i] *= w[i];
-                        sum += g[j][i] * h[j][i];
-                    }
-                }
+            for (uint32_t i = 0; i < kChunk; ++i) {
+                const float gh = g[i] * h[i];
+                dw[j][i] += gh * rstd;
+                sum += gh * w[i];
             }
         }
         const float coef = row_sum<BLOCK>(sum, lanes, shared) * rstd * rstd * rstd / (float)a.dim;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const uint32_t chunk = lane + j * width, c = chunk * kChunk;
-            if (c >= end) continue;
-            float t[kChunk];
+            const uint32_t step = j * width + group_chunk;
+            const Columns<VEC> c(lane, lanes, step);
+            float t[kChunk], g[kChunk], h[kChunk], w[kChunk];  // unpacked again: fewer registers across the sum
+            unpack(rh[j], h);
+            unpack(ry[j], g);
+            unpack(rd[j], t);
+            load_weight<T, VEC>(a.weight, a.w_f32, c, dim, w);
 #pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) t[i] = rstd * g[j][i] - h[j][i] * coef;
-            if (a.dh) {
-                float d[kChunk];
-                unpack(rd[j], d);
-#pragma unroll
-                for (uint32_t i = 0; i < kChunk; ++i) t[i] += d[i];
-            }
-            if (a.dres) store_chunk<T, VEC>((T *)a.dres + row * a.dim, c, end, t);
+            for (uint32_t i = 0; i < kChunk; ++i) t[i] += rstd * (g[i] * w[i]) - h[i] * coef;
+            if (a.dres && c.first < dim) store_chunk<T, VEC>((T *)a.dres + row * a.dim, c, dim, t);
             if (a.dx) {
-                if (a.drop.threshold) drop_chunk(a.drop, row, chunk, t);
-                store_chunk<T, VEC>((T *)a.dx + row * a.dim, c, end, t);
+                if (a.drop.threshold) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, t);
+                if (c.first < dim) store_chunk<T, VEC>((T *)a.dx + row * a.dim, c, dim, t);
             }
         }
     }
     if (!a.partial) return;
     float *mine = a.partial + (uint64_t)blockIdx.x * a.dim;
-    if (BLOCK) {
 #pragma unroll
-        for (int j = 0; j < C; ++j)
+    for (int j = 0; j < C; ++j) {
+        const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+        float *to = BLOCK ? mine : sums + threadIdx.x / lanes * a.dim;
 #pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) {
-                const uint32_t c = (lane + j * width) * kChunk + i;
-                if (c < a.dim) mine[c] = dw[j][i];
-            }
-    } else {
-        const uint32_t group = threadIdx.x / lanes;
-#pragma unroll
-        for (int j = 0; j < C; ++j)
-#pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) {
-                const uint32_t c = (lane + j * width) * kChunk + i;
-                if (c < a.dim) sums[group * a.dim + c] = dw[j][i];
-            }
-        __syncthreads();
-        for (uint32_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
-            float s = 0.f;
-            for (uint32_t q = 0; q < per_block; ++q) s += sums[q * a.dim + c];
-            mine[c] = s;
-        }
+        for (uint32_t i = 0; i < kChunk; ++i)
+            if (c.at(i) < a.dim) to[c.at(i)] = dw[j][i];
+    }
+    if (BLOCK) return;
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
+        float s = 0.f;
+        for (uint32_t q = 0; q < per_block; ++q) s += sums[q * a.dim + c];
+        mine[c] = s;
     }
 }
 
@@ -398,21 +513,19 @@ k_encode_weight(const T *w, uint64_t out, uint32_t dim, uint64_t stride, uint8_t
     for (uint32_t i = threadIdx.x; i < kF8Block * kF8Block; i += kThreads) {
         const uint64_t n = bn * kF8Block + i / kF8Block;
         const uint32_t c = bk * kF8Block + i % kF8Block;
-        if (n < out && c < dim) top = max(top, __float_as_uint(to_f32(w[n * stride + c])) & 0x7FFFFFFFu);
+        if (n < out && c < dim) top = max(top, magnitude(to_f32(w[n * stride + c])));
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) atomicMax(&peak, top);
     __syncthreads();
-    top = peak;
-    const bool bad = top >= 0x7F800000u;
-    const float scale = bad ? __uint_as_float(0x7FC00000u) : fmaxf(__uint_as_float(top) / kE4M3Max, 1.17549435e-38f);
-    const float inv = bad ? 0.f : 1.f / scale;
+    float inv;
+    const float scale = scale_of(peak, inv);
     if (threadIdx.x == 0) scales[blockIdx.x] = scale;
     for (uint32_t i = threadIdx.x; i < kF8Block * kF8Block; i += kThreads) {
         const uint64_t n = bn * kF8Block + i / kF8Block;
         const uint32_t c = bk * kF8Block + i % kF8Block;
         if (n < out && c < dim)
-            codes[n * code_stride + c] = bad ? 0 : (uint8_t)__nv_cvt_float_to_fp8(to_f32(w[n * stride + c]) * inv, __NV_SATFINITE, __NV_E4M3);
+            codes[n * code_stride + c] = (uint8_t)code2(to_f32(w[n * stride + c]), 0.f, inv);
     }
 }
 
@@ -443,28 +556,29 @@ int32_t check_rows(const char *who, uint64_t rows, uint64_t dim, int32_t dtype) 
     return AG_OK;
 }
 
-// How a row of `dim` columns is shared out: lanes (0: a whole block of `threads`) and chunks a lane.
+// How a row of `dim` columns is shared out: `lanes` of a warp (0: a whole block of `threads`) with up to
+// `chunks` chunks each.  The backward pass holds three rows and the weights' sums at once, so
+// it goes over to whole blocks at half the length.
 struct Split { uint32_t lanes, threads; int chunks; };
-Split split_row(uint32_t dim) {
+Split split_row(uint32_t dim, bool backward) {
     const uint32_t n = (dim + kChunk - 1) / kChunk;
     Split s{1, kThreads, 1};
-    if (n <= 128) {
+    if (n <= (backward ? 64u : 128u)) {
         while (s.lanes < 32 && s.lanes < n) s.lanes *= 2;
         while ((uint32_t)s.chunks * s.lanes < n) s.chunks *= 2;
     } else {
         s.lanes = 0;
-        s.threads = 128;
-        while (s.threads < 512 && s.threads * 2 < n) s.threads *= 2;
-        while ((uint32_t)s.chunks * s.threads < n) s.chunks *= 2;
+        while ((uint32_t)s.chunks * 512 < n) s.chunks *= 2;
+        s.threads = (n + 32 * s.chunks - 1) / (32 * s.chunks) * 32;
     }
     return s;
 }
 
 template <typename T, bool VEC, bool F8>
 cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
-    const Split s = split_row(a.dim);
+    const Split s = split_row(a.dim, false);
     const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((a.rows + per - 1) / per, 1u << 30), lanes = s.lanes ? s.lanes : 32;
+    const uint32_t grid = (uint32_t)((a.rows + per - 1) / per), lanes = s.lanes ? s.lanes : 32;  // rows of a whole block are 2 KB and more
     if (s.lanes) {
         if (s.chunks == 1) k_norm<T, VEC, 1, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
         else if (s.chunks == 2) k_norm<T, VEC, 2, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
@@ -478,7 +592,7 @@ cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
 }
 
 uint32_t back_blocks(uint64_t rows, uint32_t dim) {
-    const Split s = split_row(dim);
+    const Split s = split_row(dim, true);
     const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
     return (uint32_t)std::min<uint64_t>((rows + per - 1) / per, (uint64_t)kSMs * (2048 / s.threads) / 2);
 }
@@ -492,11 +606,10 @@ cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t grid, cu
 
 template <typename T, bool VEC>
 cudaError_t launch_back(const NormBackArgs &a, uint32_t grid, cudaStream_t st) {
-    const Split s = split_row(a.dim);
+    const Split s = split_row(a.dim, true);
     if (s.lanes) {
         if (s.chunks == 1) return launch_back<T, VEC, 1, false>(a, s, grid, st);
-        if (s.chunks == 2) return launch_back<T, VEC, 2, false>(a, s, grid, st);
-        return launch_back<T, VEC, 4, false>(a, s, grid, st);
+        return launch_back<T, VEC, 2, false>(a, s, grid, st);
     }
     if (s.chunks == 1) return launch_back<T, VEC, 1, true>(a, s, grid, st);
     if (s.chunks == 2) return launch_back<T, VEC, 2, true>(a, s, grid, st);
@@ -515,16 +628,17 @@ __global__ void k_scales_bad(const float *scales, uint64_t n, uint32_t *bad) {
         if (isnan(scales[i])) *bad = 1;
 }
 
-// A row a block, for rows of any length; encode_chunk does the work.
+// A row a block, for rows of any length; encode_columns does the work.
 __global__ void __launch_bounds__(kThreads)
 k_encode_rows(const float *src, uint64_t rows, uint32_t dim, uint64_t pitch, uint8_t *codes, float *scales) {
     const uint64_t per_row = (dim + kF8Block - 1) / kF8Block;
     for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x)
         for (uint32_t c0 = 0; c0 < dim; c0 += kThreads * kChunk) {
-            const uint32_t c = c0 + threadIdx.x * kChunk;
+            const uint32_t lane = threadIdx.x & 31;
+            const Columns<false> c(lane, 32, c0 / kChunk + (threadIdx.x & ~31u));
             float v[kChunk];
             unpack(load_chunk<float, false>(src + row * dim, c, dim), v);
-            encode_chunk(v, 32, c, dim, codes + row * pitch, scales + row * per_row);
+            encode_columns<false>(v, c, lane, 32, dim, codes + row * pitch, scales + row * per_row);
         }
 }
 }  // namespace
@@ -553,9 +667,12 @@ extern "C" int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64
     const uint64_t chunks = rows * ((dim + kChunk - 1) / kChunk);
     const uint32_t grid = (uint32_t)std::min<uint64_t>((chunks + kThreads - 1) / kThreads, 1u << 30);
     const bool vec = vec_rows(x, x_stride, elem_size(dtype)) && vec_rows(y, y_stride, elem_size(dtype));
+    const bool flat = dim % kChunk && (x_stride == dim || rows == 1) && (y_stride == dim || rows == 1) && vec_rows(x, 0, elem_size(dtype)) &&
+                      vec_rows(y, 0, elem_size(dtype)) && chunks < (1ull << 38);
     with_type(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (vec) k_dropout<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, rows, (uint32_t)dim, x_stride, y_stride, d);
+        if (flat) k_dropout_flat<T><<<(uint32_t)((chunks + kThreads - 1) / kThreads), kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, d);
+        else if (vec) k_dropout<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, rows, (uint32_t)dim, x_stride, y_stride, d);
         else k_dropout<T, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, rows, (uint32_t)dim, x_stride, y_stride, d);
     });
     AG_CUDA(cudaGetLastError());
@@ -585,7 +702,7 @@ extern "C" int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream) 
     a.y_stride = n->y_stride; a.h_stride = n->h_stride; a.code_stride = n->code_stride; a.dim = (uint32_t)n->dim;
     a.w_f32 = n->weight_dtype == AG_F32; a.plain = n->encode_only; a.eps = n->eps;
     const uint32_t e = elem_size(n->dtype);
-    const bool vec = vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.y, a.y_stride, e) && vec_rows(a.h, a.h_stride, e);
+    const bool vec = vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.y, a.y_stride, e) && vec_rows(a.h, a.h_stride, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -631,7 +748,7 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
     a.rows = n->rows; a.dim = (uint32_t)n->dim; a.dy_stride = n->dy_stride; a.dh_stride = n->dh_stride; a.h_stride = n->h_stride;
     a.w_f32 = n->weight_dtype == AG_F32;
     const uint32_t e = elem_size(n->dtype);
-    const bool vec = vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
+    const bool vec = vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
                      vec_rows(a.dx, a.dim, e) && vec_rows(a.dres, a.dim, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
