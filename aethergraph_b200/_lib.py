@@ -229,7 +229,7 @@ SIGNATURES = {
     "ag_rows_dropout": (C.c_int32, [_P, _P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64, C.c_int32, C.c_double, C.c_uint64,
                                     C.c_uint64, C.c_int32, _P]),
     "ag_rows_norm": (C.c_int32, [_P, C.c_int32, _P]),
-    "ag_rows_norm_backward_scratch": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_int32, _U64P]),
+    "ag_rows_norm_backward_scratch": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, _U64P]),
     "ag_rows_norm_backward": (C.c_int32, [_P, C.c_int32, _P]),
     "ag_rows_encode_weight": (C.c_int32, [_P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_int32, _P, C.c_uint64, _P, C.c_int32, _P]),
     "ag_rows_product": (C.c_int32, [_P, C.c_int32, _P]),

@@ -26,6 +26,29 @@ constexpr uint32_t kChunk = 8;
 constexpr float kE4M3Max = 448.0f;
 constexpr uint32_t kMaxNormDim = 16384;  // 512 threads x 4 chunks
 
+// Division of 32-bit numbers by a divisor that the host knows: one high product instead of a division
+// (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994, figure 4.1).
+struct Divide {
+    uint32_t by = 1, m = 1, s1 = 0, s2 = 0;
+    explicit Divide(uint32_t d) : by(d) {
+        uint32_t l = 0;
+        while (l < 32 && (1ull << l) < d) ++l;
+        m = (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+        s1 = l < 1 ? l : 1;
+        s2 = l ? l - 1 : 0;
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        const uint32_t t = __umulhi(m, n);
+        return (t + ((n - t) >> s1)) >> s2;
+    }
+    // Quotient and remainder of what may pass 32 bits.
+    __device__ __forceinline__ uint64_t operator()(uint64_t n, uint32_t &rest) const {
+        const uint64_t q = n <= 0xFFFFFFFFull ? (*this)((uint32_t)n) : n / by;
+        rest = (uint32_t)(n - q * by);
+        return q;
+    }
+};
+
 // ------------------------------------------------------------ row access --
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
@@ -130,7 +153,8 @@ template <typename T, bool VEC> __device__ __forceinline__ void load_weight(cons
 
 // ---------------------------------------------------------------- dropout --
 struct Drop {
-    uint32_t threshold;  // an element stays iff its 16 random bits are at least this; 0: no dropout, 65536: nothing stays
+    uint32_t on;   // 0: no dropout
+    uint32_t bar;  // an element stays iff its 16 random bits, moved to the upper half of a word, are above (T << 16) - 1
     float scale;
     uint64_t seed, offset;
 };
@@ -138,12 +162,14 @@ struct Drop {
 __device__ __forceinline__ uint4 lots_of(const Drop &d, uint64_t row, uint32_t chunk) {
     return philox4x32_10(d.seed, (uint32_t)d.offset, row << 32 | chunk, (uint32_t)(d.offset >> 32));
 }
-__device__ __forceinline__ uint32_t lot(const uint4 &r, uint32_t i) {  // i is a constant where this is used
+// Bits of element i of a chunk; i is a constant where this is used.  The lower bits of an odd element's
+// word stay: they cannot lift it over the bar, which ends in ones.
+__device__ __forceinline__ uint32_t lot(const uint4 &r, uint32_t i) {
     const uint32_t w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
-    return i & 1 ? w >> 16 : w & 0xFFFFu;
+    return i & 1 ? w : w << 16;
 }
 // A select: a dropped infinity or NaN is gone.
-__device__ __forceinline__ float kept(const Drop &d, uint32_t u, float v) { return u >= d.threshold ? v * d.scale : 0.f; }
+__device__ __forceinline__ float kept(const Drop &d, uint32_t bits, float v) { return bits > d.bar ? v * d.scale : 0.f; }
 
 // Dropout of a thread's eight columns.  Unless they are a chunk, the group's lanes make the lots of one
 // chunk each and pass them around in shared memory (16 bytes a lane); the whole warp calls this.
@@ -159,82 +185,87 @@ __device__ __forceinline__ void drop_columns(const Drop &d, uint64_t row, uint32
         __syncwarp();
         const uint16_t *group = (const uint16_t *)(warp_lots + ((threadIdx.x & 31) - lane));
 #pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) v[i] = kept(d, group[lane + i * lanes], v[i]);
+        for (uint32_t i = 0; i < kChunk; ++i) v[i] = kept(d, (uint32_t)group[lane + i * lanes] << 16, v[i]);
     }
 }
 
 constexpr int kThreads = 256;
 
-// A thread per chunk.
+// Two chunks a thread, a block's width apart; both loads are in flight before either is used.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-k_dropout(const T *x, T *y, uint64_t rows, uint32_t dim, uint64_t x_stride, uint64_t y_stride, Drop d) {
-    const uint32_t chunks = (dim + kChunk - 1) / kChunk;
-    const uint64_t total = rows * chunks;
-    for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < total; i += (uint64_t)gridDim.x * kThreads) {
-        const uint64_t row = i / chunks;
-        const uint32_t chunk = (uint32_t)(i - row * chunks), c = chunk * kChunk;
+k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_t x_stride, uint64_t y_stride, Drop d) {
+    Raw<T> r[2];
+    uint64_t row[2];
+    uint32_t chunk[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const uint64_t i = ((uint64_t)blockIdx.x * 2 + u) * kThreads + threadIdx.x;
+        row[u] = chunks(i, chunk[u]);
+        if (i < total) r[u] = load_chunk<T, VEC>(x + row[u] * x_stride, Columns<VEC>(0, 1, chunk[u]), dim);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        if (((uint64_t)blockIdx.x * 2 + u) * kThreads + threadIdx.x >= total) break;
+        const uint4 lots = lots_of(d, row[u], chunk[u]);
         float v[kChunk];
-        if (VEC && c + kChunk <= dim) {
-            Raw<T> r;
-            load_words(r, x + row * x_stride + c);
-            unpack(r, v);
-        } else {
+        unpack(r[u], v);
 #pragma unroll
-            for (uint32_t e = 0; e < kChunk; ++e) v[e] = c + e < dim ? to_f32(x[row * x_stride + c + e]) : 0.f;
-        }
-        const uint4 r = lots_of(d, row, chunk);
-#pragma unroll
-        for (uint32_t e = 0; e < kChunk; ++e) v[e] = kept(d, lot(r, e), v[e]);
-        if (VEC && c + kChunk <= dim) {
-            store_words(pack<T>(v), y + row * y_stride + c);
-        } else {
-#pragma unroll
-            for (uint32_t e = 0; e < kChunk; ++e)
-                if (c + e < dim) y[row * y_stride + c + e] = from_f32<T>(v[e]);
-        }
+        for (uint32_t e = 0; e < kChunk; ++e) v[e] = kept(d, lot(lots, e), v[e]);
+        store_chunk<T, VEC>(y + row[u] * y_stride, Columns<VEC>(0, 1, chunk[u]), dim, v);
     }
 }
 
 // Contiguous rows whose length is no multiple of eight: the lots belong to chunks, the memory is walked
-// in aligned vectors of eight elements, whatever row they are in.  A block's 256 chunks cover one
-// run of elements; the threads leave a byte per element that says whether it stays, and read
-// eight of them back for their vector.  The vectors at the run's ends belong to two blocks, element by element.
+// in aligned vectors of eight elements, whatever row they are in.  A block takes 1024 vectors, four a
+// thread, and makes the lots of every chunk that reaches into them (those at its ends are made by two
+// blocks): a bit per element in shared memory says whether it stays.
+constexpr uint32_t kFlatVectors = 4, kFlatElements = kThreads * kFlatVectors * kChunk;
+constexpr uint64_t kFlatMaxDim = 1u << 28;  // positions within a block's rows fit 32 bits
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-k_dropout_flat(const T *x, T *y, uint64_t total, uint32_t dim, Drop d) {
-    __shared__ __align__(16) uint8_t stays[kThreads * kChunk + 16];
-    const uint32_t chunks = (dim + kChunk - 1) / kChunk;
-    const uint64_t i0 = blockIdx.x * (uint64_t)kThreads, i1 = min(i0 + kThreads, total);
-    auto element = [&](uint64_t i) { return i / chunks * dim + (uint32_t)(i % chunks) * kChunk; };
-    const uint64_t from = element(i0), to = element(i1), origin = from & ~(uint64_t)(kChunk - 1);
-    const uint64_t mine = origin + threadIdx.x * kChunk;
-    Raw<T> r{};
-    if (mine >= from && mine + kChunk <= to) load_words(r, x + mine);
-    const uint32_t rest = (uint32_t)(i0 % chunks) + threadIdx.x, over = rest / chunks, chunk = rest - over * chunks;
-    const uint64_t row = i0 / chunks + over;
-    if (i0 + threadIdx.x < i1) {
-        const uint4 lots = lots_of(d, row, chunk);
-        uint8_t *at = stays + (uint32_t)(row * dim + chunk * kChunk - origin);
-        const uint32_t len = min(kChunk, dim - chunk * kChunk);
+k_dropout_flat(const T *x, T *y, uint64_t total, Divide dim, Divide chunks, Drop d) {
+    __shared__ uint32_t stays[kFlatElements / 32];
+    for (uint32_t i = threadIdx.x; i < kFlatElements / 32; i += kThreads) stays[i] = 0;
+    const uint64_t origin = (uint64_t)blockIdx.x * kFlatElements, at = origin + threadIdx.x * kChunk;
+    const int end = (int)min(total - origin, (uint64_t)kFlatElements);
+    Raw<T> r[kFlatVectors];
 #pragma unroll
-        for (uint32_t e = 0; e < kChunk; ++e)
-            if (e < len) at[e] = lot(lots, e) >= d.threshold;
+    for (uint32_t j = 0; j < kFlatVectors; ++j)
+        if (at + j * kThreads * kChunk + kChunk <= total) load_words(r[j], x + at + j * kThreads * kChunk);
+    uint32_t c0;
+    const uint64_t row0 = dim(origin, c0);
+    __syncthreads();
+    for (uint32_t k = c0 / kChunk + threadIdx.x;; k += kThreads) {
+        const uint32_t over = chunks(k), chunk = k - over * chunks.by;
+        int pos = (int)(over * dim.by + chunk * kChunk - c0);  // of the chunk's first element, from the origin
+        if (pos >= end) break;
+        const uint4 lots = lots_of(d, row0 + over, chunk);
+        uint32_t m = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < kChunk; ++e) m |= (uint32_t)(lot(lots, e) > d.bar) << e;
+        const uint32_t len = dim.by - chunk * kChunk;
+        if (len < kChunk) m &= (1u << len) - 1;
+        if (pos < 0) { m >>= -pos; pos = 0; }
+        const uint32_t word = (uint32_t)pos / 32, shift = pos % 32;
+        atomicOr(&stays[word], m << shift);
+        if (shift > 32 - kChunk && word + 1 < kFlatElements / 32) atomicOr(&stays[word + 1], m >> (32 - shift));
     }
     __syncthreads();
-    for (uint64_t f = mine; f < to; f += kThreads * kChunk) {
-        const uint8_t *at = stays + (uint32_t)(f - origin);
-        if (f >= from && f + kChunk <= to) {
-            if (f != mine) load_words(r, x + f);
-            const uint2 flags = *(const uint2 *)at;
-            float v[kChunk];
-            unpack(r, v);
 #pragma unroll
-            for (uint32_t e = 0; e < kChunk; ++e) v[e] = (e < 4 ? flags.x : flags.y) >> (8 * (e & 3)) & 1 ? v[e] * d.scale : 0.f;
+    for (uint32_t j = 0; j < kFlatVectors; ++j) {
+        const uint64_t f = at + j * kThreads * kChunk;
+        if (f >= total) break;
+        const uint32_t m = ((const uint8_t *)stays)[threadIdx.x + j * kThreads];
+        if (f + kChunk <= total) {
+            float v[kChunk];
+            unpack(r[j], v);
+#pragma unroll
+            for (uint32_t e = 0; e < kChunk; ++e) v[e] = m >> e & 1 ? v[e] * d.scale : 0.f;
             store_words(pack<T>(v), y + f);
         } else {
-            for (uint32_t e = 0; e < kChunk; ++e)
-                if (f + e >= from && f + e < to) y[f + e] = at[e] ? from_f32<T>(to_f32(x[f + e]) * d.scale) : from_f32<T>(0.f);
+            for (uint32_t e = 0; f + e < total; ++e) y[f + e] = from_f32<T>(m >> e & 1 ? to_f32(x[f + e]) * d.scale : 0.f);
         }
     }
 }
@@ -249,15 +280,18 @@ struct NormArgs {
     uint64_t rows, x_stride, res_stride, y_stride, h_stride, code_stride;
     uint32_t dim;
     int w_f32, plain;  // plain: no norm, the rows themselves are encoded
-    float eps;
+    float eps, inv_dim;
     Drop drop;
 };
 
 // Sum over the `lanes` (power of two, at most 32) of a row's group, or over the whole block.
-template <bool BLOCK> __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float *shared) {
-    for (uint32_t o = (BLOCK ? 32 : lanes) / 2; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+// AGAIN: the block calls it once more, so the sums of this time must have been read by then.
+template <bool BLOCK, bool AGAIN> __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float *shared) {
+#pragma unroll
+    for (uint32_t o = 16; o > 0; o /= 2)
+        if (BLOCK || o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (BLOCK) {
-        __syncthreads();  // the previous row's sum has been read
+        if (AGAIN) __syncthreads();
         if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
         __syncthreads();
         v = 0.f;
@@ -269,12 +303,13 @@ template <bool BLOCK> __device__ __forceinline__ float row_sum(float v, uint32_t
 // Scale of a block of 128 columns whose largest magnitude has the bits `top` (as bits NaN lies above
 // infinity above every number), and its reciprocal.  The scale puts that magnitude on 448; a block with an infinity or
 // NaN gets a NaN scale, so that every value read from it is NaN.  At least the least normal
-// f32, so that the reciprocal is finite.  Reciprocal and product are rounded once each: a code is
-// off by half a step and 2^-23 of the value.
+// f32, so that the reciprocal is finite.  Its approximation is good to one step and products are
+// rounded once: a code is off by half a step and 2^-22 of the value.
 __device__ __forceinline__ float scale_of(uint32_t top, float &inv) {
     const bool bad = top >= 0x7F800000u;
-    const float scale = bad ? __uint_as_float(0x7FC00000u) : fmaxf(__uint_as_float(top) / kE4M3Max, 1.17549435e-38f);
-    inv = bad ? 0.f : 1.f / scale;
+    const float scale = bad ? __uint_as_float(0x7FC00000u) : fmaxf(__uint_as_float(top) * (1.f / kE4M3Max), 1.17549435e-38f);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+    if (bad) inv = 0.f;
     return scale;
 }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
@@ -289,7 +324,9 @@ __device__ __forceinline__ void encode_columns(const float v[kChunk], const Colu
         uint32_t top = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i) top = max(top, magnitude(v[i]));
-        for (uint32_t o = min(lanes, kF8Block / kChunk) / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        #pragma unroll
+        for (uint32_t o = 8; o > 0; o /= 2)
+            if (o < lanes) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (c.first >= dim) return;
         float inv;
         const float scale = scale_of(top, inv);
@@ -301,7 +338,9 @@ __device__ __forceinline__ void encode_columns(const float v[kChunk], const Colu
 #pragma unroll
         for (uint32_t i = 0; i < kChunk / 2; ++i) { lo = max(lo, magnitude(v[i])); hi = max(hi, magnitude(v[i + kChunk / 2])); }
         if (lanes < 32) lo = hi = max(lo, hi);
-        for (uint32_t o = lanes / 2; o > 0; o /= 2) {
+#pragma unroll
+        for (uint32_t o = 16; o > 0; o /= 2) {
+            if (o >= lanes) continue;
             lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, o));
             hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
@@ -320,13 +359,14 @@ __device__ __forceinline__ void encode_columns(const float v[kChunk], const Colu
 // h = res + dropout(x); y = h rsqrt(mean(h^2) + eps) w.  `lanes` lanes a row (BLOCK: the whole
 // block), C chunks each; the row stays in registers between the sum and the output.
 template <typename T, bool VEC, int C, bool BLOCK, bool F8>
-__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : C == 1 ? 5 : C == 2 ? 4 : 2)
-k_norm(const NormArgs a, uint32_t lanes) {
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : C == 1 ? 5 : 4)
+k_norm(const NormArgs a, uint32_t log2_lanes) {
+    const uint32_t lanes = C > 1 || BLOCK ? 32 : 1u << log2_lanes;  // more chunks than one: all lanes
     __shared__ float shared[32];
     __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
     uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
     const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
-    const uint64_t row = BLOCK ? blockIdx.x : (uint64_t)blockIdx.x * (blockDim.x / lanes) + threadIdx.x / lanes;
+    const uint64_t row = BLOCK ? blockIdx.x : (uint64_t)blockIdx.x * (kThreads >> log2_lanes) + (threadIdx.x >> log2_lanes);
     const uint32_t dim = row < a.rows ? a.dim : 0;  // lanes without a row still take part in the exchanges
     float v[C][kChunk];
     {
@@ -345,7 +385,7 @@ k_norm(const NormArgs a, uint32_t lanes) {
 #pragma unroll
             for (uint32_t i = 0; i < kChunk; ++i) v[j][i] = 0.f;
             if (c.first < dim) unpack(rx[j], v[j]);
-            if (a.drop.threshold) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, v[j]);
+            if (a.drop.on) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, v[j]);
             if (a.res && c.first < dim) {
                 float r[kChunk];
                 unpack(rr[j], r);
@@ -363,7 +403,7 @@ k_norm(const NormArgs a, uint32_t lanes) {
         for (uint32_t i = 0; i < kChunk; ++i) sum += v[j][i] * v[j][i];
     }
     if (!a.plain) {
-        const float rstd = rsqrtf(row_sum<BLOCK>(sum, lanes, shared) / (float)a.dim + a.eps);
+        const float rstd = rsqrtf(row_sum<BLOCK, false>(sum, lanes, shared) * a.inv_dim + a.eps);
         if (a.rstd && dim && (BLOCK ? threadIdx.x : lane) == 0) a.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -391,6 +431,7 @@ struct NormBackArgs {
     uint64_t rows, dy_stride, dh_stride, h_stride;
     uint32_t dim;
     int w_f32;
+    float inv_dim;
     Drop drop;
 };
 
@@ -400,20 +441,21 @@ struct NormBackArgs {
 // No atomics: the same bits every time on the same GPU.
 template <typename T, bool VEC, int C, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : C == 1 ? 4 : 2)
-k_norm_back(const NormBackArgs a, uint32_t lanes) {
+k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
+    const uint32_t lanes = C > 1 || BLOCK ? 32 : 1u << log2_lanes;
     __shared__ float shared[32];
     __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
     extern __shared__ float sums[];  // [groups of the block][dim], not BLOCK
     uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
     const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
-    const uint64_t per_block = BLOCK ? 1 : blockDim.x / lanes;
+    const uint64_t per_block = BLOCK ? 1 : kThreads >> log2_lanes;
     float dw[C][kChunk];
 #pragma unroll
     for (int j = 0; j < C; ++j)
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i) dw[j][i] = 0.f;
     for (uint64_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block) {
-        const uint64_t row = base + (BLOCK ? 0 : threadIdx.x / lanes);
+        const uint64_t row = base + (BLOCK ? 0 : threadIdx.x >> log2_lanes);
         const uint32_t dim = row < a.rows ? a.dim : 0;
         Raw<T> ry[C], rh[C], rd[C];
 #pragma unroll
@@ -442,7 +484,7 @@ k_norm_back(const NormBackArgs a, uint32_t lanes) {
                 sum += gh * w[i];
             }
         }
-        const float coef = row_sum<BLOCK>(sum, lanes, shared) * rstd * rstd * rstd / (float)a.dim;
+        const float coef = row_sum<BLOCK, true>(sum, lanes, shared) * rstd * rstd * rstd * a.inv_dim;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const uint32_t step = j * width + group_chunk;
@@ -456,7 +498,7 @@ k_norm_back(const NormBackArgs a, uint32_t lanes) {
             for (uint32_t i = 0; i < kChunk; ++i) t[i] += rstd * (g[i] * w[i]) - h[i] * coef;
             if (a.dres && c.first < dim) store_chunk<T, VEC>((T *)a.dres + row * a.dim, c, dim, t);
             if (a.dx) {
-                if (a.drop.threshold) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, t);
+                if (a.drop.on) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, t);
                 if (c.first < dim) store_chunk<T, VEC>((T *)a.dx + row * a.dim, c, dim, t);
             }
         }
@@ -466,7 +508,7 @@ k_norm_back(const NormBackArgs a, uint32_t lanes) {
 #pragma unroll
     for (int j = 0; j < C; ++j) {
         const Columns<VEC> c(lane, lanes, j * width + group_chunk);
-        float *to = BLOCK ? mine : sums + threadIdx.x / lanes * a.dim;
+        float *to = BLOCK ? mine : sums + (threadIdx.x >> log2_lanes) * a.dim;
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
             if (c.at(i) < a.dim) to[c.at(i)] = dw[j][i];
@@ -480,22 +522,24 @@ k_norm_back(const NormBackArgs a, uint32_t lanes) {
     }
 }
 
-// dw[c] = sum of the blocks' partial sums, 32 columns a block, 16 slices of blocks each.
+// dw[c] = sum of the blocks' partial sums, 32 columns a block, 32 slices of blocks each.
 template <typename T>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(1024)
 k_norm_dw(const float *partial, uint32_t blocks, uint32_t dim, T *dw) {
-    __shared__ float sums[16][32];
+    __shared__ float sums[32][33];
     const uint32_t c = blockIdx.x * 32 + threadIdx.x;
     float s = 0.f;
-    if (c < dim)
-        for (uint32_t b = threadIdx.y; b < blocks; b += 16) s += partial[(uint64_t)b * dim + c];
+    if (c < dim) {
+#pragma unroll 8
+        for (uint32_t b = threadIdx.y; b < blocks; b += 32) s += partial[(uint64_t)b * dim + c];
+    }
     sums[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.y == 0 && c < dim) {
-        s = 0.f;
-        for (int q = 0; q < 16; ++q) s += sums[q][threadIdx.x];
-        dw[c] = from_f32<T>(s);
-    }
+    s = sums[threadIdx.x][threadIdx.y];  // column threadIdx.y of the 32, slice threadIdx.x
+#pragma unroll
+    for (uint32_t o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const uint32_t out = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && out < dim) dw[out] = from_f32<T>(s);
 }
 
 // ---------------------------------------------------- weights in 8 bits --
@@ -543,8 +587,10 @@ template <typename F> void with_type(int dtype, F f) {
 
 int32_t make_drop(double p, uint64_t seed, uint64_t offset, Drop *d) {
     if (!(p >= 0.0 && p <= 1.0)) return fail(AG_ERR_VALUE, "dropout probability must be in [0, 1], got %g", p);
-    d->threshold = (uint32_t)std::floor(p * 65536.0 + 0.5);
-    d->scale = d->threshold < 65536 ? 65536.0f / (65536 - d->threshold) : 0.0f;
+    const uint32_t t = (uint32_t)std::floor(p * 65536.0 + 0.5);
+    d->on = t != 0;
+    d->bar = (uint32_t)(((uint64_t)t << 16) - 1);  // t = 65536: nothing is above
+    d->scale = t < 65536 ? 65536.0f / (65536 - t) : 0.0f;
     d->seed = seed; d->offset = offset;
     return AG_OK;
 }
@@ -557,32 +603,41 @@ int32_t check_rows(const char *who, uint64_t rows, uint64_t dim, int32_t dtype) 
 }
 
 // How a row of `dim` columns is shared out: `lanes` of a warp (0: a whole block of `threads`) with up to
-// `chunks` chunks each.  The backward pass holds three rows and the weights' sums at once, so
-// it goes over to whole blocks at half the length.
-struct Split { uint32_t lanes, threads; int chunks; };
-Split split_row(uint32_t dim, bool backward) {
+// `chunks` chunks each.  Whole blocks: as few threads as hold the row in
+// `most` chunks each (64 bytes of f16 / bf16 or f32: a thread's loads are all in flight together, and the sum
+// waits for fewer warps), unless that leaves many of them idle.
+struct Split {
+    uint32_t lanes, threads;
+    int chunks;
+    uint32_t log2_lanes() const { uint32_t l = 0; while ((1u << l) < lanes) ++l; return lanes ? l : 5; }
+};
+Split split_row(uint32_t dim, int dtype) {
     const uint32_t n = (dim + kChunk - 1) / kChunk;
     Split s{1, kThreads, 1};
-    if (n <= (backward ? 64u : 128u)) {
+    if (n <= 64) {
         while (s.lanes < 32 && s.lanes < n) s.lanes *= 2;
         while ((uint32_t)s.chunks * s.lanes < n) s.chunks *= 2;
-    } else {
-        s.lanes = 0;
-        while ((uint32_t)s.chunks * 512 < n) s.chunks *= 2;
-        s.threads = (n + 32 * s.chunks - 1) / (32 * s.chunks) * 32;
+        return s;
     }
+    s.lanes = 0;
+    uint32_t slots = 0xFFFFFFFFu;
+    for (int c = dtype == AG_F32 ? 2 : 4; c; c /= 2) {
+        const uint32_t threads = (n + 32 * c - 1) / (32 * c) * 32;
+        if (threads > 512 || threads * c + threads * c / 8 >= slots) continue;
+        slots = threads * c; s.threads = threads; s.chunks = c;
+    }
+    if (slots == 0xFFFFFFFFu) { s.chunks = 4; s.threads = 512; }
     return s;
 }
 
 template <typename T, bool VEC, bool F8>
-cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
-    const Split s = split_row(a.dim, false);
+cudaError_t launch_norm(const NormArgs &a, int dtype, cudaStream_t st) {
+    const Split s = split_row(a.dim, dtype);
     const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
-    const uint32_t grid = (uint32_t)((a.rows + per - 1) / per), lanes = s.lanes ? s.lanes : 32;  // rows of a whole block are 2 KB and more
+    const uint32_t grid = (uint32_t)((a.rows + per - 1) / per), lanes = s.log2_lanes();  // rows of a whole block are 2 KB and more
     if (s.lanes) {
         if (s.chunks == 1) k_norm<T, VEC, 1, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
-        else if (s.chunks == 2) k_norm<T, VEC, 2, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
-        else k_norm<T, VEC, 4, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+        else k_norm<T, VEC, 2, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
     } else {
         if (s.chunks == 1) k_norm<T, VEC, 1, true, F8><<<grid, s.threads, 0, st>>>(a, lanes);
         else if (s.chunks == 2) k_norm<T, VEC, 2, true, F8><<<grid, s.threads, 0, st>>>(a, lanes);
@@ -591,22 +646,31 @@ cudaError_t launch_norm(const NormArgs &a, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-uint32_t back_blocks(uint64_t rows, uint32_t dim) {
-    const Split s = split_row(dim, true);
+// Blocks of the backward pass: those that are resident together, `per_sm` of them on each SM, and no more
+// than there are rows for.
+uint32_t back_blocks(uint64_t rows, const Split &s, uint32_t per_sm) {
     const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
-    return (uint32_t)std::min<uint64_t>((rows + per - 1) / per, (uint64_t)kSMs * (2048 / s.threads) / 2);
+    return (uint32_t)std::min<uint64_t>((rows + per - 1) / per, (uint64_t)kSMs * per_sm);
+}
+uint32_t back_blocks_bound(uint64_t rows, uint32_t dim, int dtype) {
+    const Split s = split_row(dim, dtype);
+    return back_blocks(rows, s, std::min(2048 / s.threads, 32u));
 }
 
 template <typename T, bool VEC, int C, bool BLOCK>
-cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t grid, cudaStream_t st) {
+cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t &grid, cudaStream_t st) {
     const size_t shared = BLOCK || !a.partial ? 0 : (size_t)(s.threads / s.lanes) * a.dim * 4;
-    k_norm_back<T, VEC, C, BLOCK><<<grid, s.threads, shared, st>>>(a, s.lanes ? s.lanes : 32);
+    int per_sm = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, VEC, C, BLOCK>, (int)s.threads, shared);
+    if (e != cudaSuccess) return e;
+    grid = back_blocks(a.rows, s, std::max(1, per_sm));
+    k_norm_back<T, VEC, C, BLOCK><<<grid, s.threads, shared, st>>>(a, s.log2_lanes());
     return cudaGetLastError();
 }
 
 template <typename T, bool VEC>
-cudaError_t launch_back(const NormBackArgs &a, uint32_t grid, cudaStream_t st) {
-    const Split s = split_row(a.dim, true);
+cudaError_t launch_back(const NormBackArgs &a, int dtype, uint32_t &grid, cudaStream_t st) {
+    const Split s = split_row(a.dim, dtype);
     if (s.lanes) {
         if (s.chunks == 1) return launch_back<T, VEC, 1, false>(a, s, grid, st);
         return launch_back<T, VEC, 2, false>(a, s, grid, st);
@@ -664,16 +728,25 @@ extern "C" int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64
     if (y_stride < dim) return fail(AG_ERR_VALUE, "ag_rows_dropout: rows of the output overlap");
     DeviceGuard guard(device);
     if (!guard.ok) return AG_ERR_CUDA;
-    const uint64_t chunks = rows * ((dim + kChunk - 1) / kChunk);
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((chunks + kThreads - 1) / kThreads, 1u << 30);
+    const Divide by((uint32_t)((dim + kChunk - 1) / kChunk));
+    const uint64_t chunks = rows * by.by;
+    if (chunks >= (1ull << 38)) return fail(AG_ERR_VALUE, "ag_rows_dropout: too many rows of this length");  // beyond any memory
+    if (!d.on) {
+        if (x != y)
+            AG_CUDA(cudaMemcpy2DAsync(y, y_stride * elem_size(dtype), x, x_stride * elem_size(dtype), dim * elem_size(dtype), rows,
+                                      cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
+        return AG_OK;
+    }
+    const uint32_t grid = (uint32_t)((chunks + 2 * kThreads - 1) / (2 * kThreads));
     const bool vec = vec_rows(x, x_stride, elem_size(dtype)) && vec_rows(y, y_stride, elem_size(dtype));
-    const bool flat = dim % kChunk && (x_stride == dim || rows == 1) && (y_stride == dim || rows == 1) && vec_rows(x, 0, elem_size(dtype)) &&
-                      vec_rows(y, 0, elem_size(dtype)) && chunks < (1ull << 38);
+    const bool flat = dim % kChunk && dim < kFlatMaxDim && (x_stride == dim || rows == 1) && (y_stride == dim || rows == 1) && vec_rows(x, 0, elem_size(dtype)) &&
+                      vec_rows(y, 0, elem_size(dtype));
     with_type(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (flat) k_dropout_flat<T><<<(uint32_t)((chunks + kThreads - 1) / kThreads), kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, d);
-        else if (vec) k_dropout<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, rows, (uint32_t)dim, x_stride, y_stride, d);
-        else k_dropout<T, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, rows, (uint32_t)dim, x_stride, y_stride, d);
+        if (flat) k_dropout_flat<T><<<(uint32_t)((rows * dim + kFlatElements - 1) / kFlatElements), kThreads, 0, (cudaStream_t)stream>>>(
+            (const T *)x, (T *)y, rows * dim, Divide((uint32_t)dim), by, d);
+        else if (vec) k_dropout<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
+        else k_dropout<T, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
     });
     AG_CUDA(cudaGetLastError());
     return AG_OK;
@@ -690,7 +763,7 @@ extern "C" int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream) 
     if (n->rows == 0) return AG_OK;
     if (!n->x || (!n->y && !n->codes) || (n->codes && !n->scales)) return fail(AG_ERR_VALUE, "ag_rows_norm: null argument");
     if (n->y && n->codes) return fail(AG_ERR_VALUE, "ag_rows_norm: either rows of their own type or 8-bit rows come out");
-    if (n->encode_only && (!n->codes || n->residual || n->weight || n->h || a.drop.threshold))
+    if (n->encode_only && (!n->codes || n->residual || n->weight || n->h || a.drop.on))
         return fail(AG_ERR_VALUE, "ag_rows_norm: encoding alone takes rows and gives 8-bit rows");
     if (n->codes && (n->code_stride % 16 != 0 || n->code_stride < n->dim || (uintptr_t)n->codes % 16 != 0))
         return fail(AG_ERR_VALUE, "ag_rows_norm: 8-bit rows start on multiples of 16 bytes and do not overlap");
@@ -700,27 +773,27 @@ extern "C" int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream) 
     a.x = n->x; a.res = n->residual; a.weight = n->weight; a.y = n->y; a.h = n->h; a.rstd = n->rstd;
     a.codes = (uint8_t *)n->codes; a.scales = n->scales; a.rows = n->rows; a.x_stride = n->x_stride; a.res_stride = n->residual_stride;
     a.y_stride = n->y_stride; a.h_stride = n->h_stride; a.code_stride = n->code_stride; a.dim = (uint32_t)n->dim;
-    a.w_f32 = n->weight_dtype == AG_F32; a.plain = n->encode_only; a.eps = n->eps;
+    a.w_f32 = n->weight_dtype == AG_F32; a.plain = n->encode_only; a.eps = n->eps; a.inv_dim = 1.0f / (float)n->dim;
     const uint32_t e = elem_size(n->dtype);
     const bool vec = vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.y, a.y_stride, e) && vec_rows(a.h, a.h_stride, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         cudaStream_t st = (cudaStream_t)stream;
-        if (a.codes) err = vec ? launch_norm<T, true, true>(a, st) : launch_norm<T, false, true>(a, st);
-        else err = vec ? launch_norm<T, true, false>(a, st) : launch_norm<T, false, false>(a, st);
+        if (a.codes) err = vec ? launch_norm<T, true, true>(a, n->dtype, st) : launch_norm<T, false, true>(a, n->dtype, st);
+        else err = vec ? launch_norm<T, true, false>(a, n->dtype, st) : launch_norm<T, false, false>(a, n->dtype, st);
     });
     AG_CUDA(err);
     return AG_OK;
 }
 
-extern "C" int32_t ag_rows_norm_backward_scratch(uint64_t rows, uint64_t dim, int32_t device, uint64_t *bytes) {
+extern "C" int32_t ag_rows_norm_backward_scratch(uint64_t rows, uint64_t dim, int32_t dtype, int32_t device, uint64_t *bytes) {
     if (!bytes) return fail(AG_ERR_VALUE, "ag_rows_norm_backward_scratch: null argument");
     *bytes = 0;
     if (rows == 0 || dim == 0 || dim > kMaxNormDim) return AG_OK;
     DeviceGuard guard(device);
     if (!guard.ok) return AG_ERR_CUDA;
-    *bytes = (uint64_t)back_blocks(rows, (uint32_t)dim) * dim * 4;
+    *bytes = (uint64_t)back_blocks_bound(rows, (uint32_t)dim, dtype) * dim * 4;
     return AG_OK;
 }
 
@@ -739,27 +812,27 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
         return AG_OK;
     }
     if (!n->h || !n->rstd || (n->dw && !n->scratch)) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: null argument");
-    const uint32_t grid = back_blocks(n->rows, (uint32_t)n->dim);
+    uint32_t grid = back_blocks_bound(n->rows, (uint32_t)n->dim, n->dtype);
     if (n->dw && n->scratch_bytes < (uint64_t)grid * n->dim * 4)
         return fail(AG_ERR_VALUE, "ag_rows_norm_backward: %llu bytes of scratch, %llu are needed", (unsigned long long)n->scratch_bytes,
                     (unsigned long long)grid * n->dim * 4);
     a.dy = n->dy; a.dh = n->dh; a.h = n->h; a.weight = n->weight; a.rstd = n->rstd; a.dx = n->dx; a.dres = n->dresidual;
     a.partial = n->dw ? (float *)n->scratch : nullptr;
     a.rows = n->rows; a.dim = (uint32_t)n->dim; a.dy_stride = n->dy_stride; a.dh_stride = n->dh_stride; a.h_stride = n->h_stride;
-    a.w_f32 = n->weight_dtype == AG_F32;
+    a.w_f32 = n->weight_dtype == AG_F32; a.inv_dim = 1.0f / (float)n->dim;
     const uint32_t e = elem_size(n->dtype);
     const bool vec = vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
                      vec_rows(a.dx, a.dim, e) && vec_rows(a.dres, a.dim, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        err = vec ? launch_back<T, true>(a, grid, (cudaStream_t)stream) : launch_back<T, false>(a, grid, (cudaStream_t)stream);
+        err = vec ? launch_back<T, true>(a, n->dtype, grid, (cudaStream_t)stream) : launch_back<T, false>(a, n->dtype, grid, (cudaStream_t)stream);
     });
     AG_CUDA(err);
     if (n->dw)
         with_type(n->weight_dtype, [&](auto *t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            k_norm_dw<T><<<((uint32_t)n->dim + 31) / 32, dim3(32, 16), 0, (cudaStream_t)stream>>>((const float *)n->scratch, grid, (uint32_t)n->dim, (T *)n->dw);
+            k_norm_dw<T><<<((uint32_t)n->dim + 31) / 32, dim3(32, 32), 0, (cudaStream_t)stream>>>((const float *)n->scratch, grid, (uint32_t)n->dim, (T *)n->dw);
         });
     AG_CUDA(cudaGetLastError());
     return AG_OK;

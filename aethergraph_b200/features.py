@@ -125,11 +125,10 @@ class FeatureStore:
 
         from . import ops
 
-        ops._check_f8(codes, scales, "codes", 1)
+        rows, dim, pitch, index = ops._check_f8(codes, scales, "codes", 1)
         torch.cuda.current_stream(codes.device).synchronize()
         out = C.c_void_p()
-        _lib.check(_lib.lib().ag_features_from_f8(codes.data_ptr() or None, scales.data_ptr() or None, codes.shape[0], codes.shape[1],
-                                                  codes.stride(0), codes.device.index, C.byref(out)))
+        _lib.check(_lib.lib().ag_features_from_f8(codes.data_ptr() or None, scales.data_ptr() or None, rows, dim, pitch, index, C.byref(out)))
         store = FeatureStore(out.value)
         store._keep = (codes, scales)
         return store

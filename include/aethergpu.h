@@ -735,7 +735,8 @@ typedef struct {
     double p;
     int32_t dtype, weight_dtype;
 } ag_norm_grad;
-int32_t ag_rows_norm_backward_scratch(uint64_t rows, uint64_t dim, int32_t device, uint64_t *bytes);
+int32_t ag_rows_norm_backward_scratch(uint64_t rows, uint64_t dim, int32_t dtype, int32_t device,
+                                      uint64_t *bytes);
 int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, void *stream);
 /* Weights [out, dim] as e4m3 codes (pitch as above) with one scale per 128 x 128 block, f32
  * [ceil(out / 128), ceil(dim / 128)]. */
