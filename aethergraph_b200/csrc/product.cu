@@ -106,17 +106,21 @@ k_product_dot(ProductArgs a) {
 // the epilogue warps fold each step into their sums in registers, times the row's and the weights'
 // scale.  Roles: warp 0 loads (TMA, rows by id through tile::gather4), one thread of warp 1 issues
 // tcgen05.mma (K = 32 each) and the commits, warps 4 - 11 read TMEM (a warp can reach only the 32 lanes
-// of its number mod 4, so two warps share a quarter of the rows and split the columns).
+// of its number mod 4, so two warps share a quarter of the rows and split the columns).  Warps 2 and 3 copy
+// the rows' scales into shared memory, eight steps at a time (cp.async): a row's scales lie side by side in
+// memory, so an epilogue warp that loaded its 32 rows' scale of one step itself would touch 32 lines.
 //
 // Every wait is bounded.  A role whose wait runs out marks the block dead and the sticky error
 // word; all roles then leave their loops, copies and multiplications in flight are waited for
 // (bounded too) and TMEM is freed.
 constexpr int kBM = 128, kBK = 128, kAccStages = 4, kTileThreads = 384;
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
+constexpr long long kWaitLimit = 4000000000ll;  // clocks, two seconds
 
-constexpr int load_stages(int bn) { return bn >= 128 ? 6 : 8; }
+constexpr int kScaleSteps = 8, kScalePitch = kBM + 4, kScaleBytes = kScaleSteps * kScalePitch * 4;  // the pitch keeps a copy's lanes on 32 banks
+constexpr int load_stages(int bn) { return bn >= 128 ? 5 : 7; }
 constexpr int stage_bytes(int bn) { return (kBM + bn) * kBK; }
-constexpr int tile_shared(int bn) { return load_stages(bn) * stage_bytes(bn) + 1024 + 256; }
+constexpr int kOutBytes = 8 * 32 * 128;  // each epilogue warp: 32 rows of 128 bytes on their way out
+constexpr int tile_shared(int bn) { return load_stages(bn) * stage_bytes(bn) + kOutBytes + 2 * kScaleBytes + 1024 + 256; }
 
 struct TileArgs {
     ProductArgs p;
@@ -134,19 +138,17 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
 // Waits for the barrier's phase; false when the block is dead or the time ran out (which marks it dead).
+// The clock is looked at now and then only, and it is the SM's own: reading the global timer after
+// every failed try took longer than what is waited for.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *dead) {
     if (mbar_try(bar, parity)) return true;
-    const uint64_t until = now_ns() + kWaitLimitNs;
-    for (;;) {
+    const long long since = clock64();
+    for (uint32_t i = 1;; ++i) {
         if (mbar_try(bar, parity)) return true;
+        if (i % 64) continue;
         if (*dead) return false;
-        if (now_ns() > until) {
+        if (clock64() - since > kWaitLimit) {
             *dead = 1;
             atomicOr(&g_rows_error, kErrSpinTimeout);
             return false;
@@ -155,8 +157,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 }
 // The same for what is already in flight when a dead block ends.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
-    const uint64_t until = now_ns() + kWaitLimitNs;
-    while (!mbar_try(bar, parity) && now_ns() < until) {}
+    const long long since = clock64();
+    while (!mbar_try(bar, parity) && clock64() - since < kWaitLimit) {}
 }
 __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t x, int32_t y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -165,6 +167,11 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap *map, u
 __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t x, int4 rows) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
                  :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(is));
+    return is != 0;
 }
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
@@ -212,31 +219,66 @@ template <> __device__ __forceinline__ float round_to<float>(float v) { return v
 template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// COLS sums of one output row from column n on.
+// What an epilogue warp holds of its tile, 32 rows x COLS columns, a row a thread, leaves through
+// shared memory: a thread's own row in 16-byte pieces would touch 32 sectors half by half in every store; rows
+// of up to 128 bytes one beside the other fill them.  Piece j of row r sits at j ^ (r & 7), so that neither
+// side meets a bank twice.
 template <typename T, int COLS>
-__device__ __forceinline__ void store_row(const ProductArgs &a, uint64_t m, uint32_t n, const float (&acc)[COLS], bool valid) {
-    constexpr uint32_t kPer = 16 / sizeof(T);
-    T *row = (T *)a.out + m * a.out_stride + n;
-    const bool vec = (uintptr_t)row % 16 == 0;
+__device__ __forceinline__ void store_rows(const ProductArgs &a, uint64_t m0, uint32_t n0, const float (&acc)[COLS], bool valid, uint8_t *out, uint32_t lane) {
+    constexpr uint32_t kPer = 16 / sizeof(T), kWide = 128 / sizeof(T), kCols = COLS < (int)kWide ? COLS : kWide, kPieces = kCols / kPer;
+    const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - m0);
+    const bool vec = a.out_stride % kPer == 0 && (uintptr_t)a.out % 16 == 0;
 #pragma unroll
-    for (uint32_t j = 0; j < COLS; j += kPer) {
-        T e[kPer];
+    for (uint32_t part = 0; part < COLS / kCols; ++part) {
+        const uint32_t n = n0 + part * kCols;
+        if (n >= a.out_dim) break;
+        __syncwarp();  // the last part has been read
 #pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) {
-            float v = acc[j + i];
-            if (a.bias && n + j + i < a.out_dim) v += __ldg(a.bias + n + j + i);
-            e[i] = round_to<T>(valid ? v : 0.f);
-        }
-        if (vec && n + j + kPer <= a.out_dim) {
+        for (uint32_t j = 0; j < kPieces; ++j) {
+            T e[kPer];
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i) {
+                float v = acc[part * kCols + j * kPer + i];
+                if (a.bias && n + j * kPer + i < a.out_dim) v += __ldg(a.bias + n + j * kPer + i);
+                e[i] = round_to<T>(valid ? v : 0.f);
+            }
             uint4 q;
             memcpy(&q, e, 16);
-            *(uint4 *)(row + j) = q;
-        } else {
+            *(uint4 *)(out + lane * 128 + ((j ^ (lane & 7)) * 16)) = q;
+        }
+        __syncwarp();
+        T *to = (T *)a.out + m0 * a.out_stride + n;
+        if (vec && n + kCols <= a.out_dim) {
+            constexpr uint32_t kRowsAtOnce = 32 / kPieces;
+            const uint32_t j = lane % kPieces;
 #pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i)
-                if (n + j + i < a.out_dim) row[j + i] = e[i];
+            for (uint32_t r0 = 0; r0 < 32; r0 += kRowsAtOnce) {
+                const uint32_t r = r0 + lane / kPieces;
+                if (r < rows) *(uint4 *)(to + r * a.out_stride + j * kPer) = *(const uint4 *)(out + r * 128 + ((j ^ (r & 7)) * 16));
+            }
+        } else {
+            const uint32_t cols = min(kCols, a.out_dim - n);
+            for (uint32_t r = 0; r < rows; ++r)
+                for (uint32_t c = lane; c < cols; c += 32)
+                    to[r * a.out_stride + c] = *(const T *)(out + r * 128 + (((c / kPer) ^ (r & 7)) * 16) + c % kPer * sizeof(T));
         }
     }
+}
+
+// acc += scale * v for two columns at once.
+__device__ __forceinline__ void fma2(float &a0, float &a1, float s, uint32_t v0, uint32_t v1) {
+    uint64_t a, v, ss;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(a0), "f"(a1));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(v0), "r"(v1));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(ss) : "f"(s));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(a) : "l"(v), "l"(ss));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(a));
+}
+
+// The held row that output row m takes; `held` or more where there is none.
+template <bool IDS> __device__ __forceinline__ uint64_t id_of(const ProductArgs &a, uint64_t m) {
+    if (m >= a.rows) return a.held;
+    return !IDS ? m : a.ids64 ? (uint64_t)__ldg((const long long *)a.ids + m) : (uint64_t)__ldg((const uint32_t *)a.ids + m);
 }
 
 template <int BN, bool IDS, typename T>
@@ -247,14 +289,17 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     uint8_t *shared = (uint8_t *)(((uintptr_t)raw_shared + 1023) & ~(uintptr_t)1023);  // the swizzle's period
     uint64_t *bars = (uint64_t *)(shared + kStages * stage_bytes(BN));
     const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 8 * kAccStages,
-                   done = acc_empty + 8 * kAccStages;
-    uint32_t *words = (uint32_t *)(bars + 2 * kStages + 2 * kAccStages + 1);
+                   scale_full = acc_empty + 8 * kAccStages, scale_empty = scale_full + 16, done = scale_empty + 16;
+    uint32_t *words = (uint32_t *)(bars + 2 * kStages + 2 * kAccStages + 5);
+    uint8_t *out_shared = shared + kStages * stage_bytes(BN) + 256;
+    float *scale_shared = (float *)(out_shared + kOutBytes);
     volatile uint32_t *dead = words + 1;
     const ProductArgs &a = t.p;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // the shuffles tell that all lanes agree
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
         for (int i = 0; i < kAccStages; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, 8); }
+        for (int i = 0; i < 2; ++i) { mbar_init(scale_full + 8 * i, 64); mbar_init(scale_empty + 8 * i, 8); }
         mbar_init(done, 1);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -267,7 +312,7 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = *(volatile uint32_t *)words;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *(volatile uint32_t *)words, 0), shared_at = smem_u32(shared);
     const uint32_t tiles = t.m_tiles * t.n_tiles, steps = a.blocks;
 
     if (warp == 0) {
@@ -293,11 +338,12 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 const uint32_t s = issued % kStages;
                 alive = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, (issued / kStages & 1) ^ 1, dead));
                 if (!alive) break;
-                const uint32_t at = smem_u32(shared + s * stage_bytes(BN));
-                if (lane == 0) mbar_expect(full + 8 * s, stage_bytes(BN));
+                const uint32_t at = shared_at + s * stage_bytes(BN);
+                const bool leads = elect_one();
+                if (leads) mbar_expect(full + 8 * s, stage_bytes(BN));
                 __syncwarp();
                 if (IDS) tma_gather4(at + lane * 4 * kBK, &map_a, full + 8 * s, k * kBK, rows);
-                if (lane == 0) {
+                if (leads) {
                     if (!IDS) tma_tile(at, &map_a, full + 8 * s, k * kBK, m0);
                     tma_tile(at + kBM * kBK, &map_w, full + 8 * s, k * kBK, n0);
                 }
@@ -306,75 +352,110 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         if (!alive)
             for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_drain(full + 8 * (i % kStages), i / kStages & 1);
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);  // e4m3 x e4m3 -> f32
-            uint32_t n = 0;
-            bool alive = true;
-            for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x)
-                for (uint32_t k = 0; k < steps; ++k, ++n) {
-                    const uint32_t s = n % kStages, c = n % kAccStages;
-                    alive = mbar_wait(acc_empty + 8 * c, (n / kAccStages & 1) ^ 1, dead) && mbar_wait(full + 8 * s, n / kStages & 1, dead);
+        // The whole warp walks the loop, so that addresses stay in uniform registers, and one lane issues.
+        constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);  // e4m3 x e4m3 -> f32
+        uint32_t n = 0;
+        bool alive = true;
+        for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x)
+            for (uint32_t k = 0; k < steps; ++k, ++n) {
+                const uint32_t s = n % kStages, c = n % kAccStages;
+                const uint32_t acc_parity = (n / kAccStages & 1) ^ 1, parity = n / kStages & 1;
+                const bool free = mbar_try(acc_empty + 8 * c, acc_parity), there = mbar_try(full + 8 * s, parity);  // side by side
+                if (!__all_sync(0xffffffffu, free && there)) {
+                    alive = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * c, acc_parity, dead) && mbar_wait(full + 8 * s, parity, dead));
                     if (!alive) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t at = smem_u32(shared + s * stage_bytes(BN));
-                    const uint64_t da = matrix_desc(at), db = matrix_desc(at + kBM * kBK);
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t at = shared_at + s * stage_bytes(BN);
+                const uint64_t da = matrix_desc(at), db = matrix_desc(at + kBM * kBK);
+                if (elect_one()) {
 #pragma unroll
                     for (int q = 0; q < kBK / 32; ++q) mma_f8(tmem + c * BN, da + q * 2, db + q * 2, kIdesc, q > 0);
                     mma_commit(empty + 8 * s);
                     mma_commit(acc_full + 8 * c);
                 }
-            if (!alive) {
-                mma_commit(done);
-                mbar_drain(done, 0);
+                __syncwarp();
             }
+        if (!alive) {
+            if (elect_one()) mma_commit(done);
+            __syncwarp();
+            mbar_drain(done, 0);
         }
-        __syncwarp();
-    } else if (warp >= 4) {
-        const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
+    } else if (warp < 4) {
+        const uint32_t step = lane % kScaleSteps, row0 = (warp - 2) * 64 + lane / kScaleSteps;  // rows row0, row0 + 4, ...
         uint32_t n = 0;
         bool alive = true;
         for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
-            const uint32_t m0 = tile / t.n_tiles * kBM, n0 = tile % t.n_tiles * BN;
-            const uint64_t m = m0 + quarter * 32 + lane;
-            uint64_t src = m;
-            bool valid = m < a.rows;
-            if (IDS && valid) {
-                src = a.ids64 ? (uint64_t)((const int64_t *)a.ids)[m] : (uint64_t)((const uint32_t *)a.ids)[m];
-                valid = src < a.held;
+            const uint64_t m0 = (uint64_t)(tile / t.n_tiles) * kBM + row0;
+            const float *rows[16];
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint64_t id = id_of<IDS>(a, m0 + i * 4);
+                rows[i] = a.scales + (id < a.held ? id : 0) * a.blocks + step;
             }
-            const float *sa = a.scales + (valid ? src : 0) * a.blocks;
-            const float *sw = a.weight_scales + (uint64_t)(n0 / kF8Block) * a.blocks;
+            for (uint32_t k = 0; k < steps; k += kScaleSteps, ++n) {
+                alive = __all_sync(0xffffffffu, mbar_wait(scale_empty + 8 * (n & 1), (n >> 1 & 1) ^ 1, dead));
+                if (!alive) break;
+                const uint32_t to = smem_u32(scale_shared) + (n & 1) * kScaleBytes + (step * kScalePitch + row0) * 4;
+                if (k + step < steps) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(to + i * 16), "l"(rows[i] + k) : "memory");
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(scale_full + 8 * (n & 1)) : "memory");
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
+        constexpr int kLoad = kHalf >= 32 ? 32 : 16, kParts = kHalf / kLoad;
+        uint8_t *out = out_shared + (warp - 4) * 32 * 128;
+        uint32_t n = 0, chunk = 0;
+        bool alive = true;
+        for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
+            const uint32_t m0 = tile / t.n_tiles * kBM + quarter * 32, nt = tile % t.n_tiles, n0 = nt * BN + half * kHalf;
+            const bool valid = id_of<IDS>(a, m0 + lane) < a.held;
+            const float *weights = a.weight_scales + (uint64_t)(nt * BN / kF8Block) * a.blocks;
             float acc[kHalf];
 #pragma unroll
             for (int i = 0; i < kHalf; ++i) acc[i] = 0.f;
-            for (uint32_t k = 0; k < steps; ++k, ++n) {
-                const uint32_t c = n % kAccStages;
-                const float scale = __ldg(sa + k) * __ldg(sw + k);
-                alive = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * c, n / kAccStages & 1, dead));
+            for (uint32_t k0 = 0; k0 < steps && alive; k0 += kScaleSteps, ++chunk) {
+                const float weight = k0 + lane < steps && lane < kScaleSteps ? __ldg(weights + k0 + lane) : 0.f;
+                alive = __all_sync(0xffffffffu, mbar_wait(scale_full + 8 * (chunk & 1), chunk >> 1 & 1, dead));
                 if (!alive) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t from = tmem + c * BN + half * kHalf + (quarter << 21);
-                if constexpr (kHalf >= 32) {
-                    uint32_t v[kHalf / 32][32];
+                const float *scales = scale_shared + (chunk & 1) * (kScaleBytes / 4) + quarter * 32 + lane;
+                const uint32_t end = min(steps - k0, (uint32_t)kScaleSteps);
+                for (uint32_t j = 0; j < end; ++j, ++n) {
+                    const uint32_t c = n % kAccStages, parity = n / kAccStages & 1;
+                    if (!__all_sync(0xffffffffu, mbar_try(acc_full + 8 * c, parity))) {
+                        alive = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * c, parity, dead));
+                        if (!alive) break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t from = tmem + c * BN + half * kHalf + (quarter << 21);
+                    const float scale = scales[j * kScalePitch] * __shfl_sync(0xffffffffu, weight, j);
+                    uint32_t v[kParts][kLoad];  // a part's load and the sums of the part before overlap
 #pragma unroll
-                    for (int j = 0; j < kHalf / 32; ++j) tmem_load32(from + j * 32, v[j]);
+                    for (int q = 0; q <= kParts; ++q) {
+                        if (q < kParts) {
+                            if constexpr (kLoad == 32) tmem_load32(from + q * 32, v[q]);
+                            else tmem_load16(from, v[q]);
+                        }
+                        if (q > 0) {
 #pragma unroll
-                    for (int j = 0; j < kHalf / 32; ++j) tmem_wait(v[j]);
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    if (lane == 0) mbar_arrive(acc_empty + 8 * c);
-#pragma unroll
-                    for (int j = 0; j < kHalf; ++j) acc[j] += scale * __uint_as_float(v[j / 32][j % 32]);
-                } else {
-                    uint32_t v[16];
-                    tmem_load16(from, v);
-                    tmem_wait(v);
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    if (lane == 0) mbar_arrive(acc_empty + 8 * c);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[j] += scale * __uint_as_float(v[j]);
+                            for (int i = 0; i < kLoad; i += 2) fma2(acc[(q - 1) * kLoad + i], acc[(q - 1) * kLoad + i + 1], scale, v[q - 1][i], v[q - 1][i + 1]);
+                        }
+                        if (q < kParts) tmem_wait(v[q]);
+                        if (q == kParts - 1) {
+                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                            if (lane == 0) mbar_arrive(acc_empty + 8 * c);
+                        }
+                    }
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(scale_empty + 8 * (chunk & 1));
             }
-            if (alive && m < a.rows && n0 + half * kHalf < a.out_dim) store_row<T, kHalf>(a, m, n0 + half * kHalf, acc, valid);
+            if (alive && m0 < a.rows && n0 < a.out_dim) store_rows<T, kHalf>(a, m0, n0, acc, valid, out, lane);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -456,6 +537,7 @@ extern "C" int32_t ag_rows_product(const ag_product *p, int32_t device, void *st
                     (unsigned long long)p->dim, (unsigned long long)p->out_dim, (unsigned long long)p->held);
     if (p->rows == 0) return AG_OK;
     if (!p->codes || !p->scales || !p->weight || !p->weight_scales || !p->out) return fail(AG_ERR_VALUE, "ag_rows_product: null argument");
+    if (p->held == 0) return fail(AG_ERR_VALUE, "ag_rows_product: no rows are held");
     if (!p->ids && p->held < p->rows) return fail(AG_ERR_VALUE, "ag_rows_product: %llu rows of %llu held", (unsigned long long)p->rows, (unsigned long long)p->held);
     if (p->code_stride % 16 || p->weight_stride % 16 || p->code_stride < p->dim || p->weight_stride < p->dim || (uintptr_t)p->codes % 16 ||
         (uintptr_t)p->weight % 16)
