@@ -138,6 +138,12 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+// The same without the wait that try_wait may spend on it.
+__device__ __forceinline__ bool mbar_try_once(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 // Waits for the barrier's phase; false when the block is dead or the time ran out (which marks it dead).
 // The clock is looked at now and then only, and it is the SM's own: reading the global timer after
 // every failed try took longer than what is waited for.
@@ -237,11 +243,7 @@ __device__ __forceinline__ void store_rows(const ProductArgs &a, uint64_t m0, ui
         for (uint32_t j = 0; j < kPieces; ++j) {
             T e[kPer];
 #pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) {
-                float v = acc[part * kCols + j * kPer + i];
-                if (a.bias && n + j * kPer + i < a.out_dim) v += __ldg(a.bias + n + j * kPer + i);
-                e[i] = round_to<T>(valid ? v : 0.f);
-            }
+            for (uint32_t i = 0; i < kPer; ++i) e[i] = round_to<T>(valid ? acc[part * kCols + j * kPer + i] : 0.f);
             uint4 q;
             memcpy(&q, e, 16);
             *(uint4 *)(out + lane * 128 + ((j ^ (lane & 7)) * 16)) = q;
@@ -354,28 +356,36 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     } else if (warp == 1) {
         // The whole warp walks the loop, so that addresses stay in uniform registers, and one lane issues.
         constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);  // e4m3 x e4m3 -> f32
-        uint32_t n = 0;
-        bool alive = true;
-        for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x)
-            for (uint32_t k = 0; k < steps; ++k, ++n) {
-                const uint32_t s = n % kStages, c = n % kAccStages;
-                const uint32_t acc_parity = (n / kAccStages & 1) ^ 1, parity = n / kStages & 1;
-                const bool free = mbar_try(acc_empty + 8 * c, acc_parity), there = mbar_try(full + 8 * s, parity);  // side by side
-                if (!__all_sync(0xffffffffu, free && there)) {
-                    alive = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * c, acc_parity, dead) && mbar_wait(full + 8 * s, parity, dead));
-                    if (!alive) break;
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t at = shared_at + s * stage_bytes(BN);
-                const uint64_t da = matrix_desc(at), db = matrix_desc(at + kBM * kBK);
-                if (elect_one()) {
-#pragma unroll
-                    for (int q = 0; q < kBK / 32; ++q) mma_f8(tmem + c * BN, da + q * 2, db + q * 2, kIdesc, q > 0);
-                    mma_commit(empty + 8 * s);
-                    mma_commit(acc_full + 8 * c);
-                }
-                __syncwarp();
+        // The next step's barriers are tried between this step's multiplications: these keep the tensor
+        // core busy for 64 clocks each, a try alone takes about a hundred.
+        const uint32_t total = blockIdx.x < tiles ? ((tiles - 1 - blockIdx.x) / gridDim.x + 1) * steps : 0;
+        uint32_t s = 0, c = 0, parity = 0, acc_parity = 1;
+        bool alive = true, ready = false;
+        for (uint32_t n = 0; n < total; ++n) {
+            if (!__all_sync(0xffffffffu, ready)) {
+                alive = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * c, acc_parity, dead) && mbar_wait(full + 8 * s, parity, dead));
+                if (!alive) break;
             }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = shared_at + s * stage_bytes(BN), d = tmem + c * BN, empty_bar = empty + 8 * s, acc_bar = acc_full + 8 * c;
+            const uint64_t da = matrix_desc(at), db = matrix_desc(at + kBM * kBK);
+            const bool leads = elect_one();
+            if (leads) {
+                mma_f8(d, da, db, kIdesc, false);
+                mma_f8(d, da + 2, db + 2, kIdesc, true);
+            }
+            __syncwarp();
+            if (++s == kStages) { s = 0; parity ^= 1; }
+            if (++c == kAccStages) { c = 0; acc_parity ^= 1; }
+            ready = n + 1 < total && mbar_try_once(acc_empty + 8 * c, acc_parity) && mbar_try_once(full + 8 * s, parity);
+            if (leads) {
+                mma_f8(d, da + 4, db + 4, kIdesc, true);
+                mma_f8(d, da + 6, db + 6, kIdesc, true);
+                mma_commit(empty_bar);
+                mma_commit(acc_bar);
+            }
+            __syncwarp();
+        }
         if (!alive) {
             if (elect_one()) mma_commit(done);
             __syncwarp();
@@ -417,8 +427,13 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             const bool valid = id_of<IDS>(a, m0 + lane) < a.held;
             const float *weights = a.weight_scales + (uint64_t)(nt * BN / kF8Block) * a.blocks;
             float acc[kHalf];
+            if (a.bias) {  // the sums start from it; one branch here, not one for each value where they are stored
 #pragma unroll
-            for (int i = 0; i < kHalf; ++i) acc[i] = 0.f;
+                for (int i = 0; i < kHalf; ++i) acc[i] = n0 + i < a.out_dim ? __ldg(a.bias + n0 + i) : 0.f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kHalf; ++i) acc[i] = 0.f;
+            }
             for (uint32_t k0 = 0; k0 < steps && alive; k0 += kScaleSteps, ++chunk) {
                 const float weight = k0 + lane < steps && lane < kScaleSteps ? __ldg(weights + k0 + lane) : 0.f;
                 alive = __all_sync(0xffffffffu, mbar_wait(scale_full + 8 * (chunk & 1), chunk >> 1 & 1, dead));
