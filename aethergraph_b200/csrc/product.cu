@@ -104,11 +104,10 @@ k_product_dot(ProductArgs a) {
 // A tile of 128 rows x BN output columns per turn of a persistent block, K in steps of 128 bytes,
 // which is one scale block: the tensor cores add up the 128 products of a step in f32 in TMEM, and
 // the epilogue warps fold each step into their sums in registers, times the row's and the weights'
-// scale.  Roles: warp 0 loads (TMA, rows by id through tile::gather4), one thread of warp 1 issues
+// scale.  Roles: warp 0 loads (TMA, rows by id through tile::gather4), one thread each of warps 1 and 3 issues
 // tcgen05.mma (K = 32 each) and the commits, warps 4 - 11 read TMEM (a warp can reach only the 32 lanes
-// of its number mod 4, so two warps share a quarter of the rows and split the columns).  Warps 2 and 3 copy
-// the rows' scales into shared memory, eight steps at a time (cp.async): a row's scales lie side by side in
-// memory, so an epilogue warp that loaded its 32 rows' scale of one step itself would touch 32 lines.
+// of its number mod 4, so two warps share a quarter of the rows and split the columns).  Each
+// epilogue thread loads its own row's scales, four steps at a time, four steps ahead and across tiles.
 //
 // Every wait is bounded.  A role whose wait runs out marks the block dead and the sticky error
 // word; all roles then leave their loops, copies and multiplications in flight are waited for
@@ -116,15 +115,18 @@ k_product_dot(ProductArgs a) {
 constexpr int kBM = 128, kBK = 128, kAccStages = 4, kTileThreads = 384;
 constexpr long long kWaitLimit = 4000000000ll;  // clocks, two seconds
 
-constexpr int kScaleSteps = 8, kScalePitch = kBM + 4, kScaleBytes = kScaleSteps * kScalePitch * 4;  // the pitch keeps a copy's lanes on 32 banks
-constexpr int load_stages(int bn) { return bn >= 128 ? 5 : 7; }
+constexpr int load_stages(int bn, int elem) { return bn < 128 ? 7 : elem == 2 ? 5 : 4; }
 constexpr int stage_bytes(int bn) { return (kBM + bn) * kBK; }
-constexpr int kOutBytes = 8 * 32 * 128;  // each epilogue warp: 32 rows of 128 bytes on their way out
-constexpr int tile_shared(int bn) { return load_stages(bn) * stage_bytes(bn) + kOutBytes + 2 * kScaleBytes + 1024 + 256; }
+constexpr int out_bytes(int bn, int elem) { return 8 * 32 * (bn / 2) * elem; }  // the epilogue warps' rows on their way out
+constexpr int tile_shared(int bn, int elem) { return load_stages(bn, elem) * stage_bytes(bn) + out_bytes(bn, elem) + 1024 + 256; }
+// Bytes of a row that leave together: a box of the output's tensor map is 32 rows of so many, and is its swizzle.
+constexpr int box_bytes(int bn, int elem) { return bn / 2 * elem < 128 ? bn / 2 * elem : 128; }
 
 struct TileArgs {
     ProductArgs p;
     uint32_t m_tiles, n_tiles;
+    uint32_t tma_out;      // the output's rows start on multiples of 16 bytes
+    uint32_t scale_align;  // scales of a row that one load may take: 4, 2 or 1
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -226,45 +228,50 @@ template <> __device__ __forceinline__ __half round_to<__half>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // What an epilogue warp holds of its tile, 32 rows x COLS columns, a row a thread, leaves through
-// shared memory: a thread's own row in 16-byte pieces would touch 32 sectors half by half in every store; rows
-// of up to 128 bytes one beside the other fill them.  Piece j of row r sits at j ^ (r & 7), so that neither
-// side meets a bank twice.
+// shared memory, so that rows go out one beside the other in whole sectors: by TMA, which also leaves out what
+// lies past the output's edges and works while the warp goes on, where the output's rows start on 16 bytes; else
+// column by column.  16-byte piece j of a row is swizzled as the tensor map has it, which also
+// spreads neighbouring threads' pieces over the banks.
 template <typename T, int COLS>
-__device__ __forceinline__ void store_rows(const ProductArgs &a, uint64_t m0, uint32_t n0, const float (&acc)[COLS], bool valid, uint8_t *out, uint32_t lane) {
-    constexpr uint32_t kPer = 16 / sizeof(T), kWide = 128 / sizeof(T), kCols = COLS < (int)kWide ? COLS : kWide, kPieces = kCols / kPer;
-    const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - m0);
-    const bool vec = a.out_stride % kPer == 0 && (uintptr_t)a.out % 16 == 0;
+__device__ __forceinline__ void store_rows(const TileArgs &t, const CUtensorMap *map, uint32_t m0, uint32_t n0, const float (&acc)[COLS], bool valid,
+                                           uint8_t *out, uint32_t lane) {
+    constexpr uint32_t kBox = COLS * sizeof(T) < 128 ? COLS * sizeof(T) : 128, kPer = 16 / sizeof(T), kBoxCols = kBox / sizeof(T), kPieces = kBox / 16;
+    const ProductArgs &a = t.p;
+    auto at = [&](uint32_t part, uint32_t r, uint32_t j) { return out + part * 32 * kBox + r * kBox + ((j ^ ((r * kBox / 128) % kPieces)) * 16); };
+    if (t.tma_out && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();  // the last tile's rows have been read
 #pragma unroll
-    for (uint32_t part = 0; part < COLS / kCols; ++part) {
-        const uint32_t n = n0 + part * kCols;
-        if (n >= a.out_dim) break;
-        __syncwarp();  // the last part has been read
+    for (uint32_t part = 0; part < COLS / kBoxCols; ++part)
 #pragma unroll
         for (uint32_t j = 0; j < kPieces; ++j) {
             T e[kPer];
 #pragma unroll
-            for (uint32_t i = 0; i < kPer; ++i) e[i] = round_to<T>(valid ? acc[part * kCols + j * kPer + i] : 0.f);
+            for (uint32_t i = 0; i < kPer; ++i) e[i] = round_to<T>(valid ? acc[part * kBoxCols + j * kPer + i] : 0.f);
             uint4 q;
             memcpy(&q, e, 16);
-            *(uint4 *)(out + lane * 128 + ((j ^ (lane & 7)) * 16)) = q;
+            *(uint4 *)at(part, lane, j) = q;
         }
+    if (t.tma_out) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        T *to = (T *)a.out + m0 * a.out_stride + n;
-        if (vec && n + kCols <= a.out_dim) {
-            constexpr uint32_t kRowsAtOnce = 32 / kPieces;
-            const uint32_t j = lane % kPieces;
+        if (lane == 0) {
 #pragma unroll
-            for (uint32_t r0 = 0; r0 < 32; r0 += kRowsAtOnce) {
-                const uint32_t r = r0 + lane / kPieces;
-                if (r < rows) *(uint4 *)(to + r * a.out_stride + j * kPer) = *(const uint4 *)(out + r * 128 + ((j ^ (r & 7)) * 16));
-            }
-        } else {
-            const uint32_t cols = min(kCols, a.out_dim - n);
-            for (uint32_t r = 0; r < rows; ++r)
-                for (uint32_t c = lane; c < cols; c += 32)
-                    to[r * a.out_stride + c] = *(const T *)(out + r * 128 + (((c / kPer) ^ (r & 7)) * 16) + c % kPer * sizeof(T));
+            for (uint32_t part = 0; part < COLS / kBoxCols; ++part)
+                if (n0 + part * kBoxCols < a.out_dim)
+                    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                                 :: "l"(map), "r"(smem_u32(out + part * 32 * kBox)), "r"(n0 + part * kBoxCols), "r"(m0) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
+        return;
     }
+    __syncwarp();
+    const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - m0), cols = min((uint32_t)COLS, a.out_dim - n0);
+    T *to = (T *)a.out + (uint64_t)m0 * a.out_stride + n0;
+    for (uint32_t r = 0; r < rows; ++r)
+        for (uint32_t c = lane; c < cols; c += 32) {
+            const uint32_t in = c % kBoxCols;
+            to[r * a.out_stride + c] = *(const T *)(at(c / kBoxCols, r, in / kPer) + in % kPer * sizeof(T));
+        }
 }
 
 // acc += scale * v for two columns at once.
@@ -285,24 +292,24 @@ template <bool IDS> __device__ __forceinline__ uint64_t id_of(const ProductArgs 
 
 template <int BN, bool IDS, typename T>
 __global__ void __launch_bounds__(kTileThreads, 1)
-k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const TileArgs t) {
-    constexpr int kStages = load_stages(BN), kHalf = BN / 2;
+k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
+               const __grid_constant__ TileArgs t) {
+    constexpr int kStages = load_stages(BN, sizeof(T)), kHalf = BN / 2;
     extern __shared__ uint8_t raw_shared[];
     uint8_t *shared = (uint8_t *)(((uintptr_t)raw_shared + 1023) & ~(uintptr_t)1023);  // the swizzle's period
-    uint64_t *bars = (uint64_t *)(shared + kStages * stage_bytes(BN));
+    uint64_t *bars = (uint64_t *)(shared + kStages * stage_bytes(BN) + out_bytes(BN, sizeof(T)));
     const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, acc_full = empty + 8 * kStages, acc_empty = acc_full + 8 * kAccStages,
-                   scale_full = acc_empty + 8 * kAccStages, scale_empty = scale_full + 16, done = scale_empty + 16;
-    uint32_t *words = (uint32_t *)(bars + 2 * kStages + 2 * kAccStages + 5);
-    uint8_t *out_shared = shared + kStages * stage_bytes(BN) + 256;
-    float *scale_shared = (float *)(out_shared + kOutBytes);
+                   done = acc_empty + 8 * kAccStages;
+    uint32_t *words = (uint32_t *)(bars + 2 * kStages + 2 * kAccStages + 2);
+    uint8_t *out_shared = shared + kStages * stage_bytes(BN);  // 1024-byte aligned, as the swizzle wants it
     volatile uint32_t *dead = words + 1;
     const ProductArgs &a = t.p;
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // the shuffles tell that all lanes agree
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
         for (int i = 0; i < kAccStages; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, 8); }
-        for (int i = 0; i < 2; ++i) { mbar_init(scale_full + 8 * i, 64); mbar_init(scale_empty + 8 * i, 8); }
         mbar_init(done, 1);
+        mbar_init(done + 8, 1);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -320,6 +327,12 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     if (warp == 0) {
         uint32_t issued = 0;
         bool alive = true;
+        uint64_t id[4];
+        auto load_ids = [&](uint32_t tile) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) id[i] = tile < tiles ? id_of<IDS>(a, (uint64_t)(tile / t.n_tiles) * kBM + lane * 4 + i) : a.held;
+        };
+        if (IDS) load_ids(blockIdx.x);
         for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
             const uint32_t m0 = tile / t.n_tiles * kBM, n0 = tile % t.n_tiles * BN;
             int4 rows = make_int4(0, 0, 0, 0);
@@ -327,14 +340,11 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 int r[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint64_t m = m0 + lane * 4 + i;
-                    r[i] = 0;
-                    if (m < a.rows) {
-                        const uint64_t id = source_row(a, m);
-                        if (id < a.held) r[i] = (int)id;
-                    }
+                    r[i] = id[i] < a.held ? (int)id[i] : 0;
+                    if (id[i] >= a.held && m0 + lane * 4 + i < a.rows) atomicOr(&g_rows_error, kErrBadId);
                 }
                 rows = make_int4(r[0], r[1], r[2], r[3]);
+                load_ids(tile + gridDim.x);  // a tile ahead
             }
             for (uint32_t k = 0; k < steps; ++k, ++issued) {
                 const uint32_t s = issued % kStages;
@@ -353,21 +363,22 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
         if (!alive)
             for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_drain(full + 8 * (i % kStages), i / kStages & 1);
-    } else if (warp == 1) {
+    } else if (warp & 1 && warp < 4) {
         // The whole warp walks the loop, so that addresses stay in uniform registers, and one lane issues.
         constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);  // e4m3 x e4m3 -> f32
-        // The next step's barriers are tried between this step's multiplications: these keep the tensor
-        // core busy for 64 clocks each, a try alone takes about a hundred.
+        // Two warps issue in turn: every step has accumulators and operands of its own, and a warp's
+        // overhead from one step to the next (barriers, descriptors, commits: 340 clocks) is longer than the 256
+        // that a step's multiplications take.  Each tries its next step's barriers between this one's multiplications.
         const uint32_t total = blockIdx.x < tiles ? ((tiles - 1 - blockIdx.x) / gridDim.x + 1) * steps : 0;
-        uint32_t s = 0, c = 0, parity = 0, acc_parity = 1;
         bool alive = true, ready = false;
-        for (uint32_t n = 0; n < total; ++n) {
+        for (uint32_t n = warp >> 1; n < total; n += 2) {
+            const uint32_t s = n % kStages, c = n % kAccStages;
             if (!__all_sync(0xffffffffu, ready)) {
-                alive = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * c, acc_parity, dead) && mbar_wait(full + 8 * s, parity, dead));
+                alive = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * c, (n / kAccStages & 1) ^ 1, dead) && mbar_wait(full + 8 * s, n / kStages & 1, dead));
                 if (!alive) break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t at = shared_at + s * stage_bytes(BN), d = tmem + c * BN, empty_bar = empty + 8 * s, acc_bar = acc_full + 8 * c;
+            const uint32_t at = shared_at + s * stage_bytes(BN), d = tmem + c * BN;
             const uint64_t da = matrix_desc(at), db = matrix_desc(at + kBM * kBK);
             const bool leads = elect_one();
             if (leads) {
@@ -375,57 +386,51 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 mma_f8(d, da + 2, db + 2, kIdesc, true);
             }
             __syncwarp();
-            if (++s == kStages) { s = 0; parity ^= 1; }
-            if (++c == kAccStages) { c = 0; acc_parity ^= 1; }
-            ready = n + 1 < total && mbar_try_once(acc_empty + 8 * c, acc_parity) && mbar_try_once(full + 8 * s, parity);
+            const uint32_t next = n + 2, s2 = next % kStages, c2 = next % kAccStages;
+            ready = next < total && mbar_try_once(acc_empty + 8 * c2, (next / kAccStages & 1) ^ 1) && mbar_try_once(full + 8 * s2, next / kStages & 1);
             if (leads) {
                 mma_f8(d, da + 4, db + 4, kIdesc, true);
                 mma_f8(d, da + 6, db + 6, kIdesc, true);
-                mma_commit(empty_bar);
-                mma_commit(acc_bar);
+                mma_commit(empty + 8 * s);
+                mma_commit(acc_full + 8 * c);
             }
             __syncwarp();
         }
         if (!alive) {
-            if (elect_one()) mma_commit(done);
+            if (elect_one()) mma_commit(done + 8 * (warp >> 1));
             __syncwarp();
-            mbar_drain(done, 0);
+            mbar_drain(done + 8 * (warp >> 1), 0);
         }
-    } else if (warp < 4) {
-        const uint32_t step = lane % kScaleSteps, row0 = (warp - 2) * 64 + lane / kScaleSteps;  // rows row0, row0 + 4, ...
-        uint32_t n = 0;
-        bool alive = true;
-        for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
-            const uint64_t m0 = (uint64_t)(tile / t.n_tiles) * kBM + row0;
-            const float *rows[16];
-#pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) {
-                const uint64_t id = id_of<IDS>(a, m0 + i * 4);
-                rows[i] = a.scales + (id < a.held ? id : 0) * a.blocks + step;
-            }
-            for (uint32_t k = 0; k < steps; k += kScaleSteps, ++n) {
-                alive = __all_sync(0xffffffffu, mbar_wait(scale_empty + 8 * (n & 1), (n >> 1 & 1) ^ 1, dead));
-                if (!alive) break;
-                const uint32_t to = smem_u32(scale_shared) + (n & 1) * kScaleBytes + (step * kScalePitch + row0) * 4;
-                if (k + step < steps) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i)
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" :: "r"(to + i * 16), "l"(rows[i] + k) : "memory");
-                }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(scale_full + 8 * (n & 1)) : "memory");
-            }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-    } else {
+    } else if (warp >= 4) {
         const uint32_t quarter = warp & 3, half = (warp - 4) / 4;
         constexpr int kLoad = kHalf >= 32 ? 32 : 16, kParts = kHalf / kLoad;
-        uint8_t *out = out_shared + (warp - 4) * 32 * 128;
-        uint32_t n = 0, chunk = 0;
-        bool alive = true;
+        uint8_t *out = out_shared + (warp - 4) * 32 * kHalf * sizeof(T);
+        uint32_t n = 0;
+        bool alive = true, ready = false;
+        auto id_at = [&](uint32_t tile) { return tile < tiles ? id_of<IDS>(a, (uint64_t)(tile / t.n_tiles) * kBM + quarter * 32 + lane) : a.held; };
+        uint64_t id = id_at(blockIdx.x);
+        float next[4];  // the row's scales of four steps
+        auto fetch = [&](const float *row, uint32_t k) {
+            const uint32_t left = steps - k;
+            if (t.scale_align == 4) {
+                const float4 f = __ldg((const float4 *)(row + k));
+                next[0] = f.x; next[1] = f.y; next[2] = f.z; next[3] = f.w;
+            } else if (t.scale_align == 2) {
+                const float2 lo = __ldg((const float2 *)(row + k)), hi = left > 2 ? __ldg((const float2 *)(row + k + 2)) : make_float2(0.f, 0.f);
+                next[0] = lo.x; next[1] = lo.y; next[2] = hi.x; next[3] = hi.y;
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) next[j] = j < left ? __ldg(row + k + j) : 0.f;
+            }
+        };
+        bool valid = id < a.held;
+        const float *row = a.scales + (valid ? id : 0) * steps;
+        fetch(row, 0);
         for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
             const uint32_t m0 = tile / t.n_tiles * kBM + quarter * 32, nt = tile % t.n_tiles, n0 = nt * BN + half * kHalf;
-            const bool valid = id_of<IDS>(a, m0 + lane) < a.held;
-            const float *weights = a.weight_scales + (uint64_t)(nt * BN / kF8Block) * a.blocks;
+            const float *weights = a.weight_scales + (uint64_t)(nt * BN / kF8Block) * steps;
+            float weight = lane < steps ? __ldg(weights + lane) : 0.f;  // 32 steps' in the lanes
+            id = id_at(tile + gridDim.x);
             float acc[kHalf];
             if (a.bias) {  // the sums start from it; one branch here, not one for each value where they are stored
 #pragma unroll
@@ -434,44 +439,45 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < kHalf; ++i) acc[i] = 0.f;
             }
-            for (uint32_t k0 = 0; k0 < steps && alive; k0 += kScaleSteps, ++chunk) {
-                const float weight = k0 + lane < steps && lane < kScaleSteps ? __ldg(weights + k0 + lane) : 0.f;
-                alive = __all_sync(0xffffffffu, mbar_wait(scale_full + 8 * (chunk & 1), chunk >> 1 & 1, dead));
-                if (!alive) break;
-                const float *scales = scale_shared + (chunk & 1) * (kScaleBytes / 4) + quarter * 32 + lane;
-                const uint32_t end = min(steps - k0, (uint32_t)kScaleSteps);
-                for (uint32_t j = 0; j < end; ++j, ++n) {
-                    const uint32_t c = n % kAccStages, parity = n / kAccStages & 1;
-                    if (!__all_sync(0xffffffffu, mbar_try(acc_full + 8 * c, parity))) {
-                        alive = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * c, parity, dead));
+            for (uint32_t k0 = 0; k0 < steps && alive; k0 += 4) {
+                float scale[4];
+                if (k0 && k0 % 32 == 0) weight = k0 + lane < steps ? __ldg(weights + k0 + lane) : 0.f;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) scale[j] = next[j] * __shfl_sync(0xffffffffu, weight, k0 % 32 + j);
+                if (k0 + 4 < steps) fetch(row, k0 + 4);
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    if (k0 + j >= steps) break;
+                    const uint32_t c = n % kAccStages;
+                    if (!__all_sync(0xffffffffu, ready)) {
+                        alive = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * c, n / kAccStages & 1, dead));
                         if (!alive) break;
                     }
+                    ++n;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t from = tmem + c * BN + half * kHalf + (quarter << 21);
-                    const float scale = scales[j * kScalePitch] * __shfl_sync(0xffffffffu, weight, j);
-                    uint32_t v[kParts][kLoad];  // a part's load and the sums of the part before overlap
+                    uint32_t v[kParts][kLoad];
 #pragma unroll
-                    for (int q = 0; q <= kParts; ++q) {
-                        if (q < kParts) {
-                            if constexpr (kLoad == 32) tmem_load32(from + q * 32, v[q]);
-                            else tmem_load16(from, v[q]);
-                        }
-                        if (q > 0) {
-#pragma unroll
-                            for (int i = 0; i < kLoad; i += 2) fma2(acc[(q - 1) * kLoad + i], acc[(q - 1) * kLoad + i + 1], scale, v[q - 1][i], v[q - 1][i + 1]);
-                        }
-                        if (q < kParts) tmem_wait(v[q]);
-                        if (q == kParts - 1) {
-                            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                            if (lane == 0) mbar_arrive(acc_empty + 8 * c);
-                        }
+                    for (int q = 0; q < kParts; ++q) {
+                        if constexpr (kLoad == 32) tmem_load32(from + q * 32, v[q]);
+                        else tmem_load16(from, v[q]);
                     }
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) tmem_wait(v[q]);
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    if (lane == 0) mbar_arrive(acc_empty + 8 * c);
+                    ready = mbar_try_once(acc_full + 8 * (n % kAccStages), n / kAccStages & 1);  // the answer comes beside the sums
+#pragma unroll
+                    for (int i = 0; i < kHalf; i += 2) fma2(acc[i], acc[i + 1], scale[j], v[i / kLoad][i % kLoad], v[i / kLoad][i % kLoad + 1]);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(scale_empty + 8 * (chunk & 1));
             }
-            if (alive && m0 < a.rows && n0 < a.out_dim) store_rows<T, kHalf>(a, m0, n0, acc, valid, out, lane);
+            const bool keep = valid;
+            valid = id < a.held;
+            row = a.scales + (valid ? id : 0) * steps;
+            if (tile + gridDim.x < tiles) fetch(row, 0);
+            if (alive && m0 < a.rows && n0 < a.out_dim) store_rows<T, kHalf>(t, &map_out, m0, n0, acc, keep, out, lane);
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -497,30 +503,36 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-// Rows of bytes as a tensor map: 128 columns x `box` rows a load, what lies outside reads as zeros.
-int32_t rows_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t dim, uint64_t pitch, uint32_t box) {
+// Rows of elements of `elem` bytes as a tensor map of boxes `box_cols` x `box_rows`, swizzled over a box's
+// bytes (128, 64 or 32).  What lies outside reads as zeros and is not written.
+int32_t rows_map(CUtensorMap *map, const void *base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t elem, uint32_t box_cols, uint32_t box_rows) {
     if (!encode_tiled()) return fail(AG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    const cuuint64_t dims[2] = {dim, rows}, strides[1] = {pitch};
-    const cuuint32_t boxes[2] = {kBK, box}, steps[2] = {1, 1};
-    const CUresult r = encode_tiled()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, boxes, steps,
-                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+    const cuuint32_t boxes[2] = {box_cols, box_rows}, steps[2] = {1, 1};
+    const uint32_t bytes = box_cols * elem;
+    const CUresult r = encode_tiled()(map, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT32,
+                                      2, const_cast<void *>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                      bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                                      CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
-        return fail(AG_ERR_CUDA, "cannot describe %llu rows of %llu bytes at a pitch of %llu (driver error %d)", (unsigned long long)rows,
-                    (unsigned long long)dim, (unsigned long long)pitch, (int)r);
+        return fail(AG_ERR_CUDA, "cannot describe %llu rows of %llu elements at a pitch of %llu bytes (driver error %d)", (unsigned long long)rows,
+                    (unsigned long long)cols, (unsigned long long)pitch, (int)r);
     return AG_OK;
 }
 
 template <int BN, bool IDS, typename T>
 int32_t launch_tile(const ProductArgs &a, cudaStream_t st) {
-    TileArgs t{a, (uint32_t)((a.rows + kBM - 1) / kBM), (a.out_dim + BN - 1) / BN};
-    CUtensorMap map_a, map_w;
-    AG_TRY(rows_map(&map_a, a.codes, IDS ? a.held : a.rows, a.dim, a.code_stride, IDS ? 1 : kBM));
-    AG_TRY(rows_map(&map_w, a.weight, a.out_dim, a.dim, a.weight_stride, BN));
-    AG_CUDA(cudaFuncSetAttribute(k_product_tile<BN, IDS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_shared(BN)));
+    const uint64_t pitch = a.out_stride * sizeof(T);
+    TileArgs t{a, (uint32_t)((a.rows + kBM - 1) / kBM), (a.out_dim + BN - 1) / BN, pitch % 16 == 0 && (uintptr_t)a.out % 16 == 0 && pitch < (1ull << 40),
+               a.blocks % 4 == 0 && (uintptr_t)a.scales % 16 == 0 ? 4u : a.blocks % 2 == 0 && (uintptr_t)a.scales % 8 == 0 ? 2u : 1u};
+    CUtensorMap map_a, map_w, map_out{};
+    AG_TRY(rows_map(&map_a, a.codes, IDS ? a.held : a.rows, a.dim, a.code_stride, 1, kBK, IDS ? 1 : kBM));
+    AG_TRY(rows_map(&map_w, a.weight, a.out_dim, a.dim, a.weight_stride, 1, kBK, BN));
+    if (t.tma_out) AG_TRY(rows_map(&map_out, a.out, a.rows, a.out_dim, pitch, sizeof(T), box_bytes(BN, sizeof(T)) / sizeof(T), 32));
+    AG_CUDA(cudaFuncSetAttribute(k_product_tile<BN, IDS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_shared(BN, sizeof(T))));
     const uint64_t tiles = (uint64_t)t.m_tiles * t.n_tiles;
     if (tiles > 0x7FFFFFFFull) return fail(AG_ERR_VALUE, "ag_rows_product: the output is too large");
-    k_product_tile<BN, IDS, T><<<(uint32_t)std::min<uint64_t>(tiles, kSMs), kTileThreads, tile_shared(BN), st>>>(map_a, map_w, t);
+    k_product_tile<BN, IDS, T><<<(uint32_t)std::min<uint64_t>(tiles, kSMs), kTileThreads, tile_shared(BN, sizeof(T)), st>>>(map_a, map_w, map_out, t);
     return AG_OK;
 }
 
