@@ -104,7 +104,9 @@ k_product_dot(ProductArgs a) {
 // A tile of 128 rows x BN output columns per turn of a persistent block, K in steps of 128 bytes,
 // which is one scale block: the tensor cores add up the 128 products of a step in f32 in TMEM, and
 // the epilogue warps fold each step into their sums in registers, times the row's and the weights'
-// scale.  Roles: warp 0 loads (TMA, rows by id through tile::gather4), one thread each of warps 1 and 3 issues
+// scale.  Roles: warp 0 loads by TMA, and rows by id come through warps 0 and 2 with cp.async (the
+// gather form of the TMA load takes about 19 clocks a row: 25 us for 38 411 rows of 256, of them 10 waiting
+// for it), one thread each of warps 1 and 3 issues
 // tcgen05.mma (K = 32 each) and the commits, warps 4 - 11 read TMEM (a warp can reach only the 32 lanes
 // of its number mod 4, so two warps share a quarter of the rows and split the columns).  Each
 // epilogue thread loads its own row's scales, four steps at a time, four steps ahead and across tiles.
@@ -118,7 +120,7 @@ constexpr long long kWaitLimit = 4000000000ll;  // clocks, two seconds
 constexpr int load_stages(int bn, int elem) { return bn < 128 ? 7 : elem == 2 ? 5 : 4; }
 constexpr int stage_bytes(int bn) { return (kBM + bn) * kBK; }
 constexpr int out_bytes(int bn, int elem) { return 8 * 32 * (bn / 2) * elem; }  // the epilogue warps' rows on their way out
-constexpr int tile_shared(int bn, int elem) { return load_stages(bn, elem) * stage_bytes(bn) + out_bytes(bn, elem) + 1024 + 256; }
+constexpr int tile_shared(int bn, int elem) { return load_stages(bn, elem) * stage_bytes(bn) + out_bytes(bn, elem) + 1024 + 256 + kBM * 4; }
 // Bytes of a row that leave together: a box of the output's tensor map is 32 rows of so many, and is its swizzle.
 constexpr int box_bytes(int bn, int elem) { return bn / 2 * elem < 128 ? bn / 2 * elem : 128; }
 
@@ -171,10 +173,6 @@ __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t x, int32_t y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
-}
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, uint32_t bar, int32_t x, int4 rows) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-                 :: "r"(dst), "l"(map), "r"(bar), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w) : "memory");
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t is;
@@ -303,10 +301,11 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     uint32_t *words = (uint32_t *)(bars + 2 * kStages + 2 * kAccStages + 2);
     uint8_t *out_shared = shared + kStages * stage_bytes(BN);  // 1024-byte aligned, as the swizzle wants it
     volatile uint32_t *dead = words + 1;
+    uint32_t *row_ids = words + 4;  // of a tile's rows
     const ProductArgs &a = t.p;
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // the shuffles tell that all lanes agree
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) { mbar_init(full + 8 * i, 1); mbar_init(empty + 8 * i, 1); }
+        for (int i = 0; i < kStages; ++i) { mbar_init(full + 8 * i, IDS ? 3 : 1); mbar_init(empty + 8 * i, 1); }
         for (int i = 0; i < kAccStages; ++i) { mbar_init(acc_full + 8 * i, 1); mbar_init(acc_empty + 8 * i, 8); }
         mbar_init(done, 1);
         mbar_init(done + 8, 1);
@@ -324,26 +323,34 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const uint32_t tmem = __shfl_sync(0xffffffffu, *(volatile uint32_t *)words, 0), shared_at = smem_u32(shared);
     const uint32_t tiles = t.m_tiles * t.n_tiles, steps = a.blocks;
 
-    if (warp == 0) {
-        uint32_t issued = 0;
+    if (IDS ? warp == 0 || warp == 2 : warp == 0) {
+        uint32_t issued = 0, landed = 0;
         bool alive = true;
-        uint64_t id[4];
+        uint64_t id[2];  // rows half + lane and half + lane + 32 of the tile
+        const uint32_t first = warp * 32, piece = lane % 8;
         auto load_ids = [&](uint32_t tile) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) id[i] = tile < tiles ? id_of<IDS>(a, (uint64_t)(tile / t.n_tiles) * kBM + lane * 4 + i) : a.held;
+            for (int i = 0; i < 2; ++i) id[i] = tile < tiles ? id_of<IDS>(a, (uint64_t)(tile / t.n_tiles) * kBM + first + lane + i * 32) : a.held;
+        };
+        // This warp's copies of step `landed` are there: made visible to the tensor core, then reported.
+        auto report = [&] {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * (landed % kStages));
+            ++landed;
         };
         if (IDS) load_ids(blockIdx.x);
         for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
             const uint32_t m0 = tile / t.n_tiles * kBM, n0 = tile % t.n_tiles * BN;
-            int4 rows = make_int4(0, 0, 0, 0);
+            uint32_t *mine = row_ids + first;
             if (IDS) {  // rows without one, and ids outside, load row 0: the epilogue leaves its zeros
-                int r[4];
+                __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    r[i] = id[i] < a.held ? (int)id[i] : 0;
-                    if (id[i] >= a.held && m0 + lane * 4 + i < a.rows) atomicOr(&g_rows_error, kErrBadId);
+                for (int i = 0; i < 2; ++i) {
+                    mine[lane + i * 32] = id[i] < a.held ? (uint32_t)id[i] : 0;
+                    if (id[i] >= a.held && m0 + first + lane + i * 32 < a.rows) atomicOr(&g_rows_error, kErrBadId);
                 }
-                rows = make_int4(r[0], r[1], r[2], r[3]);
+                __syncwarp();
                 load_ids(tile + gridDim.x);  // a tile ahead
             }
             for (uint32_t k = 0; k < steps; ++k, ++issued) {
@@ -351,17 +358,33 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 alive = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, (issued / kStages & 1) ^ 1, dead));
                 if (!alive) break;
                 const uint32_t at = shared_at + s * stage_bytes(BN);
-                const bool leads = elect_one();
-                if (leads) mbar_expect(full + 8 * s, stage_bytes(BN));
-                __syncwarp();
-                if (IDS) tma_gather4(at + lane * 4 * kBK, &map_a, full + 8 * s, k * kBK, rows);
-                if (leads) {
+                if (warp == 0 && elect_one()) {
+                    mbar_expect(full + 8 * s, IDS ? BN * kBK : stage_bytes(BN));
                     if (!IDS) tma_tile(at, &map_a, full + 8 * s, k * kBK, m0);
                     tma_tile(at + kBM * kBK, &map_w, full + 8 * s, k * kBK, n0);
                 }
+                if (IDS) {  // eight lanes a row, 16 bytes each, swizzled as the tensor maps do; zeros past the row's end
+                    const uint32_t c = k * kBK + piece * 16, bytes = c < a.dim ? min(a.dim - c, 16u) : 0;
+                    const uint8_t *from = a.codes + (bytes ? c : 0);
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; ++i) {
+                        const uint32_t r = lane / 8 + i * 4;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                     :: "r"(at + (first + r) * kBK + ((piece ^ (r % 8)) * 16)), "l"(from + (uint64_t)mine[r] * a.code_stride), "r"(bytes) : "memory");
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (issued - landed >= kStages - 2) {
+                        asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 2) : "memory");
+                        report();
+                    }
+                }
             }
         }
-        if (!alive)
+        if (IDS) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            while (landed < issued) report();  // of a dead block too: the loads' barriers end
+        }
+        if (!alive && warp == 0)
             for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_drain(full + 8 * (i % kStages), i / kStages & 1);
     } else if (warp & 1 && warp < 4) {
         // The whole warp walks the loop, so that addresses stay in uniform registers, and one lane issues.
@@ -525,8 +548,8 @@ int32_t launch_tile(const ProductArgs &a, cudaStream_t st) {
     const uint64_t pitch = a.out_stride * sizeof(T);
     TileArgs t{a, (uint32_t)((a.rows + kBM - 1) / kBM), (a.out_dim + BN - 1) / BN, pitch % 16 == 0 && (uintptr_t)a.out % 16 == 0 && pitch < (1ull << 40),
                a.blocks % 4 == 0 && (uintptr_t)a.scales % 16 == 0 ? 4u : a.blocks % 2 == 0 && (uintptr_t)a.scales % 8 == 0 ? 2u : 1u};
-    CUtensorMap map_a, map_w, map_out{};
-    AG_TRY(rows_map(&map_a, a.codes, IDS ? a.held : a.rows, a.dim, a.code_stride, 1, kBK, IDS ? 1 : kBM));
+    CUtensorMap map_a{}, map_w, map_out{};
+    if (!IDS) AG_TRY(rows_map(&map_a, a.codes, a.rows, a.dim, a.code_stride, 1, kBK, kBM));
     AG_TRY(rows_map(&map_w, a.weight, a.out_dim, a.dim, a.weight_stride, 1, kBK, BN));
     if (t.tma_out) AG_TRY(rows_map(&map_out, a.out, a.rows, a.out_dim, pitch, sizeof(T), box_bytes(BN, sizeof(T)) / sizeof(T), 32));
     AG_CUDA(cudaFuncSetAttribute(k_product_tile<BN, IDS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_shared(BN, sizeof(T))));
