@@ -1,4 +1,5 @@
-"""Builds libaethergpu.so (the CUDA kernels and the C ABI) for sm_100a, in-tree.
+"""Builds libaethergpu.so (the CUDA kernels and the C ABI) for sm_100a, and _ops.so (the row
+operators as PyTorch functions, over the C ABI), in-tree.
 
     python -m aethergraph_b200.build [--force] [--verbose]
 
@@ -16,6 +17,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaethergpu.so")
+OPS = os.path.join(HERE, "_ops.so")
 SOURCES = ["api.cu", "gather.cu", "sampler.cu", "synth.cu", "loader.cu", "noalloc.cu", "hetero.cu", "hop.cu", "shard.cu",
            "hetero_loader.cu", "rewrite.cu", "hot.cu", "peer_block.cu", "reorder.cu", "workspace.cu",
            "rows.cu", "product.cu"]
@@ -33,12 +35,28 @@ def _nvcc() -> str:
 
 
 def _stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(OPS):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(OPS))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(HERE, "..", "include", "aethergpu.h"))
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
+
+
+def _ops_command(host: str) -> list[str]:
+    """g++ over csrc/ops_torch.cpp against the installed PyTorch; finds libaethergpu.so beside it."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    includes = [*cpp_extension.include_paths(), sysconfig.get_path("include"), os.path.join(cuda, "include")]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    return [host, "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_ops",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes),
+            os.path.join(CSRC, "ops_torch.cpp"), "-o", OPS + ".tmp", f"-L{HERE}", "-l:libaethergpu.so", f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+            "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -74,6 +92,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError("libaethergpu.so: link failed\n" + r.stdout.decode(errors="replace"))
     os.replace(LIB + ".tmp", LIB)
+    r = subprocess.run(_ops_command(host), env=env, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    if r.returncode != 0:
+        raise RuntimeError("_ops.so: compilation failed\n" + r.stdout.decode(errors="replace")[-4000:])
+    os.replace(OPS + ".tmp", OPS)
     return LIB
 
 

@@ -125,10 +125,11 @@ class FeatureStore:
 
         from . import ops
 
-        rows, dim, pitch, index = ops._check_f8(codes, scales, "codes", 1)
+        ops._ops.check_f8(codes, scales, "codes", 1)
         torch.cuda.current_stream(codes.device).synchronize()
         out = C.c_void_p()
-        _lib.check(_lib.lib().ag_features_from_f8(codes.data_ptr() or None, scales.data_ptr() or None, rows, dim, pitch, index, C.byref(out)))
+        _lib.check(_lib.lib().ag_features_from_f8(codes.data_ptr() or None, scales.data_ptr() or None, codes.shape[0], codes.shape[1],
+                                                  codes.stride(0), codes.get_device(), C.byref(out)))
         store = FeatureStore(out.value)
         store._keep = (codes, scales)
         return store
@@ -246,12 +247,7 @@ class FeatureStore:
 
         from . import ops
 
-        return ops._product(self._f8_rows(), weight, weight_scales, ids, bias, torch.bfloat16 if dtype is None else dtype)
-
-    def _f8_rows(self):
-        codes, scales, pitch = C.c_void_p(), C.c_void_p(), C.c_uint64()
-        _lib.check(_lib.lib().ag_features_f8_rows(self._h, C.byref(codes), C.byref(scales), C.byref(pitch)))
-        return codes.value, scales.value, pitch.value, self._n, self._dim, self._device
+        return ops._ops.project(self._h.value, ids, weight, weight_scales, bias, torch.bfloat16 if dtype is None else dtype)
 
     def gather_stats(self) -> tuple[int, int, int]:
         """Sharded views: `(rows requested, rows loaded, rows loaded from the local copy of
