@@ -21,7 +21,7 @@ import numpy as np
 
 from ..features import FeatureStore
 from ..hetero import HeteroCsrGraph, HeteroNeighborLoader as NativeHeteroLoader, HeteroSamplingConfig
-from .loader import Batch, epoch_sampling_seed, make_batch_getter, normalize_input_nodes
+from .loader import Batch, FeatureDropout, epoch_sampling_seed, make_batch_getter, normalize_input_nodes
 
 __all__ = ["HeteroBatch", "HeteroLoaderMetrics", "HeteroNeighborLoader"]
 
@@ -80,13 +80,15 @@ class HeteroNeighborLoader:
     """Drop-in for `aethergraph.pytorch.HeteroNeighborLoader` on a GPU-resident
     `HeteroCsrGraph`.  `features` maps node types to a `FeatureStore` or a float32
     `[num_nodes(type), dim]` array (kept in GPU memory); `x` of a batch is gathered
-    on the GPU from the batch's `n_id`."""
+    on the GPU from the batch's `n_id`.  `feature_dropout` drops elements of every type's `x` with
+    that probability (`ops.dropout`), for training."""
 
     def __init__(self, data: HeteroCsrGraph, num_neighbors: dict[tuple[str, str, str], list[int]],
                  input_nodes=None, batch_size: int = 128, shuffle: bool = True, replace: bool = False,
                  num_workers: int = 0, pin_memory: bool = False, device: str | None = None,
                  transfer_depth: int = 2, prefetch_factor: int = 2, seed: int | None = None,
-                 max_degree: int | None = None, transform: Callable | None = None, features: dict | None = None):
+                 max_degree: int | None = None, transform: Callable | None = None, features: dict | None = None,
+                 feature_dropout: float = 0.0):
         if num_workers < 0:
             raise ValueError(f"num_workers must be >= 0, got {num_workers}")
         if not num_neighbors:
@@ -138,6 +140,9 @@ class HeteroNeighborLoader:
             self._input_nodes = normalize_input_nodes(node_ids, num_nodes=n_type,
                                                       what=f"input_nodes for node type '{seed_type}'")
             self._num_input_nodes = len(self._input_nodes)
+        self._feature_dropout = FeatureDropout.check(feature_dropout)
+        if self._feature_dropout and not self._stores:
+            raise ValueError("feature_dropout needs features")
         self._rng = np.random.default_rng(seed)
         self._sampling_seeds = np.random.SeedSequence(seed) if seed is not None else None
         self._metrics = HeteroLoaderMetrics()
@@ -163,6 +168,7 @@ class HeteroNeighborLoader:
                                    seed=epoch_sampling_seed(self._sampling_seeds), max_degree=self._max_degree)
         native = NativeHeteroLoader(self.graph, cfg, self._seed_type, prefetch_depth=self.prefetch_factor,
                                     sampler_threads=self._threads, features=self._stores or None)
+        drop = FeatureDropout(self._feature_dropout, cfg.seed)
         dev = torch.device("cuda", self.graph.device)
         submitted = received = 0
         input_ids: dict[int, np.ndarray] = {}
@@ -180,13 +186,13 @@ class HeteroNeighborLoader:
                 batch_idx, sg = got
                 received += 1
                 data = _new_hetero_data()
-                for nt in self._node_types:
+                for t, nt in enumerate(self._node_types):
                     n_id = sg.nodes_t(nt)
                     store = data[nt]
                     store.n_id = n_id
                     store.num_nodes = int(n_id.shape[0])
                     if nt in self._stores:
-                        store.x = sg.x_t(nt)  # gathered on the GPU in the sampling launch chain
+                        store.x = drop(sg.x_t(nt), batch_idx, t)  # gathered on the GPU in the sampling launch chain
                 for et in self._edge_types:
                     data[et].edge_index = sg.edge_index_local_t(*et)
                 seed_store = data[self._seed_type]

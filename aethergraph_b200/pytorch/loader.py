@@ -29,12 +29,13 @@ from typing import Any, Callable, Iterator
 
 import numpy as np
 
+from .. import _lib
 from ..features import FeatureStore
 from ..graph import CsrGraph
 from ..loader import NeighborLoader as NativeLoader
 from ..sampler import SamplingConfig
 
-__all__ = ["Batch", "LoaderMetrics", "NeighborLoader", "epoch_sampling_seed", "make_batch_getter",
+__all__ = ["Batch", "FeatureDropout", "LoaderMetrics", "NeighborLoader", "epoch_sampling_seed", "make_batch_getter",
            "normalize_input_nodes"]
 
 
@@ -150,6 +151,31 @@ def epoch_sampling_seed(seeds: np.random.SeedSequence | None) -> int | None:
     return int(child.generate_state(1, dtype=np.uint64)[0])
 
 
+class FeatureDropout:
+    """Dropout of the batches' feature rows, in place where they were gathered: one pass over rows
+    that are the batch's own.  Batch b of an epoch uses the key batch_seed(epoch seed, b) and a
+    stream of its own per node type, so a seeded loader drops the same elements at any number of workers."""
+
+    STREAM = 0x66656174 << 32  # apart from the counters that sampling under the same key uses
+
+    def __init__(self, p: float, epoch_seed: int | None):
+        self._p = p
+        self._seed = epoch_seed if epoch_seed is not None else epoch_sampling_seed(np.random.SeedSequence())
+
+    @staticmethod
+    def check(p: float) -> float:
+        if not 0.0 <= p < 1.0:
+            raise ValueError(f"feature_dropout must be in [0, 1), got {p}")
+        return float(p)
+
+    def __call__(self, x, batch_idx: int, node_type: int = 0):
+        if self._p == 0.0 or x is None:
+            return x
+        from .. import ops
+
+        return ops.dropout_(x, self._p, _lib.lib().ag_batch_seed(self._seed, batch_idx), self.STREAM + node_type)
+
+
 @dataclass
 class LoaderMetrics:
     """Counters of the most recent epoch (loader.py:296-341)."""
@@ -173,6 +199,7 @@ class NeighborLoader:
     `features` may be a `FeatureStore`, a float32 `[num_nodes, dim]` array (kept in
     GPU memory as f32) or left out in favour of `feature_path` (an AETHFEAT file).
     `num_workers` is the number of native sampler threads (0 and 1 both mean one).
+    `feature_dropout` drops elements of `x` with that probability (`ops.dropout`), for training.
     Not available on this path: `DynamicGraph` inputs, `feature_source`
     (`rdma://`), `input_time`, and the sampling modes `SamplingConfig` rejects.
     """
@@ -185,7 +212,7 @@ class NeighborLoader:
                  seed: int | None = None, generator: np.random.Generator | None = None,
                  max_degree: int | None = None, cumulative: bool = False, subgraph_type: str = "directional",
                  track_edge_ids: bool = True, neighbor_sampler: Callable | None = None, features=None,
-                 feature_path=None, group: int = 8, rng_mode: str = "wyrand_exact"):
+                 feature_path=None, group: int = 8, rng_mode: str = "wyrand_exact", feature_dropout: float = 0.0):
         if not isinstance(data, CsrGraph):
             raise TypeError(f"data must be an aethergraph_b200 Graph resident on the GPU, got {type(data).__name__}")
         if batch_size < 1:
@@ -227,6 +254,9 @@ class NeighborLoader:
                 raise ValueError(f"features.shape[0]={arr.shape[0]} does not match graph num_nodes={n}")
             features = FeatureStore.from_array(np.ascontiguousarray(arr), dtype="f32", device=data.device)
         self._features: FeatureStore | None = features
+        self._feature_dropout = FeatureDropout.check(feature_dropout)
+        if self._feature_dropout and (features is None or neighbor_sampler is not None):
+            raise ValueError("feature_dropout needs features that the loader gathers itself")
         if input_nodes is None:
             self._input_nodes, self._num_input_nodes = None, n
         else:
@@ -260,9 +290,9 @@ class NeighborLoader:
         sampling = dataclasses.replace(self._sampling, seed=epoch_sampling_seed(self._sampling_seeds))
         native = NativeLoader(self.graph, sampling, self.prefetch_factor, self._threads, features=self._features,
                               group=self._group)
-        yield from self._drive_epoch(native, num_batches, get_batch)
+        yield from self._drive_epoch(native, num_batches, get_batch, FeatureDropout(self._feature_dropout, sampling.seed))
 
-    def _drive_epoch(self, native: NativeLoader, num_batches: int, get_batch) -> Iterator:
+    def _drive_epoch(self, native: NativeLoader, num_batches: int, get_batch, drop: FeatureDropout) -> Iterator:
         """Prime a window of submissions, then receive / resubmit one for one
         (loader.py:817-897).  The window is at least `prefetch_factor` and at least
         what the native workers can hold in flight (threads x group)."""
@@ -290,7 +320,7 @@ class NeighborLoader:
                 input_id = torch.from_numpy(np.ascontiguousarray(input_ids.pop(batch_idx))).to(dev, non_blocking=True)
                 seed_index = sg.seed_indices_t
                 data = _make_data(
-                    x=x, edge_index=sg.edge_index_local_t, e_id=sg.edge_ids_t if self._track_edge_ids else None,
+                    x=drop(x, batch_idx), edge_index=sg.edge_index_local_t, e_id=sg.edge_ids_t if self._track_edge_ids else None,
                     n_id=sg.nodes_t, batch_size=int(seed_index.shape[0]), input_id=input_id, seed_index=seed_index,
                     num_nodes=sg.num_nodes, num_sampled_nodes=sg.num_sampled_nodes_per_hop,
                     num_sampled_edges=sg.num_sampled_edges_per_hop)
