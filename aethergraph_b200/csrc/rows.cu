@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 #include "common.cuh"
 #include "internal.h"
@@ -106,49 +107,72 @@ template <typename T, bool VEC> __device__ __forceinline__ Raw<T> load_chunk(con
     }
     return r;
 }
-template <typename T> __device__ __forceinline__ void unpack(const Raw<T> &r, float v[kChunk]) {
-    T e[kChunk];
-    memcpy(e, &r, sizeof r);
+// Pairs at a time: one instruction converts or packs two 16-bit values that share a register, and
+// sm_100 multiplies and adds two f32 at once.
+__device__ __forceinline__ float2 pair_f32(__half, uint32_t w) { return __half22float2(*(__half2 *)&w); }
+__device__ __forceinline__ float2 pair_f32(__nv_bfloat16, uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ uint32_t pair_bits(__half, float2 v) { const __half2 h = __float22half2_rn(v); return *(const uint32_t *)&h; }
+__device__ __forceinline__ uint32_t pair_bits(__nv_bfloat16, float2 v) { const __nv_bfloat162 h = __float22bfloat162_rn(v); return *(const uint32_t *)&h; }
+
+constexpr int kPairs = kChunk / 2;
+struct Chunk { float2 p[kPairs]; };
+template <typename T> __device__ __forceinline__ Chunk unpack(const Raw<T> &r) {
+    Chunk v;
 #pragma unroll
-    for (uint32_t i = 0; i < kChunk; ++i) v[i] = to_f32(e[i]);
+    for (int i = 0; i < kPairs; ++i) {
+        if constexpr (sizeof(T) == 4) v.p[i] = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+        else v.p[i] = pair_f32(T(), r.w[i]);
+    }
+    return v;
 }
-template <typename T> __device__ __forceinline__ Raw<T> pack(const float v[kChunk]) {
-    T e[kChunk];
-#pragma unroll
-    for (uint32_t i = 0; i < kChunk; ++i) e[i] = from_f32<T>(v[i]);
+template <typename T> __device__ __forceinline__ Raw<T> pack(const Chunk &v) {
     Raw<T> r;
-    memcpy(&r, e, sizeof r);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+        if constexpr (sizeof(T) == 4) { r.w[2 * i] = __float_as_uint(v.p[i].x); r.w[2 * i + 1] = __float_as_uint(v.p[i].y); }
+        else r.w[i] = pair_bits(T(), v.p[i]);
+    }
     return r;
 }
-template <typename T, bool VEC> __device__ __forceinline__ void store_chunk(T *row, const Columns<VEC> &c, uint32_t dim, const float v[kChunk]) {
+__device__ __forceinline__ float &at(Chunk &v, uint32_t i) { return i & 1 ? v.p[i / 2].y : v.p[i / 2].x; }
+__device__ __forceinline__ float at(const Chunk &v, uint32_t i) { return i & 1 ? v.p[i / 2].y : v.p[i / 2].x; }
+__device__ __forceinline__ Chunk filled(float f) {
+    Chunk v;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) v.p[i] = make_float2(f, f);
+    return v;
+}
+__device__ __forceinline__ float2 both(float f) { return make_float2(f, f); }
+template <typename T, bool VEC> __device__ __forceinline__ void store_chunk(T *row, const Columns<VEC> &c, uint32_t dim, const Chunk &v) {
     if (VEC && c.first + kChunk <= dim) {
         store_words(pack<T>(v), row + c.first);
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
-            if (c.at(i) < dim) row[c.at(i)] = from_f32<T>(v[i]);
+            if (c.at(i) < dim) row[c.at(i)] = from_f32<T>(at(v, i));
     }
 }
 // The norm's weights, of the rows' type or f32: the same few for every row (L1).
-template <typename T, bool VEC> __device__ __forceinline__ void load_weight(const void *w, int w_f32, const Columns<VEC> &c, uint32_t dim, float v[kChunk]) {
-    if (!w) {
-#pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) v[i] = 1.f;
-    } else if (VEC && c.first + kChunk <= dim) {
-        if (w_f32) {
+template <typename T, bool VEC> __device__ __forceinline__ Chunk load_weight(const void *w, int w_f32, const Columns<VEC> &c, uint32_t dim) {
+    if (!w) return filled(1.f);
+    Chunk v;
+    if (VEC && c.first + kChunk <= dim) {
+        if (sizeof(T) == 4 || w_f32) {
             const float4 lo = __ldg((const float4 *)((const float *)w + c.first)), hi = __ldg((const float4 *)((const float *)w + c.first) + 1);
-            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w; v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+            v.p[0] = make_float2(lo.x, lo.y); v.p[1] = make_float2(lo.z, lo.w);
+            v.p[2] = make_float2(hi.x, hi.y); v.p[3] = make_float2(hi.z, hi.w);
         } else if constexpr (sizeof(T) == 2) {
             const uint4 q = __ldg((const uint4 *)((const T *)w + c.first));
             Raw<T> r;
-            memcpy(&r, &q, sizeof q);
-            unpack(r, v);
+            r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
+            v = unpack(r);
         }
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
-            v[i] = c.at(i) >= dim ? 0.f : w_f32 ? __ldg((const float *)w + c.at(i)) : to_f32(((const T *)w)[c.at(i)]);
+            at(v, i) = c.at(i) >= dim ? 0.f : sizeof(T) == 4 || w_f32 ? __ldg((const float *)w + c.at(i)) : to_f32(((const T *)w)[c.at(i)]);
     }
+    return v;
 }
 
 // ---------------------------------------------------------------- dropout --
@@ -168,24 +192,30 @@ __device__ __forceinline__ uint32_t lot(const uint4 &r, uint32_t i) {
     const uint32_t w = i < 2 ? r.x : i < 4 ? r.y : i < 6 ? r.z : r.w;
     return i & 1 ? w : w << 16;
 }
-// A select: a dropped infinity or NaN is gone.
-__device__ __forceinline__ float kept(const Drop &d, uint32_t bits, float v) { return bits > d.bar ? v * d.scale : 0.f; }
+// Selects: a dropped infinity or NaN is gone.
+__device__ __forceinline__ float kept(const Drop &d, uint32_t bits, float v) { return bits > d.bar ? v : 0.f; }
+__device__ __forceinline__ void drop_chunk(const Drop &d, const uint4 &lots, Chunk &v) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+        const float2 f = __fmul2_rn(v.p[i], both(d.scale));
+        v.p[i] = make_float2(kept(d, lot(lots, 2 * i), f.x), kept(d, lot(lots, 2 * i + 1), f.y));
+    }
+}
 
 // Dropout of a thread's eight columns.  Unless they are a chunk, the group's lanes make the lots of one
 // chunk each and pass them around in shared memory (16 bytes a lane); the whole warp calls this.
 template <bool VEC>
-__device__ __forceinline__ void drop_columns(const Drop &d, uint64_t row, uint32_t lane, uint32_t lanes, uint32_t step_chunk, uint4 *warp_lots, float v[kChunk]) {
+__device__ __forceinline__ void drop_columns(const Drop &d, uint32_t row, uint32_t lane, uint32_t lanes, uint32_t step_chunk, uint4 *warp_lots, Chunk &v) {
     const uint4 r = lots_of(d, row, step_chunk + lane);
     if (VEC) {
-#pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) v[i] = kept(d, lot(r, i), v[i]);
+        drop_chunk(d, r, v);
     } else {
         __syncwarp();
         warp_lots[threadIdx.x & 31] = r;
         __syncwarp();
         const uint16_t *group = (const uint16_t *)(warp_lots + ((threadIdx.x & 31) - lane));
 #pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) v[i] = kept(d, (uint32_t)group[lane + i * lanes] << 16, v[i]);
+        for (uint32_t i = 0; i < kChunk; ++i) at(v, i) = kept(d, (uint32_t)group[lane + i * lanes] << 16, at(v, i) * d.scale);
     }
 }
 
@@ -208,10 +238,8 @@ k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_
     for (int u = 0; u < 2; ++u) {
         if (((uint64_t)blockIdx.x * 2 + u) * kThreads + threadIdx.x >= total) break;
         const uint4 lots = lots_of(d, row[u], chunk[u]);
-        float v[kChunk];
-        unpack(r[u], v);
-#pragma unroll
-        for (uint32_t e = 0; e < kChunk; ++e) v[e] = kept(d, lot(lots, e), v[e]);
+        Chunk v = unpack(r[u]);
+        drop_chunk(d, lots, v);
         store_chunk<T, VEC>(y + row[u] * y_stride, Columns<VEC>(0, 1, chunk[u]), dim, v);
     }
 }
@@ -259,10 +287,12 @@ k_dropout_flat(const T *x, T *y, uint64_t total, Divide dim, Divide chunks, Drop
         if (f >= total) break;
         const uint32_t m = ((const uint8_t *)stays)[threadIdx.x + j * kThreads];
         if (f + kChunk <= total) {
-            float v[kChunk];
-            unpack(r[j], v);
+            Chunk v = unpack(r[j]);
 #pragma unroll
-            for (uint32_t e = 0; e < kChunk; ++e) v[e] = m >> e & 1 ? v[e] * d.scale : 0.f;
+            for (int i = 0; i < kPairs; ++i) {
+                const float2 s = __fmul2_rn(v.p[i], both(d.scale));
+                v.p[i] = make_float2(m >> 2 * i & 1 ? s.x : 0.f, m >> (2 * i + 1) & 1 ? s.y : 0.f);
+            }
             store_words(pack<T>(v), y + f);
         } else {
             for (uint32_t e = 0; f + e < total; ++e) y[f + e] = from_f32<T>(m >> e & 1 ? to_f32(x[f + e]) * d.scale : 0.f);
@@ -277,7 +307,7 @@ struct NormArgs {
     float *rstd;
     uint8_t *codes;  // 8-bit output instead of y
     float *scales;
-    uint64_t rows, x_stride, res_stride, y_stride, h_stride, code_stride;
+    uint32_t rows, x_stride, res_stride, y_stride, h_stride, code_stride;  // pitches in elements
     uint32_t dim;
     int w_f32, plain;  // plain: no norm, the rows themselves are encoded
     float eps, inv_dim;
@@ -313,17 +343,18 @@ __device__ __forceinline__ float scale_of(uint32_t top, float &inv) {
     return scale;
 }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-__device__ __forceinline__ uint32_t code2(float a, float b, float inv) {  // a reciprocal of 0: a block that is not finite
-    return inv == 0.f ? 0u : (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
+// A reciprocal of 0 (a block that is not finite) gives codes of 0 or NaN: its scale is NaN anyway.
+__device__ __forceinline__ uint32_t code2(float2 v, float inv) {
+    return __nv_cvt_float2_to_fp8x2(__fmul2_rn(v, both(inv)), __NV_SATFINITE, __NV_E4M3);
 }
 
 // e4m3 codes and scales of a group's step; the whole warp calls this.
 template <bool VEC>
-__device__ __forceinline__ void encode_columns(const float v[kChunk], const Columns<VEC> &c, uint32_t lane, uint32_t lanes, uint32_t dim, uint8_t *codes, float *scales) {
+__device__ __forceinline__ void encode_columns(const Chunk &v, const Columns<VEC> &c, uint32_t lane, uint32_t lanes, uint32_t dim, uint8_t *codes, float *scales) {
     if (VEC) {  // the 16 lanes of a block reduce; a chunk lies in one block
         uint32_t top = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) top = max(top, magnitude(v[i]));
+        for (uint32_t i = 0; i < kChunk; ++i) top = max(top, magnitude(at(v, i)));
         #pragma unroll
         for (uint32_t o = 8; o > 0; o /= 2)
             if (o < lanes) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -332,11 +363,11 @@ __device__ __forceinline__ void encode_columns(const float v[kChunk], const Colu
         const float scale = scale_of(top, inv);
         if (c.first % kF8Block == 0) scales[c.first / kF8Block] = scale;
         // the pitch is a multiple of 16 bytes, so its padding takes what a last chunk writes past the row
-        *(uint2 *)(codes + c.first) = make_uint2(code2(v[0], v[1], inv) | code2(v[2], v[3], inv) << 16, code2(v[4], v[5], inv) | code2(v[6], v[7], inv) << 16);
+        *(uint2 *)(codes + c.first) = make_uint2(code2(v.p[0], inv) | code2(v.p[1], inv) << 16, code2(v.p[2], inv) | code2(v.p[3], inv) << 16);
     } else {  // 32 lanes: columns 0 - 3 of each thread are one block, 4 - 7 the next; fewer lanes have at most one block
         uint32_t lo = 0, hi = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kChunk / 2; ++i) { lo = max(lo, magnitude(v[i])); hi = max(hi, magnitude(v[i + kChunk / 2])); }
+        for (uint32_t i = 0; i < kChunk / 2; ++i) { lo = max(lo, magnitude(at(v, i))); hi = max(hi, magnitude(at(v, i + kChunk / 2))); }
         if (lanes < 32) lo = hi = max(lo, hi);
 #pragma unroll
         for (uint32_t o = 16; o > 0; o /= 2) {
@@ -352,7 +383,7 @@ __device__ __forceinline__ void encode_columns(const float v[kChunk], const Colu
         }
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
-            if (c.at(i) < dim) codes[c.at(i)] = (uint8_t)code2(v[i], 0.f, i < kChunk / 2 ? inv_lo : inv_hi);
+            if (c.at(i) < dim) codes[c.at(i)] = (uint8_t)code2(make_float2(at(v, i), 0.f), i < kChunk / 2 ? inv_lo : inv_hi);
     }
 }
 
@@ -366,60 +397,65 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
     __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
     uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
     const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
-    const uint64_t row = BLOCK ? blockIdx.x : (uint64_t)blockIdx.x * (kThreads >> log2_lanes) + (threadIdx.x >> log2_lanes);
+    const uint32_t row = BLOCK ? blockIdx.x : blockIdx.x * (kThreads >> log2_lanes) + (threadIdx.x >> log2_lanes);
     const uint32_t dim = row < a.rows ? a.dim : 0;  // lanes without a row still take part in the exchanges
-    float v[C][kChunk];
+    Chunk v[C];
     {
+        const T *x = (const T *)a.x + (uint64_t)row * a.x_stride, *res = (const T *)a.res + (uint64_t)row * a.res_stride;
         Raw<T> rx[C], rr[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const Columns<VEC> c(lane, lanes, j * width + group_chunk);
             if (c.first >= dim) continue;
-            rx[j] = load_chunk<T, VEC>((const T *)a.x + row * a.x_stride, c, dim);
-            if (a.res) rr[j] = load_chunk<T, VEC>((const T *)a.res + row * a.res_stride, c, dim);
+            rx[j] = load_chunk<T, VEC>(x, c, dim);
+            if (a.res) rr[j] = load_chunk<T, VEC>(res, c, dim);
         }
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const uint32_t step = j * width + group_chunk;
             const Columns<VEC> c(lane, lanes, step);
-#pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) v[j][i] = 0.f;
-            if (c.first < dim) unpack(rx[j], v[j]);
+            v[j] = c.first < dim ? unpack(rx[j]) : filled(0.f);
             if (a.drop.on) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, v[j]);
             if (a.res && c.first < dim) {
-                float r[kChunk];
-                unpack(rr[j], r);
+                const Chunk r = unpack(rr[j]);
 #pragma unroll
-                for (uint32_t i = 0; i < kChunk; ++i) v[j][i] += r[i];
+                for (int i = 0; i < kPairs; ++i) v[j].p[i] = __fadd2_rn(v[j].p[i], r.p[i]);
             }
         }
     }
-    float sum = 0.f;
+    if (a.h) {
+        T *h = (T *)a.h + (uint64_t)row * a.h_stride;
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-        const Columns<VEC> c(lane, lanes, j * width + group_chunk);
-        if (a.h && c.first < dim) store_chunk<T, VEC>((T *)a.h + row * a.h_stride, c, dim, v[j]);
-#pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) sum += v[j][i] * v[j][i];
+        for (int j = 0; j < C; ++j) {
+            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+            if (c.first < dim) store_chunk<T, VEC>(h, c, dim, v[j]);
+        }
     }
     if (!a.plain) {
-        const float rstd = rsqrtf(row_sum<BLOCK, false>(sum, lanes, shared) * a.inv_dim + a.eps);
+        float2 sum = both(0.f);
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) sum = __ffma2_rn(v[j].p[i], v[j].p[i], sum);
+        const float rstd = rsqrtf(row_sum<BLOCK, false>(sum.x + sum.y, lanes, shared) * a.inv_dim + a.eps);
         if (a.rstd && dim && (BLOCK ? threadIdx.x : lane) == 0) a.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const Columns<VEC> c(lane, lanes, j * width + group_chunk);
             if (c.first >= dim) continue;
-            float w[kChunk];
-            load_weight<T, VEC>(a.weight, a.w_f32, c, dim, w);
+            const Chunk w = load_weight<T, VEC>(a.weight, a.w_f32, c, dim);
 #pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) v[j][i] *= rstd * w[i];
+            for (int i = 0; i < kPairs; ++i) v[j].p[i] = __fmul2_rn(v[j].p[i], __fmul2_rn(w.p[i], both(rstd)));
         }
     }
+    T *y = (T *)a.y + (uint64_t)row * a.y_stride;
+    uint8_t *codes = a.codes + (uint64_t)row * a.code_stride;
+    float *scales = a.scales + (uint64_t)row * ((a.dim + kF8Block - 1) / kF8Block);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
         const Columns<VEC> c(lane, lanes, j * width + group_chunk);
-        if (F8) encode_columns<VEC>(v[j], c, lane, lanes, dim, a.codes + row * a.code_stride, a.scales + row * ((a.dim + kF8Block - 1) / kF8Block));
-        else if (c.first < dim) store_chunk<T, VEC>((T *)a.y + row * a.y_stride, c, dim, v[j]);
+        if (F8) encode_columns<VEC>(v[j], c, lane, lanes, dim, codes, scales);
+        else if (c.first < dim) store_chunk<T, VEC>(y, c, dim, v[j]);
     }
 }
 
@@ -428,7 +464,7 @@ struct NormBackArgs {
     const float *rstd;
     void *dx, *dres;
     float *partial;  // [blocks, dim] sums of dy h rstd over a block's rows, or null
-    uint64_t rows, dy_stride, dh_stride, h_stride;
+    uint32_t rows, dy_stride, dh_stride, h_stride;
     uint32_t dim;
     int w_f32;
     float inv_dim;
@@ -440,7 +476,7 @@ struct NormBackArgs {
 // sums; a block adds its lane groups in order into its row of `partial`, and k_norm_dw adds those.
 // No atomics: the same bits every time on the same GPU.
 template <typename T, bool VEC, int C, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : C == 1 ? 4 : 2)
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? (C == 1 ? 2 : 1) : C == 1 ? 4 : 2)
 k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
     const uint32_t lanes = C > 1 || BLOCK ? 32 : 1u << log2_lanes;
     __shared__ float shared[32];
@@ -448,58 +484,53 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
     extern __shared__ float sums[];  // [groups of the block][dim], not BLOCK
     uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
     const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
-    const uint64_t per_block = BLOCK ? 1 : kThreads >> log2_lanes;
-    float dw[C][kChunk];
+    const uint32_t per_block = BLOCK ? 1 : kThreads >> log2_lanes;
+    Chunk dw[C];
 #pragma unroll
-    for (int j = 0; j < C; ++j)
-#pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) dw[j][i] = 0.f;
-    for (uint64_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block) {
-        const uint64_t row = base + (BLOCK ? 0 : threadIdx.x >> log2_lanes);
+    for (int j = 0; j < C; ++j) dw[j] = filled(0.f);
+    for (uint32_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block) {  // rows + a grid's worth fit 32 bits
+        const uint32_t row = base + (BLOCK ? 0 : threadIdx.x >> log2_lanes);
         const uint32_t dim = row < a.rows ? a.dim : 0;
+        const T *h_row = (const T *)a.h + (uint64_t)row * a.h_stride, *dy_row = (const T *)a.dy + (uint64_t)row * a.dy_stride,
+                *dh_row = (const T *)a.dh + (uint64_t)row * a.dh_stride;
         Raw<T> ry[C], rh[C], rd[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const Columns<VEC> c(lane, lanes, j * width + group_chunk);
             ry[j] = rh[j] = rd[j] = Raw<T>{};
             if (c.first >= dim) continue;
-            rh[j] = load_chunk<T, VEC>((const T *)a.h + row * a.h_stride, c, dim);
-            if (a.dy) ry[j] = load_chunk<T, VEC>((const T *)a.dy + row * a.dy_stride, c, dim);
-            if (a.dh) rd[j] = load_chunk<T, VEC>((const T *)a.dh + row * a.dh_stride, c, dim);
+            rh[j] = load_chunk<T, VEC>(h_row, c, dim);
+            if (a.dy) ry[j] = load_chunk<T, VEC>(dy_row, c, dim);
+            if (a.dh) rd[j] = load_chunk<T, VEC>(dh_row, c, dim);
         }
         const float rstd = dim ? a.rstd[row] : 0.f;
-        float sum = 0.f;
+        Chunk gw[C], h[C];  // dy w and h
+        float2 sum = both(0.f);
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const Columns<VEC> c(lane, lanes, j * width + group_chunk);
-            if (c.first >= dim) continue;
-            float g[kChunk], h[kChunk], w[kChunk];
-            unpack(rh[j], h);
-            unpack(ry[j], g);
-            load_weight<T, VEC>(a.weight, a.w_f32, c, dim, w);
+            const Chunk g = unpack(ry[j]), w = c.first < dim ? load_weight<T, VEC>(a.weight, a.w_f32, c, dim) : filled(0.f);
+            h[j] = unpack(rh[j]);
 #pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) {
-                const float gh = g[i] * h[i];
-                dw[j][i] += gh * rstd;
-                sum += gh * w[i];
+            for (int i = 0; i < kPairs; ++i) {
+                dw[j].p[i] = __ffma2_rn(__fmul2_rn(g.p[i], h[j].p[i]), both(rstd), dw[j].p[i]);
+                gw[j].p[i] = __fmul2_rn(g.p[i], w.p[i]);
+                sum = __ffma2_rn(gw[j].p[i], h[j].p[i], sum);
             }
         }
-        const float coef = row_sum<BLOCK, true>(sum, lanes, shared) * rstd * rstd * rstd * a.inv_dim;
+        const float coef = -row_sum<BLOCK, true>(sum.x + sum.y, lanes, shared) * rstd * rstd * rstd * a.inv_dim;
+        T *dres = (T *)a.dres + (uint64_t)row * a.dim, *dx = (T *)a.dx + (uint64_t)row * a.dim;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const uint32_t step = j * width + group_chunk;
             const Columns<VEC> c(lane, lanes, step);
-            float t[kChunk], g[kChunk], h[kChunk], w[kChunk];  // unpacked again: fewer registers across the sum
-            unpack(rh[j], h);
-            unpack(ry[j], g);
-            unpack(rd[j], t);
-            load_weight<T, VEC>(a.weight, a.w_f32, c, dim, w);
+            Chunk t = unpack(rd[j]);
 #pragma unroll
-            for (uint32_t i = 0; i < kChunk; ++i) t[i] += rstd * (g[i] * w[i]) - h[i] * coef;
-            if (a.dres && c.first < dim) store_chunk<T, VEC>((T *)a.dres + row * a.dim, c, dim, t);
+            for (int i = 0; i < kPairs; ++i) t.p[i] = __fadd2_rn(t.p[i], __ffma2_rn(gw[j].p[i], both(rstd), __fmul2_rn(h[j].p[i], both(coef))));
+            if (a.dres && c.first < dim) store_chunk<T, VEC>(dres, c, dim, t);
             if (a.dx) {
                 if (a.drop.on) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, t);
-                if (c.first < dim) store_chunk<T, VEC>((T *)a.dx + row * a.dim, c, dim, t);
+                if (c.first < dim) store_chunk<T, VEC>(dx, c, dim, t);
             }
         }
     }
@@ -511,7 +542,7 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
         float *to = BLOCK ? mine : sums + (threadIdx.x >> log2_lanes) * a.dim;
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
-            if (c.at(i) < a.dim) to[c.at(i)] = dw[j][i];
+            if (c.at(i) < a.dim) to[c.at(i)] = at(dw[j], i);
     }
     if (BLOCK) return;
     __syncthreads();
@@ -569,7 +600,7 @@ k_encode_weight(const T *w, uint64_t out, uint32_t dim, uint64_t stride, uint8_t
         const uint64_t n = bn * kF8Block + i / kF8Block;
         const uint32_t c = bk * kF8Block + i % kF8Block;
         if (n < out && c < dim)
-            codes[n * code_stride + c] = (uint8_t)code2(to_f32(w[n * stride + c]), 0.f, inv);
+            codes[n * code_stride + c] = (uint8_t)code2(make_float2(to_f32(w[n * stride + c]), 0.f), inv);
     }
 }
 
@@ -597,8 +628,14 @@ int32_t make_drop(double p, uint64_t seed, uint64_t offset, Drop *d) {
 
 int32_t check_rows(const char *who, uint64_t rows, uint64_t dim, int32_t dtype) {
     if (dtype < AG_F32 || dtype > AG_BF16) return fail(AG_ERR_VALUE, "%s: rows are f32, f16 or bf16, got dtype tag %d", who, dtype);
-    if (rows > 0xFFFFFFFFull) return fail(AG_ERR_VALUE, "%s: at most 2^32 - 1 rows, got %llu", who, (unsigned long long)rows);
+    if (rows > 0xF0000000ull) return fail(AG_ERR_VALUE, "%s: at most 0xF0000000 rows, got %llu", who, (unsigned long long)rows);
     if (dim == 0 || dim > 0xFFFFFFF0ull) return fail(AG_ERR_VALUE, "%s: rows of 1 to 2^32 - 16 columns, got %llu", who, (unsigned long long)dim);
+    return AG_OK;
+}
+
+int32_t check_pitches(const char *who, std::initializer_list<uint64_t> pitches) {
+    for (const uint64_t p : pitches)
+        if (p > 0xFFFFFFFFull) return fail(AG_ERR_VALUE, "%s: rows at most 2^32 - 1 elements apart, got %llu", who, (unsigned long long)p);
     return AG_OK;
 }
 
@@ -700,8 +737,7 @@ k_encode_rows(const float *src, uint64_t rows, uint32_t dim, uint64_t pitch, uin
         for (uint32_t c0 = 0; c0 < dim; c0 += kThreads * kChunk) {
             const uint32_t lane = threadIdx.x & 31;
             const Columns<false> c(lane, 32, c0 / kChunk + (threadIdx.x & ~31u));
-            float v[kChunk];
-            unpack(load_chunk<float, false>(src + row * dim, c, dim), v);
+            const Chunk v = unpack(load_chunk<float, false>(src + row * dim, c, dim));
             encode_columns<false>(v, c, lane, 32, dim, codes + row * pitch, scales + row * per_row);
         }
 }
@@ -767,12 +803,13 @@ extern "C" int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream) 
         return fail(AG_ERR_VALUE, "ag_rows_norm: encoding alone takes rows and gives 8-bit rows");
     if (n->codes && (n->code_stride % 16 != 0 || n->code_stride < n->dim || (uintptr_t)n->codes % 16 != 0))
         return fail(AG_ERR_VALUE, "ag_rows_norm: 8-bit rows start on multiples of 16 bytes and do not overlap");
+    AG_TRY(check_pitches("ag_rows_norm", {n->x_stride, n->residual_stride, n->y_stride, n->h_stride, n->code_stride}));
     if ((n->y && n->y_stride < n->dim) || (n->h && n->h_stride < n->dim)) return fail(AG_ERR_VALUE, "ag_rows_norm: rows of the output overlap");
     DeviceGuard guard(device);
     if (!guard.ok) return AG_ERR_CUDA;
     a.x = n->x; a.res = n->residual; a.weight = n->weight; a.y = n->y; a.h = n->h; a.rstd = n->rstd;
-    a.codes = (uint8_t *)n->codes; a.scales = n->scales; a.rows = n->rows; a.x_stride = n->x_stride; a.res_stride = n->residual_stride;
-    a.y_stride = n->y_stride; a.h_stride = n->h_stride; a.code_stride = n->code_stride; a.dim = (uint32_t)n->dim;
+    a.codes = (uint8_t *)n->codes; a.scales = n->scales; a.rows = (uint32_t)n->rows; a.x_stride = (uint32_t)n->x_stride; a.res_stride = (uint32_t)n->residual_stride;
+    a.y_stride = (uint32_t)n->y_stride; a.h_stride = (uint32_t)n->h_stride; a.code_stride = (uint32_t)n->code_stride; a.dim = (uint32_t)n->dim;
     a.w_f32 = n->weight_dtype == AG_F32; a.plain = n->encode_only; a.eps = n->eps; a.inv_dim = 1.0f / (float)n->dim;
     const uint32_t e = elem_size(n->dtype);
     const bool vec = vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.y, a.y_stride, e) && vec_rows(a.h, a.h_stride, e);
@@ -803,6 +840,7 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
     if (n->dim > kMaxNormDim) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: at most %u columns, got %llu", kMaxNormDim, (unsigned long long)n->dim);
     if (n->weight && n->weight_dtype != n->dtype && n->weight_dtype != AG_F32)
         return fail(AG_ERR_VALUE, "ag_rows_norm_backward: the weights are f32 or of the rows' type");
+    AG_TRY(check_pitches("ag_rows_norm_backward", {n->dy_stride, n->dh_stride, n->h_stride}));
     NormBackArgs a{};
     AG_TRY(make_drop(n->p, n->seed, n->offset, &a.drop));
     DeviceGuard guard(device);
@@ -818,7 +856,7 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
                     (unsigned long long)grid * n->dim * 4);
     a.dy = n->dy; a.dh = n->dh; a.h = n->h; a.weight = n->weight; a.rstd = n->rstd; a.dx = n->dx; a.dres = n->dresidual;
     a.partial = n->dw ? (float *)n->scratch : nullptr;
-    a.rows = n->rows; a.dim = (uint32_t)n->dim; a.dy_stride = n->dy_stride; a.dh_stride = n->dh_stride; a.h_stride = n->h_stride;
+    a.rows = (uint32_t)n->rows; a.dim = (uint32_t)n->dim; a.dy_stride = (uint32_t)n->dy_stride; a.dh_stride = (uint32_t)n->dh_stride; a.h_stride = (uint32_t)n->h_stride;
     a.w_f32 = n->weight_dtype == AG_F32; a.inv_dim = 1.0f / (float)n->dim;
     const uint32_t e = elem_size(n->dtype);
     const bool vec = vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
