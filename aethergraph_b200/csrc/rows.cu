@@ -390,7 +390,7 @@ __device__ __forceinline__ void encode_columns(const Chunk &v, const Columns<VEC
 // h = res + dropout(x); y = h rsqrt(mean(h^2) + eps) w.  `lanes` lanes a row (BLOCK: the whole
 // block), C chunks each; the row stays in registers between the sum and the output.
 template <typename T, bool VEC, int C, bool BLOCK, bool F8>
-__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? 1 : C == 1 ? 5 : 4)
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? (sizeof(T) * C <= 8 ? 2 : 1) : C == 1 ? 5 : 4)
 k_norm(const NormArgs a, uint32_t log2_lanes) {
     const uint32_t lanes = C > 1 || BLOCK ? 32 : 1u << log2_lanes;  // more chunks than one: all lanes
     __shared__ float shared[32];
@@ -399,7 +399,7 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
     const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
     const uint32_t row = BLOCK ? blockIdx.x : blockIdx.x * (kThreads >> log2_lanes) + (threadIdx.x >> log2_lanes);
     const uint32_t dim = row < a.rows ? a.dim : 0;  // lanes without a row still take part in the exchanges
-    Chunk v[C];
+    Chunk v[C], w[C];
     {
         const T *x = (const T *)a.x + (uint64_t)row * a.x_stride, *res = (const T *)a.res + (uint64_t)row * a.res_stride;
         Raw<T> rx[C], rr[C];
@@ -409,6 +409,7 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
             if (c.first >= dim) continue;
             rx[j] = load_chunk<T, VEC>(x, c, dim);
             if (a.res) rr[j] = load_chunk<T, VEC>(res, c, dim);
+            if (C == 1) w[j] = load_weight<T, VEC>(a.weight, a.w_f32, c, dim);  // early, where it costs few registers
         }
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -443,9 +444,9 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
         for (int j = 0; j < C; ++j) {
             const Columns<VEC> c(lane, lanes, j * width + group_chunk);
             if (c.first >= dim) continue;
-            const Chunk w = load_weight<T, VEC>(a.weight, a.w_f32, c, dim);
+            if (C > 1) w[j] = load_weight<T, VEC>(a.weight, a.w_f32, c, dim);
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) v[j].p[i] = __fmul2_rn(v[j].p[i], __fmul2_rn(w.p[i], both(rstd)));
+            for (int i = 0; i < kPairs; ++i) v[j].p[i] = __fmul2_rn(v[j].p[i], __fmul2_rn(w[j].p[i], both(rstd)));
         }
     }
     T *y = (T *)a.y + (uint64_t)row * a.y_stride;
@@ -553,24 +554,30 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
     }
 }
 
-// dw[c] = sum of the blocks' partial sums, 32 columns a block, 32 slices of blocks each.
-template <typename T>
+// dw[c] = sum of the blocks' partial sums: COLS columns a block, 1024 / COLS slices of the rows.  Eight columns
+// (a sector of every partial row) as long as that is no more than one block per SM, 32 beyond: 602
+// columns (19 blocks of 32) 9.5 and 5.8 us, 4096 columns (512 blocks of 8) 5.6 and 9.8.
+template <typename T, uint32_t kDwCols>
 __global__ void __launch_bounds__(1024)
 k_norm_dw(const float *partial, uint32_t blocks, uint32_t dim, T *dw) {
-    __shared__ float sums[32][33];
-    const uint32_t c = blockIdx.x * 32 + threadIdx.x;
+    constexpr uint32_t kDwSlices = 1024 / kDwCols;
+    __shared__ float sums[kDwSlices][kDwCols + 1];
+    const uint32_t c = blockIdx.x * kDwCols + threadIdx.x;
     float s = 0.f;
     if (c < dim) {
 #pragma unroll 8
-        for (uint32_t b = threadIdx.y; b < blocks; b += 32) s += partial[(uint64_t)b * dim + c];
+        for (uint32_t b = threadIdx.y; b < blocks; b += kDwSlices) s += partial[(uint64_t)b * dim + c];
     }
     sums[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    s = sums[threadIdx.x][threadIdx.y];  // column threadIdx.y of the 32, slice threadIdx.x
+    const uint32_t thread = threadIdx.y * kDwCols + threadIdx.x, column = thread / 32, lane = thread % 32, out = blockIdx.x * kDwCols + column;
+    if (column >= kDwCols) return;
+    s = 0.f;
+#pragma unroll
+    for (uint32_t q = 0; q < kDwSlices / 32; ++q) s += sums[q * 32 + lane][column];
 #pragma unroll
     for (uint32_t o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const uint32_t out = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && out < dim) dw[out] = from_f32<T>(s);
+    if (lane == 0 && out < dim) dw[out] = from_f32<T>(s);
 }
 
 // ---------------------------------------------------- weights in 8 bits --
@@ -642,13 +649,14 @@ int32_t check_pitches(const char *who, std::initializer_list<uint64_t> pitches) 
 // How a row of `dim` columns is shared out: `lanes` of a warp (0: a whole block of `threads`) with up to
 // `chunks` chunks each.  Whole blocks: as few threads as hold the row in
 // `most` chunks each (64 bytes of f16 / bf16 or f32: a thread's loads are all in flight together, and the sum
-// waits for fewer warps), unless that leaves many of them idle.
+// waits for fewer warps), unless that leaves many of them idle; a chunk each where there are no more rows than
+// SMs, and the time is one row's latency.  16 384 rows of 4096 f16, forward: four chunks 52 us, two 64, one 66.
 struct Split {
     uint32_t lanes, threads;
     int chunks;
     uint32_t log2_lanes() const { uint32_t l = 0; while ((1u << l) < lanes) ++l; return lanes ? l : 5; }
 };
-Split split_row(uint32_t dim, int dtype) {
+Split split_row(uint64_t rows, uint32_t dim, int dtype) {
     const uint32_t n = (dim + kChunk - 1) / kChunk;
     Split s{1, kThreads, 1};
     if (n <= 64) {
@@ -657,19 +665,23 @@ Split split_row(uint32_t dim, int dtype) {
         return s;
     }
     s.lanes = 0;
+    const int most = rows <= (uint64_t)kSMs ? 1 : dtype == AG_F32 ? 2 : 4;
     uint32_t slots = 0xFFFFFFFFu;
-    for (int c = dtype == AG_F32 ? 2 : 4; c; c /= 2) {
+    for (int c = most; c; c /= 2) {
         const uint32_t threads = (n + 32 * c - 1) / (32 * c) * 32;
         if (threads > 512 || threads * c + threads * c / 8 >= slots) continue;
         slots = threads * c; s.threads = threads; s.chunks = c;
     }
-    if (slots == 0xFFFFFFFFu) { s.chunks = 4; s.threads = 512; }
+    if (slots == 0xFFFFFFFFu) {  // longer than that many chunks a thread
+        s.chunks = n <= 1024 ? 2 : 4;
+        s.threads = (n + 32 * s.chunks - 1) / (32 * s.chunks) * 32;
+    }
     return s;
 }
 
 template <typename T, bool VEC, bool F8>
 cudaError_t launch_norm(const NormArgs &a, int dtype, cudaStream_t st) {
-    const Split s = split_row(a.dim, dtype);
+    const Split s = split_row(a.rows, a.dim, dtype);
     const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
     const uint32_t grid = (uint32_t)((a.rows + per - 1) / per), lanes = s.log2_lanes();  // rows of a whole block are 2 KB and more
     if (s.lanes) {
@@ -690,7 +702,7 @@ uint32_t back_blocks(uint64_t rows, const Split &s, uint32_t per_sm) {
     return (uint32_t)std::min<uint64_t>((rows + per - 1) / per, (uint64_t)kSMs * per_sm);
 }
 uint32_t back_blocks_bound(uint64_t rows, uint32_t dim, int dtype) {
-    const Split s = split_row(dim, dtype);
+    const Split s = split_row(rows, dim, dtype);
     return back_blocks(rows, s, std::min(2048 / s.threads, 32u));
 }
 
@@ -707,7 +719,7 @@ cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t &grid, c
 
 template <typename T, bool VEC>
 cudaError_t launch_back(const NormBackArgs &a, int dtype, uint32_t &grid, cudaStream_t st) {
-    const Split s = split_row(a.dim, dtype);
+    const Split s = split_row(a.rows, a.dim, dtype);
     if (s.lanes) {
         if (s.chunks == 1) return launch_back<T, VEC, 1, false>(a, s, grid, st);
         return launch_back<T, VEC, 2, false>(a, s, grid, st);
@@ -870,7 +882,10 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
     if (n->dw)
         with_type(n->weight_dtype, [&](auto *t) {
             using T = std::remove_pointer_t<decltype(t)>;
-            k_norm_dw<T><<<((uint32_t)n->dim + 31) / 32, dim3(32, 32), 0, (cudaStream_t)stream>>>((const float *)n->scratch, grid, (uint32_t)n->dim, (T *)n->dw);
+            const float *partial = (const float *)n->scratch;
+            const uint32_t dim = (uint32_t)n->dim;
+            if (dim <= (uint32_t)kSMs * 8) k_norm_dw<T, 8><<<(dim + 7) / 8, dim3(8, 128), 0, (cudaStream_t)stream>>>(partial, grid, dim, (T *)n->dw);
+            else k_norm_dw<T, 32><<<(dim + 31) / 32, dim3(32, 32), 0, (cudaStream_t)stream>>>(partial, grid, dim, (T *)n->dw);
         });
     AG_CUDA(cudaGetLastError());
     return AG_OK;
