@@ -108,6 +108,7 @@ void dropout_(const Tensor &x, double p, uint64_t seed, uint64_t offset) {
     if (!r.t.is_same(x) || (r.rows > 1 && r.pitch < r.dim)) refuse("dropout_ needs rows of consecutive columns that do not overlap");
     const int64_t pitch = std::max(r.pitch, r.dim);  // the pitch of a single row is free
     check(ag_rows_dropout(x.data_ptr(), x.data_ptr(), r.rows, r.dim, pitch, pitch, tag, p, seed, offset, x.get_device(), stream_of(x)));
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();  // whoever saved x for a backward pass is told
 }
 
 // -------------------------------------------------------------------- norm --

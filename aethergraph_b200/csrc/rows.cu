@@ -13,6 +13,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <initializer_list>
 
@@ -237,9 +238,8 @@ k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         if (((uint64_t)blockIdx.x * 2 + u) * kThreads + threadIdx.x >= total) break;
-        const uint4 lots = lots_of(d, row[u], chunk[u]);
         Chunk v = unpack(r[u]);
-        drop_chunk(d, lots, v);
+        if (d.on) drop_chunk(d, lots_of(d, row[u], chunk[u]), v);
         store_chunk<T, VEC>(y + row[u] * y_stride, Columns<VEC>(0, 1, chunk[u]), dim, v);
     }
 }
@@ -709,10 +709,15 @@ uint32_t back_blocks_bound(uint64_t rows, uint32_t dim, int dtype) {
 template <typename T, bool VEC, int C, bool BLOCK>
 cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t &grid, cudaStream_t st) {
     const size_t shared = BLOCK || !a.partial ? 0 : (size_t)(s.threads / s.lanes) * a.dim * 4;
-    int per_sm = 1;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, VEC, C, BLOCK>, (int)s.threads, shared);
-    if (e != cudaSuccess) return e;
-    grid = back_blocks(a.rows, s, std::max(1, per_sm));
+    static std::atomic<int> known[17];  // blocks of 32 i threads that an SM holds; registers decide, not the sums' shared memory
+    int per_sm = known[s.threads / 32].load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, VEC, C, BLOCK>, (int)s.threads, shared);
+        if (e != cudaSuccess) return e;
+        per_sm = std::max(1, per_sm);
+        known[s.threads / 32].store(per_sm, std::memory_order_relaxed);
+    }
+    grid = back_blocks(a.rows, s, per_sm);
     k_norm_back<T, VEC, C, BLOCK><<<grid, s.threads, shared, st>>>(a, s.log2_lanes());
     return cudaGetLastError();
 }
@@ -779,15 +784,10 @@ extern "C" int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64
     const Divide by((uint32_t)((dim + kChunk - 1) / kChunk));
     const uint64_t chunks = rows * by.by;
     if (chunks >= (1ull << 38)) return fail(AG_ERR_VALUE, "ag_rows_dropout: too many rows of this length");  // beyond any memory
-    if (!d.on) {
-        if (x != y)
-            AG_CUDA(cudaMemcpy2DAsync(y, y_stride * elem_size(dtype), x, x_stride * elem_size(dtype), dim * elem_size(dtype), rows,
-                                      cudaMemcpyDeviceToDevice, (cudaStream_t)stream));
-        return AG_OK;
-    }
+    if (!d.on && x == y) return AG_OK;
     const uint32_t grid = (uint32_t)((chunks + 2 * kThreads - 1) / (2 * kThreads));
     const bool vec = vec_rows(x, x_stride, elem_size(dtype)) && vec_rows(y, y_stride, elem_size(dtype));
-    const bool flat = dim % kChunk && dim < kFlatMaxDim && (x_stride == dim || rows == 1) && (y_stride == dim || rows == 1) && vec_rows(x, 0, elem_size(dtype)) &&
+    const bool flat = d.on && dim % kChunk && dim < kFlatMaxDim && (x_stride == dim || rows == 1) && (y_stride == dim || rows == 1) && vec_rows(x, 0, elem_size(dtype)) &&
                       vec_rows(y, 0, elem_size(dtype));
     with_type(dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -811,6 +811,7 @@ extern "C" int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream) 
     if (n->rows == 0) return AG_OK;
     if (!n->x || (!n->y && !n->codes) || (n->codes && !n->scales)) return fail(AG_ERR_VALUE, "ag_rows_norm: null argument");
     if (n->y && n->codes) return fail(AG_ERR_VALUE, "ag_rows_norm: either rows of their own type or 8-bit rows come out");
+    if (!n->encode_only && !(n->eps >= 0.f)) return fail(AG_ERR_VALUE, "ag_rows_norm: eps must not be negative, got %g", n->eps);
     if (n->encode_only && (!n->codes || n->residual || n->weight || n->h || a.drop.on))
         return fail(AG_ERR_VALUE, "ag_rows_norm: encoding alone takes rows and gives 8-bit rows");
     if (n->codes && (n->code_stride % 16 != 0 || n->code_stride < n->dim || (uintptr_t)n->codes % 16 != 0))

@@ -76,7 +76,7 @@ def add_rms_norm_f8(x: torch.Tensor, weight: torch.Tensor | None = None, residua
 
 
 def encode_f8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """(codes, scales): rows in 8 bits.  A block's scale puts its largest magnitude on 448; a block
+    """(codes, scales): rows, of at most 16384 columns, in 8 bits.  A block's scale puts its largest magnitude on 448; a block
     that holds an infinity or NaN reads as NaN throughout."""
     return _ops.encode_f8(x)
 

@@ -63,7 +63,7 @@ def _norm(**kw):
 
 @pytest.mark.parametrize("kw,text", [
     (dict(dim=16385, y_stride=16385), "16384"), (dict(dim=0), "columns"), (dict(dtype=4), "dtype tag"), (dict(p=2.0), "probability"),
-    (dict(x=None), "null"), (dict(y=None), "null"), (dict(codes=16), "null"), (dict(codes=16, scales=16, code_stride=16), "either"),
+    (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(x_stride=1 << 32), "apart"), (dict(x=None), "null"), (dict(y=None), "null"), (dict(codes=16), "null"), (dict(codes=16, scales=16, code_stride=16), "either"),
     (dict(y=None, codes=16, scales=16, code_stride=8), "16 bytes"), (dict(y=None, codes=8, scales=16, code_stride=16), "16 bytes"),
     (dict(weight=16, dtype=1, weight_dtype=2), "weights"), (dict(encode_only=1), "encoding"), (dict(y_stride=4), "overlap"),
     (dict(h=16, h_stride=4), "overlap"), (dict(y=None, codes=16, scales=16, code_stride=16, encode_only=1, residual=16), "encoding")])

@@ -79,6 +79,43 @@ def test_dropout_layouts(ops):
     assert torch.equal(wide[:, 3:43], want) and not bool(wide[:, :3].any()) and not bool(wide[:, 43:].any())
 
 
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_dropout_pitches(ops, dtype, p):
+    """Aligned rows with a ragged end, rows that are one row, rows two gigabytes apart."""
+    x = rand(1, 30, 44, dtype=dtype)
+    want = x.double().cpu() * f.mask(30, 44, p, 8, 1)
+    wide = torch.zeros(30, 64, dtype=dtype, device="cuda")
+    wide[:, :44] = x
+    tol = (f.STEP[dtype] + 2 * U) * want.abs() + LEAST[dtype]
+    near(ops.dropout(wide[:, :44], p, 8, 1), want, tol)
+    ops.dropout_(wide[:, :44], p, 8, 1)
+    near(wide[:, :44], want, tol)
+    assert not bool(wide[:, 44:].any())
+    one = x[:1].expand(30, 44)
+    assert torch.equal(ops.dropout(one, p, 8, 1), ops.dropout(one.contiguous(), p, 8, 1))
+    far = torch.empty((3 << 30) // x.element_size(), dtype=dtype, device="cuda").as_strided((2, 44), ((3 << 29) // x.element_size(), 1))
+    far.copy_(x[:2])
+    assert torch.equal(ops.dropout(far, p, 8, 1), ops.dropout(x[:2], p, 8, 1))
+
+
+def test_changes_in_place_are_seen_by_autograd(ops):
+    x, w = rand(1, 8, 16), rand(2, 8, 16).requires_grad_()
+    y = x * w  # saves x
+    ops.dropout_(x, 0.5, 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        ops.dropout_(rand(1, 8, 16), 0.5, 1)
+
+
+def test_differentiable_once(ops):
+    x = rand(1, 8, 16).requires_grad_()
+    for out in (ops.dropout(x, 0.5, 1), ops.add_rms_norm(x)[0]):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
 def test_dropped_infinities_and_nan_are_zero(ops):
     x = torch.full((8, 64), float("inf"), device="cuda")
     x[::2] = float("nan")
@@ -408,6 +445,28 @@ def test_product_ids_outside(ops, rows):
     assert not bool(got[bad.cuda()].any()) and torch.equal(got[~bad.cuda()], good[~bad.cuda()])
 
 
+@pytest.mark.parametrize("dim", [100, 602])
+@pytest.mark.parametrize("rows", [3, 150])
+def test_product_reads_nothing_beside_its_rows(ops, rows, dim):
+    """NaN codes in the pitch's padding, NaN scales of a row that only ids outside would fall back on."""
+    a, sa, w, sw = product_case(rows, dim, 70)
+    good = ops.product_f8(a, sa, w, sw)
+    wide = [torch.full((len(t), t.stride(0) + 16), 0x7F, dtype=torch.uint8, device="cuda") for t in (a, w)]
+    for t, v in zip(wide, (a, w)):
+        t[:, :dim] = v.view(torch.uint8)
+    na, nw = (t.view(torch.float8_e4m3fn)[:, :dim] for t in wide)
+    assert torch.equal(ops.product_f8(na, sa, nw, sw), good)
+    ids = torch.arange(rows, device="cuda")
+    assert torch.equal(ops.product_f8(na, sa, nw, sw, ids=ids), good)
+    sa[0] = float("nan")
+    ids[:] = rows
+    ids[1] = 1
+    got = ops.product_f8(na, sa, nw, sw, ids=ids, bias=torch.full((70,), 3.0, device="cuda"))
+    assert bool(got[1].isfinite().all()) and not bool(got[0].any()) and not bool(got[2:].any())
+    with pytest.raises(ValueError, match="out of bounds"):
+        ops.check()
+
+
 @pytest.mark.parametrize("rows", [2, 300])
 def test_product_of_nan_rows_stays_in_them(ops, rows):
     a, sa, w, sw = product_case(rows, 300, 200)
@@ -487,6 +546,31 @@ def test_other_stream_and_captured_graph(ops):
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_two_streams_at_once(ops):
+    """Calls that overlap share nothing."""
+    x, w, res, _ = norm_case(4000, 512, torch.bfloat16, 0.1, True, torch.bfloat16)
+    dy = rand(6, 4000, 512, dtype=torch.bfloat16)
+    case = product_case(3000, 640, 384)
+
+    def work():
+        leaves = [t.detach().requires_grad_() for t in (x, w, res)]
+        y, h = ops.add_rms_norm(*leaves, p=0.1, seed=3)
+        return [y.detach(), *torch.autograd.grad((y, h), leaves, (dy, dy)), ops.product_f8(*case)]
+
+    want = work()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
 # ------------------------------------------------------------ as they are used --
 def test_layers_over_a_sampled_batch(ops):
     """Sampled batch -> projection straight from 8-bit rows -> dropout + norm -> 8-bit rows -> next store -> next product."""
@@ -518,3 +602,25 @@ def test_layers_over_a_sampled_batch(ops):
     check_product(out, codes, scales, *c2, ids=ids, dtype=torch.float32)
     with pytest.raises(ValueError):
         ag.FeatureStore.from_array(rand(1, 4, 8)).project(ids, *c2)
+
+
+@pytest.mark.parametrize("dim", [21, 64])
+def test_typed_batches_over_8_bit_rows(dim):
+    """8-bit stores beside others in the loader of a typed graph."""
+    import numpy as np
+
+    import aethergraph_b200 as ag
+
+    rng = np.random.default_rng(3)
+    e = lambda n, a, b: (rng.integers(0, a, n).astype(np.uint32), rng.integers(0, b, n).astype(np.uint32))  # noqa: E731
+    h = ag.HeteroCsrGraph.from_edge_arrays({"a": 300, "b": 200}, [("a", "to", "b", *e(3000, 300, 200)), ("b", "to", "a", *e(3000, 200, 300))])
+    stores = {"a": ag.FeatureStore.from_array(rand(1, 300, dim), "f8"), "b": ag.FeatureStore.from_array(rand(2, 200, dim), "bf16")}
+    cfg = ag.HeteroSamplingConfig({("a", "to", "b"): [4, 3], ("b", "to", "a"): [4, 3]}, seed=1)
+    loader = ag.HeteroNeighborLoader(h, cfg, "b", prefetch_depth=2, features=stores)
+    for i in range(3):
+        loader.submit(i, np.arange(i * 20, i * 20 + 20))
+    for _ in range(3):
+        _, sg = loader.next_batch()
+        for t in ("a", "b"):
+            assert torch.equal(sg.x_t(t), stores[t].gather(sg.nodes_t(t)))
+    loader.shutdown()
