@@ -314,14 +314,13 @@ struct NormArgs {
     Drop drop;
 };
 
-// Sum over the `lanes` (power of two, at most 32) of a row's group, or over the whole block.
-// AGAIN: the block calls it once more, so the sums of this time must have been read by then.
-template <bool BLOCK, bool AGAIN> __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float *shared) {
+// Sum over the `lanes` (power of two, at most 32) of a row's group, or over the whole block: through
+// `shared`, a word a warp, which the block's next call but one may use again (one barrier a call).
+template <bool BLOCK> __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float *shared) {
 #pragma unroll
     for (uint32_t o = 16; o > 0; o /= 2)
         if (BLOCK || o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (BLOCK) {
-        if (AGAIN) __syncthreads();
         if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
         __syncthreads();
         v = 0.f;
@@ -438,7 +437,7 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
         for (int j = 0; j < C; ++j)
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) sum = __ffma2_rn(v[j].p[i], v[j].p[i], sum);
-        const float rstd = rsqrtf(row_sum<BLOCK, false>(sum.x + sum.y, lanes, shared) * a.inv_dim + a.eps);
+        const float rstd = rsqrtf(row_sum<BLOCK>(sum.x + sum.y, lanes, shared) * a.inv_dim + a.eps);
         if (a.rstd && dim && (BLOCK ? threadIdx.x : lane) == 0) a.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
@@ -489,7 +488,8 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
     Chunk dw[C];
 #pragma unroll
     for (int j = 0; j < C; ++j) dw[j] = filled(0.f);
-    for (uint32_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block) {  // rows + a grid's worth fit 32 bits
+    uint32_t turn = 0;
+    for (uint32_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block, turn ^= 16) {  // rows + a grid's worth fit 32 bits
         const uint32_t row = base + (BLOCK ? 0 : threadIdx.x >> log2_lanes);
         const uint32_t dim = row < a.rows ? a.dim : 0;
         const T *h_row = (const T *)a.h + (uint64_t)row * a.h_stride, *dy_row = (const T *)a.dy + (uint64_t)row * a.dy_stride,
@@ -519,7 +519,7 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
                 sum = __ffma2_rn(gw[j].p[i], h[j].p[i], sum);
             }
         }
-        const float coef = -row_sum<BLOCK, true>(sum.x + sum.y, lanes, shared) * rstd * rstd * rstd * a.inv_dim;
+        const float coef = -row_sum<BLOCK>(sum.x + sum.y, lanes, shared + turn) * rstd * rstd * rstd * a.inv_dim;
         T *dres = (T *)a.dres + (uint64_t)row * a.dim, *dx = (T *)a.dx + (uint64_t)row * a.dim;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
