@@ -83,7 +83,7 @@ template <typename T> __device__ __forceinline__ void store_words(const Raw<T> &
 }
 
 // Which eight columns of a row a thread holds in its step j.  Aligned rows (VEC: every row starts on a
-// multiple of eight elements' bytes): a chunk, one vector load.  Others: the lanes of a group take
+// multiple of eight elements' bytes, and is whole chunks long unless RAGGED says otherwise): a chunk, one vector load.  Others: the lanes of a group take
 // consecutive columns, so that its eight loads of one element each are coalesced: the thread's
 // columns lie `stride` apart, and the group still covers whole chunks together.
 template <bool VEC> struct Columns {
@@ -96,9 +96,9 @@ template <bool VEC> struct Columns {
 };
 
 // A thread's eight columns; what lies past the row's end reads as zeros.
-template <typename T, bool VEC> __device__ __forceinline__ Raw<T> load_chunk(const T *row, const Columns<VEC> &c, uint32_t dim) {
+template <typename T, bool VEC, bool RAGGED = false> __device__ __forceinline__ Raw<T> load_chunk(const T *row, const Columns<VEC> &c, uint32_t dim) {
     Raw<T> r;
-    if (VEC && c.first + kChunk <= dim) {
+    if (VEC && (!RAGGED || c.first + kChunk <= dim)) {
         load_words(r, row + c.first);
     } else {
         T e[kChunk];
@@ -144,8 +144,8 @@ __device__ __forceinline__ Chunk filled(float f) {
     return v;
 }
 __device__ __forceinline__ float2 both(float f) { return make_float2(f, f); }
-template <typename T, bool VEC> __device__ __forceinline__ void store_chunk(T *row, const Columns<VEC> &c, uint32_t dim, const Chunk &v) {
-    if (VEC && c.first + kChunk <= dim) {
+template <typename T, bool VEC, bool RAGGED = false> __device__ __forceinline__ void store_chunk(T *row, const Columns<VEC> &c, uint32_t dim, const Chunk &v) {
+    if (VEC && (!RAGGED || c.first + kChunk <= dim)) {
         store_words(pack<T>(v), row + c.first);
     } else {
 #pragma unroll
@@ -157,7 +157,7 @@ template <typename T, bool VEC> __device__ __forceinline__ void store_chunk(T *r
 template <typename T, bool VEC> __device__ __forceinline__ Chunk load_weight(const void *w, int w_f32, const Columns<VEC> &c, uint32_t dim) {
     if (!w) return filled(1.f);
     Chunk v;
-    if (VEC && c.first + kChunk <= dim) {
+    if (VEC) {
         if (sizeof(T) == 4 || w_f32) {
             const float4 lo = __ldg((const float4 *)((const float *)w + c.first)), hi = __ldg((const float4 *)((const float *)w + c.first) + 1);
             v.p[0] = make_float2(lo.x, lo.y); v.p[1] = make_float2(lo.z, lo.w);
@@ -223,7 +223,7 @@ __device__ __forceinline__ void drop_columns(const Drop &d, uint32_t row, uint32
 constexpr int kThreads = 256;
 
 // Two chunks a thread, a block's width apart; both loads are in flight before either is used.
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool RAGGED>
 __global__ void __launch_bounds__(kThreads)
 k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_t x_stride, uint64_t y_stride, Drop d) {
     Raw<T> r[2];
@@ -233,14 +233,14 @@ k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_
     for (int u = 0; u < 2; ++u) {
         const uint64_t i = ((uint64_t)blockIdx.x * 2 + u) * kThreads + threadIdx.x;
         row[u] = chunks(i, chunk[u]);
-        if (i < total) r[u] = load_chunk<T, VEC>(x + row[u] * x_stride, Columns<VEC>(0, 1, chunk[u]), dim);
+        if (i < total) r[u] = load_chunk<T, VEC, RAGGED>(x + row[u] * x_stride, Columns<VEC>(0, 1, chunk[u]), dim);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         if (((uint64_t)blockIdx.x * 2 + u) * kThreads + threadIdx.x >= total) break;
         Chunk v = unpack(r[u]);
         if (d.on) drop_chunk(d, lots_of(d, row[u], chunk[u]), v);
-        store_chunk<T, VEC>(y + row[u] * y_stride, Columns<VEC>(0, 1, chunk[u]), dim, v);
+        store_chunk<T, VEC, RAGGED>(y + row[u] * y_stride, Columns<VEC>(0, 1, chunk[u]), dim, v);
     }
 }
 
@@ -361,7 +361,6 @@ __device__ __forceinline__ void encode_columns(const Chunk &v, const Columns<VEC
         float inv;
         const float scale = scale_of(top, inv);
         if (c.first % kF8Block == 0) scales[c.first / kF8Block] = scale;
-        // the pitch is a multiple of 16 bytes, so its padding takes what a last chunk writes past the row
         *(uint2 *)(codes + c.first) = make_uint2(code2(v.p[0], inv) | code2(v.p[1], inv) << 16, code2(v.p[2], inv) | code2(v.p[3], inv) << 16);
     } else {  // 32 lanes: columns 0 - 3 of each thread are one block, 4 - 7 the next; fewer lanes have at most one block
         uint32_t lo = 0, hi = 0;
@@ -793,8 +792,9 @@ extern "C" int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64
         using T = std::remove_pointer_t<decltype(t)>;
         if (flat) k_dropout_flat<T><<<(uint32_t)((rows * dim + kFlatElements - 1) / kFlatElements), kThreads, 0, (cudaStream_t)stream>>>(
             (const T *)x, (T *)y, rows * dim, Divide((uint32_t)dim), by, d);
-        else if (vec) k_dropout<T, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
-        else k_dropout<T, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
+        else if (vec && dim % kChunk == 0) k_dropout<T, true, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
+        else if (vec) k_dropout<T, true, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
+        else k_dropout<T, false, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
     });
     AG_CUDA(cudaGetLastError());
     return AG_OK;
@@ -825,7 +825,7 @@ extern "C" int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream) 
     a.y_stride = (uint32_t)n->y_stride; a.h_stride = (uint32_t)n->h_stride; a.code_stride = (uint32_t)n->code_stride; a.dim = (uint32_t)n->dim;
     a.w_f32 = n->weight_dtype == AG_F32; a.plain = n->encode_only; a.eps = n->eps; a.inv_dim = 1.0f / (float)n->dim;
     const uint32_t e = elem_size(n->dtype);
-    const bool vec = vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.y, a.y_stride, e) && vec_rows(a.h, a.h_stride, e);
+    const bool vec = a.dim % kChunk == 0 && vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.y, a.y_stride, e) && vec_rows(a.h, a.h_stride, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
@@ -872,7 +872,7 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
     a.rows = (uint32_t)n->rows; a.dim = (uint32_t)n->dim; a.dy_stride = (uint32_t)n->dy_stride; a.dh_stride = (uint32_t)n->dh_stride; a.h_stride = (uint32_t)n->h_stride;
     a.w_f32 = n->weight_dtype == AG_F32; a.inv_dim = 1.0f / (float)n->dim;
     const uint32_t e = elem_size(n->dtype);
-    const bool vec = vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
+    const bool vec = a.dim % kChunk == 0 && vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
                      vec_rows(a.dx, a.dim, e) && vec_rows(a.dres, a.dim, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
