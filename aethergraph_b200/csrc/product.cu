@@ -63,9 +63,12 @@ __device__ __forceinline__ void load_codes(const uint8_t *row, uint32_t c, uint3
 }
 
 constexpr int kDotThreads = 256, kDotRows = 4;
-constexpr uint64_t kFewRows = 8;
+// Beyond this the tensor-core tiles are faster: 1024 x 1024 1, 2, 4, 8 rows 3.6, 4.2, 5.3, 5.8 us this way,
+// 5.1, 5.1, 5.0, 5.2 the other; 2048 x 1024 4.8, 5.8, 7.8, 8.2 and 6.5, 6.5, 6.8, 6.8; 256 x 256 3.1, 3.2, 3.9, 3.8 and 4.0, 3.8, 3.8, 4.1.
+constexpr uint64_t kFewRows = 3;
 
-// Few rows: a warp per column of the output and up to kDotRows rows.
+// Few rows: a warp per column of the output and up to kDotRows rows, a lane 16 codes a turn, which lie in one scale
+// block.  The weights are all there is to read; 1 x 1024 x 1024: 3.6 us, of which launch and one dependent load are most.
 __global__ void __launch_bounds__(kDotThreads)
 k_product_dot(ProductArgs a) {
     const uint32_t lane = threadIdx.x & 31;
@@ -104,12 +107,16 @@ k_product_dot(ProductArgs a) {
 // A tile of 128 rows x BN output columns per turn of a persistent block, K in steps of 128 bytes,
 // which is one scale block: the tensor cores add up the 128 products of a step in f32 in TMEM, and
 // the epilogue warps fold each step into their sums in registers, times the row's and the weights'
-// scale.  Roles: warp 0 loads by TMA, and rows by id come through warps 0 and 2 with cp.async (the
-// gather form of the TMA load takes about 19 clocks a row: 25 us for 38 411 rows of 256, of them 10 waiting
-// for it), one thread each of warps 1 and 3 issues
-// tcgen05.mma (K = 32 each) and the commits, warps 4 - 11 read TMEM (a warp can reach only the 32 lanes
+// scale.  Roles: warp 0 loads by TMA, and rows by id come through warps 0 and 2 with cp.async (38 411 rows of
+// 256 by id: 25 us with the gather form of the TMA load, 20 so); one thread each of warps 1 and 3 issues
+// tcgen05.mma (K = 32 each) and the commits; warps 4 - 11 read TMEM (a warp can reach only the 32 lanes
 // of its number mod 4, so two warps share a quarter of the rows and split the columns).  Each
 // epilogue thread loads its own row's scales, four steps at a time, four steps ahead and across tiles.
+//
+// Measured: 131 072 x 2048 x 1024 to bf16 305 us (1.8 PFLOP/s, 1.1 of the measured bf16 rate of the library's
+// product; 230 us of it are the loads and multiplications alone, 32 KB a step and SM from L2, the rest
+// is TMEM reads and sums that do not hide behind them).  38 411 x 256 x 256 without ids 11.8 us, of them
+// about 4 the launch and the first tile's chain, then 1.6 us a round of 148 tiles: 4.5 TB/s.
 //
 // Every wait is bounded.  A role whose wait runs out marks the block dead and the sticky error
 // word; all roles then leave their loops, copies and multiplications in flight are waited for
@@ -149,8 +156,7 @@ __device__ __forceinline__ bool mbar_try_once(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 // Waits for the barrier's phase; false when the block is dead or the time ran out (which marks it dead).
-// The clock is looked at now and then only, and it is the SM's own: reading the global timer after
-// every failed try took longer than what is waited for.
+// The clock is looked at now and then only.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *dead) {
     if (mbar_try(bar, parity)) return true;
     const long long since = clock64();
@@ -228,7 +234,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(flo
 // What an epilogue warp holds of its tile, 32 rows x COLS columns, a row a thread, leaves through
 // shared memory, so that rows go out one beside the other in whole sectors: by TMA, which also leaves out what
 // lies past the output's edges and works while the warp goes on, where the output's rows start on 16 bytes; else
-// column by column.  16-byte piece j of a row is swizzled as the tensor map has it, which also
+// in units of eight bytes, or one by one.  16-byte piece j of a row is swizzled as the tensor map has it, which also
 // spreads neighbouring threads' pieces over the banks.
 template <typename T, int COLS>
 __device__ __forceinline__ void store_rows(const TileArgs &t, const CUtensorMap *map, uint32_t m0, uint32_t n0, const float (&acc)[COLS], bool valid,
@@ -265,11 +271,19 @@ __device__ __forceinline__ void store_rows(const TileArgs &t, const CUtensorMap 
     __syncwarp();
     const uint32_t rows = (uint32_t)min((uint64_t)32, a.rows - m0), cols = min((uint32_t)COLS, a.out_dim - n0);
     T *to = (T *)a.out + (uint64_t)m0 * a.out_stride + n0;
-    for (uint32_t r = 0; r < rows; ++r)
-        for (uint32_t c = lane; c < cols; c += 32) {
+    auto copy = [&](auto unit, uint32_t from, uint32_t end) {  // columns [from, end) of the rows, a unit a lane
+        using U = decltype(unit);
+        constexpr uint32_t kUnit = sizeof(U) / sizeof(T), kLanes = COLS / kUnit < 32 ? COLS / kUnit : 32;  // lanes a row
+        for (uint32_t c = from + lane % kLanes * kUnit; c < end; c += kLanes * kUnit) {
             const uint32_t in = c % kBoxCols;
-            to[r * a.out_stride + c] = *(const T *)(at(c / kBoxCols, r, in / kPer) + in % kPer * sizeof(T));
+            for (uint32_t r = lane / kLanes; r < rows; r += 32 / kLanes)
+                *(U *)(to + (uint64_t)r * a.out_stride + c) = *(const U *)(at(c / kBoxCols, r, in / kPer) + in % kPer * sizeof(T));
         }
+    };
+    constexpr uint32_t kPerUnit = 8 / sizeof(T);
+    const uint32_t whole = a.out_stride % kPerUnit == 0 && (uintptr_t)a.out % 8 == 0 ? cols / kPerUnit * kPerUnit : 0;
+    if (whole) copy(uint2(), 0, whole);
+    if (whole < cols) copy(T(), whole, cols);
 }
 
 // acc += scale * v for two columns at once.
@@ -560,10 +574,13 @@ int32_t launch_tile(const ProductArgs &a, cudaStream_t st) {
 }
 
 template <bool IDS, typename T> int32_t launch_tile(const ProductArgs &a, cudaStream_t st) {
-    // The widest tile that no half of is empty and that still gives every SM one.
+    // Width by the rounds of tiles that it makes and what a round costs: 1.56, 1.10 and 0.98 us for 128, 64 and 32
+    // columns at dim 256.  2000 x 512 x 512: 5.7, 4.9 and 5.8 us (1, 1 and 2 rounds); 38 411 x 256 x 256: 11.8, 13.9
+    // and 20.7 (5, 9 and 17); 20 000 x 256 x 64: 6.3, 5.5, 6.3 (2, 2, 3).
     const uint64_t m_tiles = (a.rows + kBM - 1) / kBM;
-    uint32_t bn = 128;
-    while (bn > 32 && (bn / 2 >= a.out_dim || m_tiles * ((a.out_dim + bn - 1) / bn) < (uint64_t)kSMs)) bn /= 2;
+    auto cost = [&](uint32_t width, uint32_t each) { return (m_tiles * ((a.out_dim + width - 1) / width) + kSMs - 1) / kSMs * each; };
+    const uint64_t c128 = cost(128, 156), c64 = cost(64, 110), c32 = cost(32, 98);
+    const uint32_t bn = c128 <= c64 && c128 <= c32 ? 128 : c64 <= c32 ? 64 : 32;
     if (bn == 128) return launch_tile<128, IDS, T>(a, st);
     if (bn == 64) return launch_tile<64, IDS, T>(a, st);
     return launch_tile<32, IDS, T>(a, st);
