@@ -223,8 +223,8 @@ __device__ __forceinline__ void drop_columns(const Drop &d, uint32_t row, uint32
 constexpr int kThreads = 256;
 
 // Two chunks a thread, a block's width apart; both loads are in flight before either is used.  38 411 x 256
-// bf16: 10.6 us (0.57 of the copy rate); one chunk a thread 11.6.  Bound by instructions: of about 170
-// that a chunk takes 70 are the generator's.
+// bf16: 10.6 us (0.57 of the copy rate), bound by instructions, of which the generator's ten rounds are
+// the largest part.
 template <typename T, bool VEC, bool RAGGED>
 __global__ void __launch_bounds__(kThreads)
 k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_t x_stride, uint64_t y_stride, Drop d) {
@@ -266,7 +266,7 @@ __device__ __forceinline__ uint32_t stay_bits(const uint4 &r, uint32_t not_bar) 
 // in aligned vectors of eight elements, whatever row they are in.  A block takes 1024 vectors, four a
 // thread, and makes the lots of every chunk that reaches into them (those at its ends are made by two
 // blocks): a bit per element in shared memory says whether it stays.  250 007 x 301 f16: 67 us (0.68 of the copy
-// rate; instructions: generator, bits, two atomics a chunk), a chunk a thread with loads of single
+// rate; bound by instructions: generator, bits, two atomics a chunk), a chunk a thread with loads of single
 // elements 174.  Fewer vectors a block or more resident blocks are slower (two vectors 78 us, five blocks 72).
 constexpr uint32_t kFlatVectors = 4, kFlatElements = kThreads * kFlatVectors * kChunk;
 constexpr uint64_t kFlatMaxDim = 1u << 28;  // positions within a block's rows fit 32 bits
