@@ -55,7 +55,7 @@ def _ops_command(host: str) -> list[str]:
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     return [host, "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_ops",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes),
-            os.path.join(CSRC, "ops_torch.cpp"), "-o", OPS + ".tmp", f"-L{HERE}", "-l:libaethergpu.so", f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+            os.path.join(CSRC, "ops_torch.cpp"), "-o", OPS + ".tmp", f"-L{HERE}", "-l:libaethergpu.so", f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
             "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{libs}"]
 
 

@@ -2,6 +2,7 @@
 // PyTorch's current stream and autograd around the C ABI (include/aethergpu.h).  In C++ because the
 // kernels of a small batch take less time than Python needs to make one call: a norm with its gradients
 // spends 120 us of host time written in Python, most of it in the autograd engine's thread.
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -59,7 +60,9 @@ struct Rows {
     }
 };
 
-Tensor fresh_like(const Tensor &x) { return at::empty(x.sizes(), x.options().memory_format(std::nullopt).requires_grad(false)); }
+// PyTorch's allocator without its dispatcher, which takes as long as the allocation.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) { return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt); }
+Tensor fresh_like(const Tensor &x) { return fresh(x.sizes(), x.scalar_type(), x); }
 void *stream_of(const Tensor &x) { return c10::cuda::getCurrentCUDAStream(x.get_device()).stream(); }
 bool has(const MaybeTensor &t) { return t.has_value() && t->defined(); }
 void once(const char *what) {
@@ -156,7 +159,7 @@ NormOut run_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &
         c.n.h = out.h.data_ptr(); c.n.h_stride = c.x.dim;
     }
     if (want_rstd) {
-        out.rstd = at::empty({c.x.rows}, x.options().dtype(at::kFloat).requires_grad(false));
+        out.rstd = fresh({c.x.rows}, at::kFloat, x);
         c.n.rstd = out.rstd.data_ptr<float>();
     }
     check(ag_rows_norm(&c.n, x.get_device(), stream_of(x)));
@@ -210,10 +213,12 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
         if (weight.defined()) {
             w = weight.contiguous();
             n.weight = w.data_ptr(); n.weight_dtype = tag_of(w.scalar_type());
-            if (need_w && dy) {
+            if (need_w && !dy) {  // h alone was used: the weights have no part in it
+                got[1] = at::zeros_like(w);
+            } else if (need_w) {
                 check(ag_rows_norm_backward_scratch(r.rows, r.dim, n.dtype, h.get_device(), &n.scratch_bytes));
                 got[1] = fresh_like(w);
-                scratch = at::empty({(int64_t)n.scratch_bytes}, h.options().dtype(at::kByte).requires_grad(false));
+                scratch = fresh({(int64_t)n.scratch_bytes}, at::kByte, h);
                 n.dw = got[1].data_ptr(); n.scratch = scratch.data_ptr();
             }
         }
@@ -238,10 +243,10 @@ int64_t blocks_of(int64_t n) { return (n + kF8Block - 1) / kF8Block; }
 int64_t f8_pitch(int64_t dim) { return (dim + 15) / 16 * 16; }
 Tensor empty_codes(int64_t rows, int64_t dim, const Tensor &like) {
     const int64_t pitch = f8_pitch(dim);
-    Tensor t = at::empty({rows, pitch}, like.options().dtype(at::kFloat8_e4m3fn).requires_grad(false));
+    Tensor t = fresh({rows, pitch}, at::kFloat8_e4m3fn, like);
     return pitch == dim ? t : t.narrow(1, 0, dim);
 }
-Tensor empty_scales(int64_t rows, int64_t dim, const Tensor &like) { return at::empty({rows, blocks_of(dim)}, like.options().dtype(at::kFloat).requires_grad(false)); }
+Tensor empty_scales(int64_t rows, int64_t dim, const Tensor &like) { return fresh({rows, blocks_of(dim)}, at::kFloat, like); }
 
 std::pair<Tensor, Tensor> to_f8(NormCall &c, const Tensor &x) {
     Tensor codes = empty_codes(c.x.rows, c.x.dim, x), scales = empty_scales(c.x.rows, c.x.dim, x);
@@ -320,7 +325,7 @@ Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scal
         no_gradient("a product of 8-bit rows", {&*bias});
         p.bias = bias->data_ptr<float>();
     }
-    Tensor out = at::empty({(int64_t)p.rows, out_dim}, weight.options().dtype(dtype).requires_grad(false));
+    Tensor out = fresh({(int64_t)p.rows, out_dim}, dtype, weight);
     p.out = out.data_ptr();
     if (p.rows) check(ag_rows_product(&p, held.device, stream_of(weight)));
     return out;
