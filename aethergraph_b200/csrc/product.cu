@@ -357,6 +357,7 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         for (uint32_t tile = blockIdx.x; tile < tiles && alive; tile += gridDim.x) {
             const uint32_t m0 = tile / t.n_tiles * kBM, n0 = tile % t.n_tiles * BN;
             uint32_t *mine = row_ids + first;
+            const uint8_t *rows[16];  // rows lane / 8, lane / 8 + 4, ... of this warp's half
             if (IDS) {  // rows without one, and ids outside, load row 0: the epilogue leaves its zeros
                 __syncwarp();
 #pragma unroll
@@ -366,6 +367,8 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 }
                 __syncwarp();
                 load_ids(tile + gridDim.x);  // a tile ahead
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) rows[i] = a.codes + (uint64_t)mine[lane / 8 + i * 4] * (uint32_t)a.code_stride;
             }
             for (uint32_t k = 0; k < steps; ++k, ++issued) {
                 const uint32_t s = issued % kStages;
@@ -378,14 +381,12 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     tma_tile(at + kBM * kBK, &map_w, full + 8 * s, k * kBK, n0);
                 }
                 if (IDS) {  // eight lanes a row, 16 bytes each, swizzled as the tensor maps do; zeros past the row's end
-                    const uint32_t c = k * kBK + piece * 16, bytes = c < a.dim ? min(a.dim - c, 16u) : 0;
-                    const uint8_t *from = a.codes + (bytes ? c : 0);
+                    const uint32_t c = k * kBK + piece * 16, bytes = c < a.dim ? min(a.dim - c, 16u) : 0, from = bytes ? c : 0;
+                    const uint32_t even = at + (first + lane / 8) * kBK + ((piece ^ (lane / 8)) * 16), odd = even ^ 64;  // rows 4 apart
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; ++i) {
-                        const uint32_t r = lane / 8 + i * 4;
+                    for (uint32_t i = 0; i < 16; ++i)
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                                     :: "r"(at + (first + r) * kBK + ((piece ^ (r % 8)) * 16)), "l"(from + (uint64_t)mine[r] * a.code_stride), "r"(bytes) : "memory");
-                    }
+                                     :: "r"((i & 1 ? odd : even) + i * 4 * kBK), "l"(rows[i] + from), "r"(bytes) : "memory");
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     if (issued - landed >= kStages - 2) {
                         asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 2) : "memory");
@@ -599,7 +600,7 @@ using namespace ag;
 extern "C" int32_t ag_rows_product(const ag_product *p, int32_t device, void *stream) {
     if (!p) return fail(AG_ERR_VALUE, "ag_rows_product: null argument");
     if (p->out_dtype < AG_F32 || p->out_dtype > AG_BF16) return fail(AG_ERR_VALUE, "ag_rows_product: the output is f32, f16 or bf16, got dtype tag %d", p->out_dtype);
-    if (p->dim == 0 || p->dim > 0x7FFFFF00ull || p->out_dim == 0 || p->out_dim >= (1ull << 31) || p->held >= (1ull << 31) || p->rows >= (1ull << 31))
+    if (p->dim == 0 || p->dim > 0x7FFFFF00ull || p->code_stride > 0xFFFFFFF0ull || p->out_dim == 0 || p->out_dim >= (1ull << 31) || p->held >= (1ull << 31) || p->rows >= (1ull << 31))
         return fail(AG_ERR_VALUE, "ag_rows_product: %llu rows of %llu x %llu from %llu held rows are out of range", (unsigned long long)p->rows,
                     (unsigned long long)p->dim, (unsigned long long)p->out_dim, (unsigned long long)p->held);
     if (p->rows == 0) return AG_OK;
