@@ -379,6 +379,7 @@ cudaError_t launch_i8(const GatherArgs &a, const GatherArgs *group, uint32_t row
 // columns; value = code * scale, one multiplication, as ops.product_f8 reads them.  The lanes of a
 // row take its 4-byte words in turn, as above, for loads and 16-byte stores that lie side by side.
 // VEC: output rows start on 16 bytes; else the four floats of a word are stored one by one.
+// 300 000 rows by id of 2 M, 256 columns: 71 us (int8 81, bf16 100); 100 columns 41 (43, 43), 301 columns 164 (193, 197).
 template <int LPR, bool VEC>
 __global__ void __launch_bounds__(kThreads)
 k_gather_f8(GatherArgs a, const GatherArgs *group) {

@@ -585,6 +585,7 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
 template <typename T, uint32_t kDwCols>
 __global__ void __launch_bounds__(1024)
 k_norm_dw(const float *partial, uint32_t blocks, uint32_t dim, T *dw) {
+    chain_sync();  // launched as a programmatic dependent of k_norm_back
     constexpr uint32_t kDwSlices = 1024 / kDwCols;
     __shared__ float sums[kDwSlices][kDwCols + 1];
     const uint32_t c = blockIdx.x * kDwCols + threadIdx.x;
@@ -911,8 +912,8 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
             using T = std::remove_pointer_t<decltype(t)>;
             const float *partial = (const float *)n->scratch;
             const uint32_t dim = (uint32_t)n->dim;
-            if (dim <= (uint32_t)kSMs * 8) k_norm_dw<T, 8><<<(dim + 7) / 8, dim3(8, 128), 0, (cudaStream_t)stream>>>(partial, grid, dim, (T *)n->dw);
-            else k_norm_dw<T, 32><<<(dim + 31) / 32, dim3(32, 32), 0, (cudaStream_t)stream>>>(partial, grid, dim, (T *)n->dw);
+            if (dim <= (uint32_t)kSMs * 8) launch_chained(k_norm_dw<T, 8>, dim3((dim + 7) / 8), dim3(8, 128), (cudaStream_t)stream, partial, grid, dim, (T *)n->dw);
+            else launch_chained(k_norm_dw<T, 32>, dim3((dim + 31) / 32), dim3(32, 32), (cudaStream_t)stream, partial, grid, dim, (T *)n->dw);
         });
     AG_CUDA(cudaGetLastError());
     return AG_OK;
