@@ -93,6 +93,7 @@ template <bool VEC> struct Columns {
         first = VEC ? (step_chunk + lane) * kChunk : step_chunk * kChunk + lane;
     }
     __device__ __forceinline__ uint32_t at(uint32_t i) const { return first + i * stride; }
+    __device__ __forceinline__ bool whole(uint32_t dim) const { return at(kChunk - 1) < dim; }  // one test for eight single elements
 };
 
 // A thread's eight columns; what lies past the row's end reads as zeros.
@@ -102,8 +103,14 @@ template <typename T, bool VEC, bool RAGGED = false> __device__ __forceinline__ 
         load_words(r, row + c.first);
     } else {
         T e[kChunk];
+        const T *at = row + c.first;
+        if (c.whole(dim)) {
 #pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i) e[i] = c.at(i) < dim ? row[c.at(i)] : from_f32<T>(0.f);
+            for (uint32_t i = 0; i < kChunk; ++i) e[i] = at[i * c.stride];
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i) e[i] = c.at(i) < dim ? at[i * c.stride] : from_f32<T>(0.f);
+        }
         memcpy(&r, e, sizeof r);
     }
     return r;
@@ -148,9 +155,18 @@ template <typename T, bool VEC, bool RAGGED = false> __device__ __forceinline__ 
     if (VEC && (!RAGGED || c.first + kChunk <= dim)) {
         store_words(pack<T>(v), row + c.first);
     } else {
+        T *to = row + c.first;
+        const Raw<T> r = pack<T>(v);
+        T e[kChunk];
+        memcpy(e, &r, sizeof r);
+        if (c.whole(dim)) {
 #pragma unroll
-        for (uint32_t i = 0; i < kChunk; ++i)
-            if (c.at(i) < dim) row[c.at(i)] = from_f32<T>(at(v, i));
+            for (uint32_t i = 0; i < kChunk; ++i) to[i * c.stride] = e[i];
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk; ++i)
+                if (c.at(i) < dim) to[i * c.stride] = e[i];
+        }
     }
 }
 // The norm's weights, of the rows' type or f32: the same few for every row (L1).
@@ -171,7 +187,7 @@ template <typename T, bool VEC> __device__ __forceinline__ Chunk load_weight(con
     } else {
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
-            at(v, i) = c.at(i) >= dim ? 0.f : sizeof(T) == 4 || w_f32 ? __ldg((const float *)w + c.at(i)) : to_f32(((const T *)w)[c.at(i)]);
+            at(v, i) = c.at(i) >= dim ? 0.f : sizeof(T) == 4 || w_f32 ? __ldg((const float *)w + c.first + i * c.stride) : to_f32(((const T *)w + c.first)[i * c.stride]);
     }
     return v;
 }
@@ -408,10 +424,11 @@ __device__ __forceinline__ void encode_columns(const Chunk &v, const Columns<VEC
 // through once.  524 288 x 512 bf16 with residual to 8 bits: 288 us, the measured copy rate; 16 384 x 4096
 // f16: 50 us (0.83); 38 411 x 256 bf16 with residual and dropout: 17 us (0.70, instructions); 20 011 x 602 f32,
 // not aligned, the same: 32 us (0.93).
-template <typename T, bool VEC, int C, bool BLOCK, bool F8>
+// L: the lanes of a row where they are known (rows that are not aligned: their strides are then constants), else 0.
+template <typename T, bool VEC, int C, bool BLOCK, bool F8, int L>
 __global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? (sizeof(T) * C <= 8 ? 2 : 1) : C == 1 ? 5 : 4)
 k_norm(const NormArgs a, uint32_t log2_lanes) {
-    const uint32_t lanes = C > 1 || BLOCK ? 32 : 1u << log2_lanes;  // more chunks than one: all lanes
+    const uint32_t lanes = C > 1 || BLOCK ? 32 : L ? L : 1u << log2_lanes;  // more chunks than one: all lanes
     __shared__ float shared[32];
     __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
     uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
@@ -500,10 +517,10 @@ struct NormBackArgs {
 // 16 384 x 4096 f16: 102 us (0.80 of the copy rate), 38 411 x 256 bf16 20 us (0.75), 20 011 x 602 f32 42 us (0.88).
 // Bound by instructions with 16 to 32 warps an SM: bringing the next row into shared memory meanwhile (cp.async) made
 // it slower (139 us where this took 122), leaving the ragged path out of the aligned kernel faster (122 to 102).
-template <typename T, bool VEC, int C, bool BLOCK>
+template <typename T, bool VEC, int C, bool BLOCK, int L>
 __global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? (C == 1 ? 2 : 1) : C == 1 ? 4 : 2)
 k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
-    const uint32_t lanes = C > 1 || BLOCK ? 32 : 1u << log2_lanes;
+    const uint32_t lanes = C > 1 || BLOCK ? 32 : L ? L : 1u << log2_lanes;
     __shared__ float shared[32];
     __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
     extern __shared__ float sums[];  // [groups of the block][dim], not BLOCK
@@ -676,22 +693,23 @@ int32_t check_pitches(const char *who, std::initializer_list<uint64_t> pitches) 
 // `chunks` chunks each.  Whole blocks: as few threads as hold the row in
 // `most` chunks each (64 bytes of f16 / bf16 or f32: a thread's loads are all in flight together, and the sum
 // waits for fewer warps), unless that leaves many of them idle; a chunk each where there are no more rows than
-// SMs, and the time is one row's latency.  16 384 rows of 4096 f16, forward: four chunks 52 us, two 64, one 66.
+// SMs, and the time is one row's latency, and in the backward pass over rows that are not aligned (registers).  16 384 rows of 4096 f16, forward: four chunks 52 us, two 64, one 66.
 struct Split {
     uint32_t lanes, threads;
     int chunks;
     uint32_t log2_lanes() const { uint32_t l = 0; while ((1u << l) < lanes) ++l; return lanes ? l : 5; }
 };
-Split split_row(uint64_t rows, uint32_t dim, int dtype) {
+Split split_row(uint64_t rows, uint32_t dim, int dtype, bool vec, bool backward) {
     const uint32_t n = (dim + kChunk - 1) / kChunk;
     Split s{1, kThreads, 1};
-    if (n <= 64) {
+    if (!vec) s.lanes = 4;
+    if (n <= (!vec && backward ? 32u : 64u)) {
         while (s.lanes < 32 && s.lanes < n) s.lanes *= 2;
         while ((uint32_t)s.chunks * s.lanes < n) s.chunks *= 2;
         return s;
     }
     s.lanes = 0;
-    const int most = rows <= (uint64_t)kSMs ? 1 : dtype == AG_F32 ? 2 : 4;
+    const int most = rows <= (uint64_t)kSMs || (!vec && backward) ? 1 : dtype == AG_F32 ? 2 : 4;
     uint32_t slots = 0xFFFFFFFFu;
     for (int c = most; c; c /= 2) {
         const uint32_t threads = (n + 32 * c - 1) / (32 * c) * 32;
@@ -705,18 +723,26 @@ Split split_row(uint64_t rows, uint32_t dim, int dtype) {
     return s;
 }
 
+// f(std::integral_constant<int, L>) for the lanes of a row that is not aligned; 0 for others.
+template <bool VEC, typename F> auto with_lanes(uint32_t lanes, F f) {
+    if constexpr (VEC) return f(std::integral_constant<int, 0>{});
+    else return lanes == 4 ? f(std::integral_constant<int, 4>{}) : lanes == 8 ? f(std::integral_constant<int, 8>{}) :
+                lanes == 16 ? f(std::integral_constant<int, 16>{}) : f(std::integral_constant<int, 32>{});
+}
+
 template <typename T, bool VEC, bool F8>
 cudaError_t launch_norm(const NormArgs &a, int dtype, cudaStream_t st) {
-    const Split s = split_row(a.rows, a.dim, dtype);
+    const Split s = split_row(a.rows, a.dim, dtype, VEC, false);
     const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
-    const uint32_t grid = (uint32_t)((a.rows + per - 1) / per), lanes = s.log2_lanes();  // rows of a whole block are 2 KB and more
+    const uint32_t grid = (uint32_t)((a.rows + per - 1) / per), lanes = s.log2_lanes();  // rows of a whole block are 1 KB and more
     if (s.lanes) {
-        if (s.chunks == 1) k_norm<T, VEC, 1, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
-        else k_norm<T, VEC, 2, false, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+        if (s.chunks == 1)
+            with_lanes<VEC>(s.lanes, [&](auto l) { k_norm<T, VEC, 1, false, F8, decltype(l)::value><<<grid, s.threads, 0, st>>>(a, lanes); });
+        else k_norm<T, VEC, 2, false, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
     } else {
-        if (s.chunks == 1) k_norm<T, VEC, 1, true, F8><<<grid, s.threads, 0, st>>>(a, lanes);
-        else if (s.chunks == 2) k_norm<T, VEC, 2, true, F8><<<grid, s.threads, 0, st>>>(a, lanes);
-        else k_norm<T, VEC, 4, true, F8><<<grid, s.threads, 0, st>>>(a, lanes);
+        if (s.chunks == 1) k_norm<T, VEC, 1, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
+        else if (s.chunks == 2) k_norm<T, VEC, 2, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
+        else k_norm<T, VEC, 4, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
     }
     return cudaGetLastError();
 }
@@ -728,31 +754,35 @@ uint32_t back_blocks(uint64_t rows, const Split &s, uint32_t per_sm) {
     return (uint32_t)std::min<uint64_t>((rows + per - 1) / per, (uint64_t)kSMs * per_sm);
 }
 uint32_t back_blocks_bound(uint64_t rows, uint32_t dim, int dtype) {
-    const Split s = split_row(rows, dim, dtype);
-    return back_blocks(rows, s, std::min(2048 / s.threads, 32u));
+    uint32_t most = 0;
+    for (const bool vec : {false, true}) {
+        const Split s = split_row(rows, dim, dtype, vec, true);
+        most = std::max(most, back_blocks(rows, s, std::min(2048 / s.threads, 32u)));
+    }
+    return most;
 }
 
-template <typename T, bool VEC, int C, bool BLOCK>
+template <typename T, bool VEC, int C, bool BLOCK, int L = 0>
 cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t &grid, cudaStream_t st) {
     const size_t shared = BLOCK || !a.partial ? 0 : (size_t)(s.threads / s.lanes) * a.dim * 4;
     static std::atomic<int> known[17];  // blocks of 32 i threads that an SM holds; registers decide, not the sums' shared memory
     int per_sm = known[s.threads / 32].load(std::memory_order_relaxed);
     if (per_sm == 0) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, VEC, C, BLOCK>, (int)s.threads, shared);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, VEC, C, BLOCK, L>, (int)s.threads, shared);
         if (e != cudaSuccess) return e;
         per_sm = std::max(1, per_sm);
         known[s.threads / 32].store(per_sm, std::memory_order_relaxed);
     }
     grid = back_blocks(a.rows, s, per_sm);
-    k_norm_back<T, VEC, C, BLOCK><<<grid, s.threads, shared, st>>>(a, s.log2_lanes());
+    k_norm_back<T, VEC, C, BLOCK, L><<<grid, s.threads, shared, st>>>(a, s.log2_lanes());
     return cudaGetLastError();
 }
 
 template <typename T, bool VEC>
 cudaError_t launch_back(const NormBackArgs &a, int dtype, uint32_t &grid, cudaStream_t st) {
-    const Split s = split_row(a.rows, a.dim, dtype);
+    const Split s = split_row(a.rows, a.dim, dtype, VEC, true);
     if (s.lanes) {
-        if (s.chunks == 1) return launch_back<T, VEC, 1, false>(a, s, grid, st);
+        if (s.chunks == 1) return with_lanes<VEC>(s.lanes, [&](auto l) { return launch_back<T, VEC, 1, false, decltype(l)::value>(a, s, grid, st); });
         return launch_back<T, VEC, 2, false>(a, s, grid, st);
     }
     if (s.chunks == 1) return launch_back<T, VEC, 1, true>(a, s, grid, st);
