@@ -114,8 +114,9 @@ k_product_dot(ProductArgs a) {
 // epilogue thread loads its own row's scales, four steps at a time, four steps ahead and across tiles.
 //
 // Measured: 131 072 x 2048 x 1024 to bf16 305 us (1.8 PFLOP/s, 1.1 of the measured bf16 rate of the library's
-// product; 230 us of it are the loads and multiplications alone, 32 KB a step and SM from L2, the rest
-// is TMEM reads and sums that do not hide behind them).  38 411 x 256 x 256 without ids 11.8 us, of them
+// product).  Without the epilogue's work 230 us: a step's 32 KB pass through shared memory twice, on their
+// way in and as operands, 512 clocks at 128 bytes where its multiplications take 256.  The rest is
+// TMEM reads and sums that do not hide behind them.  38 411 x 256 x 256 without ids 11.8 us, of them
 // about 4 the launch and the first tile's chain, then 1.6 us a round of 148 tiles: 4.5 TB/s.
 //
 // Every wait is bounded.  A role whose wait runs out marks the block dead and the sticky error
@@ -470,7 +471,13 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             float weight = lane < steps ? __ldg(weights + lane) : 0.f;  // 32 steps' in the lanes
             id = id_at(tile + gridDim.x);
             float acc[kHalf];
-            if (a.bias) {  // the sums start from it; one branch here, not one for each value where they are stored
+            if (a.bias && n0 + kHalf <= a.out_dim && (uintptr_t)a.bias % 16 == 0) {  // the sums start from it: one branch here, not one for each value that is stored
+#pragma unroll
+                for (int i = 0; i < kHalf; i += 4) {
+                    const float4 f = __ldg((const float4 *)(a.bias + n0 + i));
+                    acc[i] = f.x; acc[i + 1] = f.y; acc[i + 2] = f.z; acc[i + 3] = f.w;
+                }
+            } else if (a.bias) {
 #pragma unroll
                 for (int i = 0; i < kHalf; ++i) acc[i] = n0 + i < a.out_dim ? __ldg(a.bias + n0 + i) : 0.f;
             } else {

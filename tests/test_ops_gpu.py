@@ -485,6 +485,14 @@ def test_product_of_slices(ops, rows):
     check_product(got, a[5:5 + rows, 128:320].contiguous(), sa[5:5 + rows, 1:3], w[128:330, 128:320].contiguous(), sw[1:3, 1:3])
 
 
+@pytest.mark.parametrize("out", [96, 128, 200])
+def test_product_bias_anywhere(ops, out):
+    case = product_case(140, 256, out)
+    many = rand(5, out + 1)
+    for bias in (many[:out].contiguous(), many[1:]):
+        check_product(ops.product_f8(*case, bias=bias, dtype=torch.float32), *case, bias=bias, dtype=torch.float32)
+
+
 def test_refusals(ops):
     a, sa, w, sw = product_case(8, 64, 16)
     x = rand(1, 8, 64)
