@@ -82,25 +82,35 @@ template <typename T> __device__ __forceinline__ void store_words(const Raw<T> &
     asm volatile("st.global.v4.b32 [%0], {%1,%2,%3,%4};" :: "l"(p), "r"(r.w[0]), "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]) : "memory");
 }
 
-// Which eight columns of a row a thread holds in its step j.  Aligned rows (VEC: every row starts on a
-// multiple of eight elements' bytes, and is whole chunks long unless RAGGED says otherwise): a chunk, one vector load.  Others: the lanes of a group take
-// consecutive columns, so that its eight loads of one element each are coalesced: the thread's
-// columns lie `stride` apart, and the group still covers whole chunks together.
-template <bool VEC> struct Columns {
-    uint32_t first, stride;
+// Which eight columns of a row a thread holds in its step j.  Whole chunks where every row starts on a
+// multiple of eight elements' bytes and is so many chunks long (or RAGGED says otherwise): one vector load.  Elsewhere the
+// lanes of a group take neighbouring columns, so that a group's loads are coalesced and it still covers whole
+// chunks together: pairs of 16-bit elements where rows start on four bytes and are even, else single elements.
+constexpr int kSingle = 0, kWhole = 1, kPair = 2;
+template <int MODE> struct Columns {
+    uint32_t first, stride;  // stride: from one of its loads to the next, in units
     __device__ __forceinline__ Columns(uint32_t lane, uint32_t lanes, uint32_t step_chunk) {  // lanes: of the group, at most 32
-        stride = VEC ? 1 : lanes;
-        first = VEC ? (step_chunk + lane) * kChunk : step_chunk * kChunk + lane;
+        stride = MODE == kWhole ? 1 : lanes;
+        first = MODE == kWhole ? (step_chunk + lane) * kChunk : step_chunk * kChunk + (MODE == kPair ? 2 * lane : lane);
     }
-    __device__ __forceinline__ uint32_t at(uint32_t i) const { return first + i * stride; }
-    __device__ __forceinline__ bool whole(uint32_t dim) const { return at(kChunk - 1) < dim; }  // one test for eight single elements
+    __device__ __forceinline__ uint32_t at(uint32_t i) const { return MODE == kPair ? first + i / 2 * 2 * stride + i % 2 : first + i * stride; }
+    __device__ __forceinline__ bool whole(uint32_t dim) const { return at(kChunk - 1) < dim; }  // one test for all of them
 };
 
 // A thread's eight columns; what lies past the row's end reads as zeros.
-template <typename T, bool VEC, bool RAGGED = false> __device__ __forceinline__ Raw<T> load_chunk(const T *row, const Columns<VEC> &c, uint32_t dim) {
+template <typename T, int MODE, bool RAGGED = false> __device__ __forceinline__ Raw<T> load_chunk(const T *row, const Columns<MODE> &c, uint32_t dim) {
     Raw<T> r;
-    if (VEC && (!RAGGED || c.first + kChunk <= dim)) {
+    if (MODE == kWhole && (!RAGGED || c.first + kChunk <= dim)) {
         load_words(r, row + c.first);
+    } else if constexpr (MODE == kPair) {
+        const uint32_t *at = (const uint32_t *)(row + c.first);
+        if (c.whole(dim)) {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk / 2; ++i) r.w[i] = at[i * c.stride];
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk / 2; ++i) r.w[i] = c.at(2 * i) < dim ? at[i * c.stride] : 0u;
+        }
     } else {
         T e[kChunk];
         const T *at = row + c.first;
@@ -151,9 +161,20 @@ __device__ __forceinline__ Chunk filled(float f) {
     return v;
 }
 __device__ __forceinline__ float2 both(float f) { return make_float2(f, f); }
-template <typename T, bool VEC, bool RAGGED = false> __device__ __forceinline__ void store_chunk(T *row, const Columns<VEC> &c, uint32_t dim, const Chunk &v) {
-    if (VEC && (!RAGGED || c.first + kChunk <= dim)) {
+template <typename T, int MODE, bool RAGGED = false> __device__ __forceinline__ void store_chunk(T *row, const Columns<MODE> &c, uint32_t dim, const Chunk &v) {
+    if (MODE == kWhole && (!RAGGED || c.first + kChunk <= dim)) {
         store_words(pack<T>(v), row + c.first);
+    } else if constexpr (MODE == kPair) {
+        uint32_t *to = (uint32_t *)(row + c.first);
+        const Raw<T> r = pack<T>(v);
+        if (c.whole(dim)) {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk / 2; ++i) to[i * c.stride] = r.w[i];
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk / 2; ++i)
+                if (c.at(2 * i) < dim) to[i * c.stride] = r.w[i];
+        }
     } else {
         T *to = row + c.first;
         const Raw<T> r = pack<T>(v);
@@ -170,10 +191,10 @@ template <typename T, bool VEC, bool RAGGED = false> __device__ __forceinline__ 
     }
 }
 // The norm's weights, of the rows' type or f32: the same few for every row (L1).
-template <typename T, bool VEC> __device__ __forceinline__ Chunk load_weight(const void *w, int w_f32, const Columns<VEC> &c, uint32_t dim) {
+template <typename T, int MODE> __device__ __forceinline__ Chunk load_weight(const void *w, int w_f32, const Columns<MODE> &c, uint32_t dim) {
     if (!w) return filled(1.f);
     Chunk v;
-    if (VEC) {
+    if (MODE == kWhole) {
         if (sizeof(T) == 4 || w_f32) {
             const float4 lo = __ldg((const float4 *)((const float *)w + c.first)), hi = __ldg((const float4 *)((const float *)w + c.first) + 1);
             v.p[0] = make_float2(lo.x, lo.y); v.p[1] = make_float2(lo.z, lo.w);
@@ -183,6 +204,13 @@ template <typename T, bool VEC> __device__ __forceinline__ Chunk load_weight(con
             Raw<T> r;
             r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
             v = unpack(r);
+        }
+    } else if constexpr (MODE == kPair) {
+#pragma unroll
+        for (uint32_t i = 0; i < kChunk / 2; ++i) {
+            if (c.at(2 * i) >= dim) v.p[i] = both(0.f);
+            else if (w_f32) v.p[i] = __ldg((const float2 *)((const float *)w + c.first) + i * c.stride);
+            else v.p[i] = pair_f32(T(), __ldg((const uint32_t *)((const T *)w + c.first) + i * c.stride));
         }
     } else {
 #pragma unroll
@@ -221,16 +249,25 @@ __device__ __forceinline__ void drop_chunk(const Drop &d, const uint4 &lots, Chu
 
 // Dropout of a thread's eight columns.  Unless they are a chunk, the group's lanes make the lots of one
 // chunk each and pass them around in shared memory (16 bytes a lane); the whole warp calls this.
-template <bool VEC>
+template <int MODE>
 __device__ __forceinline__ void drop_columns(const Drop &d, uint32_t row, uint32_t lane, uint32_t lanes, uint32_t step_chunk, uint4 *warp_lots, Chunk &v) {
     const uint4 r = lots_of(d, row, step_chunk + lane);
-    if (VEC) {
+    if (MODE == kWhole) {
         drop_chunk(d, r, v);
     } else {
         __syncwarp();
         warp_lots[threadIdx.x & 31] = r;
         __syncwarp();
         const uint16_t *group = (const uint16_t *)(warp_lots + ((threadIdx.x & 31) - lane));
+        if constexpr (MODE == kPair) {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk / 2; ++i) {  // the lots of two neighbours are a word, as in a chunk
+                const uint32_t u = ((const uint32_t *)group)[lane + i * lanes];
+                const float2 f = __fmul2_rn(v.p[i], both(d.scale));
+                v.p[i] = make_float2(kept(d, u << 16, f.x), kept(d, u, f.y));
+            }
+            return;
+        }
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i) at(v, i) = kept(d, (uint32_t)group[lane + i * lanes] << 16, at(v, i) * d.scale);
     }
@@ -241,7 +278,7 @@ constexpr int kThreads = 256;
 // Two chunks a thread, a block's width apart; both loads are in flight before either is used.  38 411 x 256
 // bf16: 10.6 us (0.57 of the copy rate), bound by instructions, of which the generator's ten rounds are
 // the largest part.
-template <typename T, bool VEC, bool RAGGED>
+template <typename T, int MODE, bool RAGGED>
 __global__ void __launch_bounds__(kThreads)
 k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_t x_stride, uint64_t y_stride, Drop d) {
     Raw<T> r[2];
@@ -251,14 +288,14 @@ k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_
     for (int u = 0; u < 2; ++u) {
         const uint64_t i = ((uint64_t)blockIdx.x * 2 + u) * kThreads + threadIdx.x;
         row[u] = chunks(i, chunk[u]);
-        if (i < total) r[u] = load_chunk<T, VEC, RAGGED>(x + row[u] * x_stride, Columns<VEC>(0, 1, chunk[u]), dim);
+        if (i < total) r[u] = load_chunk<T, MODE, RAGGED>(x + row[u] * x_stride, Columns<MODE>(0, 1, chunk[u]), dim);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         if (((uint64_t)blockIdx.x * 2 + u) * kThreads + threadIdx.x >= total) break;
         Chunk v = unpack(r[u]);
         if (d.on) drop_chunk(d, lots_of(d, row[u], chunk[u]), v);
-        store_chunk<T, VEC, RAGGED>(y + row[u] * y_stride, Columns<VEC>(0, 1, chunk[u]), dim, v);
+        store_chunk<T, MODE, RAGGED>(y + row[u] * y_stride, Columns<MODE>(0, 1, chunk[u]), dim, v);
     }
 }
 
@@ -382,9 +419,9 @@ __device__ __forceinline__ uint32_t code2(float2 v, float inv) {
 }
 
 // e4m3 codes and scales of a group's step; the whole warp calls this.
-template <bool VEC>
-__device__ __forceinline__ void encode_columns(const Chunk &v, const Columns<VEC> &c, uint32_t lane, uint32_t lanes, uint32_t dim, uint8_t *codes, float *scales) {
-    if (VEC) {  // the 16 lanes of a block reduce; a chunk lies in one block
+template <int MODE>
+__device__ __forceinline__ void encode_columns(const Chunk &v, const Columns<MODE> &c, uint32_t lane, uint32_t lanes, uint32_t dim, uint8_t *codes, float *scales) {
+    if (MODE == kWhole) {  // the 16 lanes of a block reduce; a chunk lies in one block
         uint32_t top = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i) top = max(top, magnitude(at(v, i)));
@@ -413,6 +450,12 @@ __device__ __forceinline__ void encode_columns(const Chunk &v, const Columns<VEC
             if (c.first < dim) scales[c.first / kF8Block] = scale_lo;
             if (lanes == 32 && c.first + kF8Block < dim) scales[c.first / kF8Block + 1] = scale_hi;
         }
+        if constexpr (MODE == kPair) {
+#pragma unroll
+            for (uint32_t i = 0; i < kChunk / 2; ++i)
+                if (c.at(2 * i) < dim) *(uint16_t *)(codes + c.at(2 * i)) = (uint16_t)code2(v.p[i], i < kChunk / 4 ? inv_lo : inv_hi);
+            return;
+        }
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
             if (c.at(i) < dim) codes[c.at(i)] = (uint8_t)code2(make_float2(at(v, i), 0.f), i < kChunk / 2 ? inv_lo : inv_hi);
@@ -423,15 +466,16 @@ __device__ __forceinline__ void encode_columns(const Chunk &v, const Columns<VEC
 // block), C chunks each; the row stays in registers between the sum and the output, so memory is gone
 // through once.  524 288 x 512 bf16 with residual to 8 bits: 288 us, the measured copy rate; 16 384 x 4096
 // f16: 50 us (0.83); 38 411 x 256 bf16 with residual and dropout: 17 us (0.70, instructions); 20 011 x 602 f32,
-// not aligned, the same: 32 us (0.93).
+// not aligned, the same: 32 us (0.93).  16-bit rows that are not aligned are bound by instructions: 300 000 x 100
+// bf16 with residual to 8 bits 60 us in pairs (0.54), 77 in single elements.
 // L: the lanes of a row where they are known (rows that are not aligned: their strides are then constants), else 0.
-template <typename T, bool VEC, int C, bool BLOCK, bool F8, int L>
+template <typename T, int MODE, int C, bool BLOCK, bool F8, int L>
 __global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? (sizeof(T) * C <= 8 ? 2 : 1) : C == 1 ? 5 : 4)
 k_norm(const NormArgs a, uint32_t log2_lanes) {
     const uint32_t lanes = C > 1 || BLOCK ? 32 : L ? L : 1u << log2_lanes;  // more chunks than one: all lanes
     __shared__ float shared[32];
-    __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
-    uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
+    __shared__ uint4 lots[MODE == kWhole ? 1 : BLOCK ? 512 : kThreads];
+    uint4 *warp_lots = MODE == kWhole ? lots : lots + (threadIdx.x & ~31u);
     const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
     const uint32_t row = BLOCK ? blockIdx.x : blockIdx.x * (kThreads >> log2_lanes) + (threadIdx.x >> log2_lanes);
     const uint32_t dim = row < a.rows ? a.dim : 0;  // lanes without a row still take part in the exchanges
@@ -441,18 +485,18 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
         Raw<T> rx[C], rr[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+            const Columns<MODE> c(lane, lanes, j * width + group_chunk);
             if (c.first >= dim) continue;
-            rx[j] = load_chunk<T, VEC>(x, c, dim);
-            if (a.res) rr[j] = load_chunk<T, VEC>(res, c, dim);
-            if (C == 1) w[j] = load_weight<T, VEC>(a.weight, a.w_f32, c, dim);  // early, where it costs few registers
+            rx[j] = load_chunk<T, MODE>(x, c, dim);
+            if (a.res) rr[j] = load_chunk<T, MODE>(res, c, dim);
+            if (C == 1) w[j] = load_weight<T, MODE>(a.weight, a.w_f32, c, dim);  // early, where it costs few registers
         }
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const uint32_t step = j * width + group_chunk;
-            const Columns<VEC> c(lane, lanes, step);
+            const Columns<MODE> c(lane, lanes, step);
             v[j] = c.first < dim ? unpack(rx[j]) : filled(0.f);
-            if (a.drop.on) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, v[j]);
+            if (a.drop.on) drop_columns<MODE>(a.drop, row, lane, lanes, step, warp_lots, v[j]);
             if (a.res && c.first < dim) {
                 const Chunk r = unpack(rr[j]);
 #pragma unroll
@@ -464,8 +508,8 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
         T *h = (T *)a.h + (uint64_t)row * a.h_stride;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
-            if (c.first < dim) store_chunk<T, VEC>(h, c, dim, v[j]);
+            const Columns<MODE> c(lane, lanes, j * width + group_chunk);
+            if (c.first < dim) store_chunk<T, MODE>(h, c, dim, v[j]);
         }
     }
     if (!a.plain) {
@@ -478,9 +522,9 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
         if (a.rstd && dim && (BLOCK ? threadIdx.x : lane) == 0) a.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+            const Columns<MODE> c(lane, lanes, j * width + group_chunk);
             if (c.first >= dim) continue;
-            if (C > 1) w[j] = load_weight<T, VEC>(a.weight, a.w_f32, c, dim);
+            if (C > 1) w[j] = load_weight<T, MODE>(a.weight, a.w_f32, c, dim);
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) v[j].p[i] = __fmul2_rn(v[j].p[i], __fmul2_rn(w[j].p[i], both(rstd)));
         }
@@ -490,9 +534,9 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
     float *scales = a.scales + (uint64_t)row * ((a.dim + kF8Block - 1) / kF8Block);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-        const Columns<VEC> c(lane, lanes, j * width + group_chunk);
-        if (F8) encode_columns<VEC>(v[j], c, lane, lanes, dim, codes, scales);
-        else if (c.first < dim) store_chunk<T, VEC>(y, c, dim, v[j]);
+        const Columns<MODE> c(lane, lanes, j * width + group_chunk);
+        if (F8) encode_columns<MODE>(v[j], c, lane, lanes, dim, codes, scales);
+        else if (c.first < dim) store_chunk<T, MODE>(y, c, dim, v[j]);
     }
 }
 
@@ -517,14 +561,14 @@ struct NormBackArgs {
 // 16 384 x 4096 f16: 102 us (0.80 of the copy rate), 38 411 x 256 bf16 20 us (0.75), 20 011 x 602 f32 42 us (0.88).
 // Bound by instructions with 16 to 32 warps an SM: bringing the next row into shared memory meanwhile (cp.async) made
 // it slower (139 us where this took 122), leaving the ragged path out of the aligned kernel faster (122 to 102).
-template <typename T, bool VEC, int C, bool BLOCK, int L>
+template <typename T, int MODE, int C, bool BLOCK, int L>
 __global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? (C == 1 ? 2 : 1) : C == 1 ? 4 : 2)
 k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
     const uint32_t lanes = C > 1 || BLOCK ? 32 : L ? L : 1u << log2_lanes;
     __shared__ float shared[32];
-    __shared__ uint4 lots[VEC ? 1 : BLOCK ? 512 : kThreads];
+    __shared__ uint4 lots[MODE == kWhole ? 1 : BLOCK ? 512 : kThreads];
     extern __shared__ float sums[];  // [groups of the block][dim], not BLOCK
-    uint4 *warp_lots = VEC ? lots : lots + (threadIdx.x & ~31u);
+    uint4 *warp_lots = MODE == kWhole ? lots : lots + (threadIdx.x & ~31u);
     const uint32_t lane = threadIdx.x & (lanes - 1), group_chunk = BLOCK ? threadIdx.x & ~31u : 0, width = BLOCK ? blockDim.x : lanes;
     const uint32_t per_block = BLOCK ? 1 : kThreads >> log2_lanes;
     Chunk dw[C];
@@ -539,20 +583,20 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
         Raw<T> ry[C], rh[C], rd[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+            const Columns<MODE> c(lane, lanes, j * width + group_chunk);
             ry[j] = rh[j] = rd[j] = Raw<T>{};
             if (c.first >= dim) continue;
-            rh[j] = load_chunk<T, VEC>(h_row, c, dim);
-            if (a.dy) ry[j] = load_chunk<T, VEC>(dy_row, c, dim);
-            if (a.dh) rd[j] = load_chunk<T, VEC>(dh_row, c, dim);
+            rh[j] = load_chunk<T, MODE>(h_row, c, dim);
+            if (a.dy) ry[j] = load_chunk<T, MODE>(dy_row, c, dim);
+            if (a.dh) rd[j] = load_chunk<T, MODE>(dh_row, c, dim);
         }
         const float rstd = dim ? a.rstd[row] : 0.f;
         Chunk gw[C], h[C];  // dy w and h
         float2 sum = both(0.f);
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Columns<VEC> c(lane, lanes, j * width + group_chunk);
-            const Chunk g = unpack(ry[j]), w = c.first < dim ? load_weight<T, VEC>(a.weight, a.w_f32, c, dim) : filled(0.f);
+            const Columns<MODE> c(lane, lanes, j * width + group_chunk);
+            const Chunk g = unpack(ry[j]), w = c.first < dim ? load_weight<T, MODE>(a.weight, a.w_f32, c, dim) : filled(0.f);
             h[j] = unpack(rh[j]);
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
@@ -566,14 +610,14 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const uint32_t step = j * width + group_chunk;
-            const Columns<VEC> c(lane, lanes, step);
+            const Columns<MODE> c(lane, lanes, step);
             Chunk t = unpack(rd[j]);
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) t.p[i] = __fadd2_rn(t.p[i], __ffma2_rn(gw[j].p[i], both(rstd), __fmul2_rn(h[j].p[i], both(coef))));
-            if (a.dres && c.first < dim) store_chunk<T, VEC>(dres, c, dim, t);
+            if (a.dres && c.first < dim) store_chunk<T, MODE>(dres, c, dim, t);
             if (a.dx) {
-                if (a.drop.on) drop_columns<VEC>(a.drop, row, lane, lanes, step, warp_lots, t);
-                if (c.first < dim) store_chunk<T, VEC>(dx, c, dim, t);
+                if (a.drop.on) drop_columns<MODE>(a.drop, row, lane, lanes, step, warp_lots, t);
+                if (c.first < dim) store_chunk<T, MODE>(dx, c, dim, t);
             }
         }
     }
@@ -581,7 +625,7 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
     float *mine = a.partial + (uint64_t)blockIdx.x * a.dim;
 #pragma unroll
     for (int j = 0; j < C; ++j) {
-        const Columns<VEC> c(lane, lanes, j * width + group_chunk);
+        const Columns<MODE> c(lane, lanes, j * width + group_chunk);
         float *to = BLOCK ? mine : sums + (threadIdx.x >> log2_lanes) * a.dim;
 #pragma unroll
         for (uint32_t i = 0; i < kChunk; ++i)
@@ -660,6 +704,16 @@ bool vec_rows(const void *p, uint64_t stride, uint32_t elem) {
     return !p || ((uintptr_t)p % (kChunk * elem) == 0 && stride % kChunk == 0);
 }
 
+// Whether pairs of its 16-bit elements are words, and pairs of f32 weights eight bytes.
+bool pair_rows(const void *p, uint64_t stride, uint32_t elem) { return !p || ((uintptr_t)p % (2 * elem) == 0 && stride % 2 == 0); }
+// f(std::integral_constant<int, MODE>) of the ways that rows of type T are walked.
+template <typename T, typename F> auto with_mode(bool vec, bool pairs, F f) {
+    if (vec) return f(std::integral_constant<int, kWhole>{});
+    if constexpr (sizeof(T) == 2)
+        if (pairs) return f(std::integral_constant<int, kPair>{});
+    return f(std::integral_constant<int, kSingle>{});
+}
+
 template <typename F> void with_type(int dtype, F f) {
     if (dtype == AG_F32) f((float *)nullptr);
     else if (dtype == AG_F16) f((__half *)nullptr);
@@ -724,25 +778,25 @@ Split split_row(uint64_t rows, uint32_t dim, int dtype, bool vec, bool backward)
 }
 
 // f(std::integral_constant<int, L>) for the lanes of a row that is not aligned; 0 for others.
-template <bool VEC, typename F> auto with_lanes(uint32_t lanes, F f) {
-    if constexpr (VEC) return f(std::integral_constant<int, 0>{});
+template <int MODE, typename F> auto with_lanes(uint32_t lanes, F f) {
+    if constexpr (MODE == kWhole) return f(std::integral_constant<int, 0>{});
     else return lanes == 4 ? f(std::integral_constant<int, 4>{}) : lanes == 8 ? f(std::integral_constant<int, 8>{}) :
                 lanes == 16 ? f(std::integral_constant<int, 16>{}) : f(std::integral_constant<int, 32>{});
 }
 
-template <typename T, bool VEC, bool F8>
+template <typename T, int MODE, bool F8>
 cudaError_t launch_norm(const NormArgs &a, int dtype, cudaStream_t st) {
-    const Split s = split_row(a.rows, a.dim, dtype, VEC, false);
+    const Split s = split_row(a.rows, a.dim, dtype, MODE == kWhole, false);
     const uint64_t per = s.lanes ? s.threads / s.lanes : 1;
     const uint32_t grid = (uint32_t)((a.rows + per - 1) / per), lanes = s.log2_lanes();  // rows of a whole block are 1 KB and more
     if (s.lanes) {
         if (s.chunks == 1)
-            with_lanes<VEC>(s.lanes, [&](auto l) { k_norm<T, VEC, 1, false, F8, decltype(l)::value><<<grid, s.threads, 0, st>>>(a, lanes); });
-        else k_norm<T, VEC, 2, false, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
+            with_lanes<MODE>(s.lanes, [&](auto l) { k_norm<T, MODE, 1, false, F8, decltype(l)::value><<<grid, s.threads, 0, st>>>(a, lanes); });
+        else k_norm<T, MODE, 2, false, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
     } else {
-        if (s.chunks == 1) k_norm<T, VEC, 1, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
-        else if (s.chunks == 2) k_norm<T, VEC, 2, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
-        else k_norm<T, VEC, 4, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
+        if (s.chunks == 1) k_norm<T, MODE, 1, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
+        else if (s.chunks == 2) k_norm<T, MODE, 2, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
+        else k_norm<T, MODE, 4, true, F8, 0><<<grid, s.threads, 0, st>>>(a, lanes);
     }
     return cudaGetLastError();
 }
@@ -762,32 +816,32 @@ uint32_t back_blocks_bound(uint64_t rows, uint32_t dim, int dtype) {
     return most;
 }
 
-template <typename T, bool VEC, int C, bool BLOCK, int L = 0>
+template <typename T, int MODE, int C, bool BLOCK, int L = 0>
 cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t &grid, cudaStream_t st) {
     const size_t shared = BLOCK || !a.partial ? 0 : (size_t)(s.threads / s.lanes) * a.dim * 4;
     static std::atomic<int> known[17];  // blocks of 32 i threads that an SM holds; registers decide, not the sums' shared memory
     int per_sm = known[s.threads / 32].load(std::memory_order_relaxed);
     if (per_sm == 0) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, VEC, C, BLOCK, L>, (int)s.threads, shared);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, MODE, C, BLOCK, L>, (int)s.threads, shared);
         if (e != cudaSuccess) return e;
         per_sm = std::max(1, per_sm);
         known[s.threads / 32].store(per_sm, std::memory_order_relaxed);
     }
     grid = back_blocks(a.rows, s, per_sm);
-    k_norm_back<T, VEC, C, BLOCK, L><<<grid, s.threads, shared, st>>>(a, s.log2_lanes());
+    k_norm_back<T, MODE, C, BLOCK, L><<<grid, s.threads, shared, st>>>(a, s.log2_lanes());
     return cudaGetLastError();
 }
 
-template <typename T, bool VEC>
+template <typename T, int MODE>
 cudaError_t launch_back(const NormBackArgs &a, int dtype, uint32_t &grid, cudaStream_t st) {
-    const Split s = split_row(a.rows, a.dim, dtype, VEC, true);
+    const Split s = split_row(a.rows, a.dim, dtype, MODE == kWhole, true);
     if (s.lanes) {
-        if (s.chunks == 1) return with_lanes<VEC>(s.lanes, [&](auto l) { return launch_back<T, VEC, 1, false, decltype(l)::value>(a, s, grid, st); });
-        return launch_back<T, VEC, 2, false>(a, s, grid, st);
+        if (s.chunks == 1) return with_lanes<MODE>(s.lanes, [&](auto l) { return launch_back<T, MODE, 1, false, decltype(l)::value>(a, s, grid, st); });
+        return launch_back<T, MODE, 2, false>(a, s, grid, st);
     }
-    if (s.chunks == 1) return launch_back<T, VEC, 1, true>(a, s, grid, st);
-    if (s.chunks == 2) return launch_back<T, VEC, 2, true>(a, s, grid, st);
-    return launch_back<T, VEC, 4, true>(a, s, grid, st);
+    if (s.chunks == 1) return launch_back<T, MODE, 1, true>(a, s, grid, st);
+    if (s.chunks == 2) return launch_back<T, MODE, 2, true>(a, s, grid, st);
+    return launch_back<T, MODE, 4, true>(a, s, grid, st);
 }
 
 }  // namespace
@@ -809,9 +863,9 @@ k_encode_rows(const float *src, uint64_t rows, uint32_t dim, uint64_t pitch, uin
     for (uint64_t row = blockIdx.x; row < rows; row += gridDim.x)
         for (uint32_t c0 = 0; c0 < dim; c0 += kThreads * kChunk) {
             const uint32_t lane = threadIdx.x & 31;
-            const Columns<false> c(lane, 32, c0 / kChunk + (threadIdx.x & ~31u));
-            const Chunk v = unpack(load_chunk<float, false>(src + row * dim, c, dim));
-            encode_columns<false>(v, c, lane, 32, dim, codes + row * pitch, scales + row * per_row);
+            const Columns<kSingle> c(lane, 32, c0 / kChunk + (threadIdx.x & ~31u));
+            const Chunk v = unpack(load_chunk<float, kSingle>(src + row * dim, c, dim));
+            encode_columns<kSingle>(v, c, lane, 32, dim, codes + row * pitch, scales + row * per_row);
         }
 }
 }  // namespace
@@ -849,9 +903,9 @@ extern "C" int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64
         using T = std::remove_pointer_t<decltype(t)>;
         if (flat) k_dropout_flat<T><<<(uint32_t)((rows * dim + kFlatElements - 1) / kFlatElements), kThreads, 0, (cudaStream_t)stream>>>(
             (const T *)x, (T *)y, rows * dim, Divide((uint32_t)dim), by, d);
-        else if (vec && dim % kChunk == 0) k_dropout<T, true, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
-        else if (vec) k_dropout<T, true, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
-        else k_dropout<T, false, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
+        else if (vec && dim % kChunk == 0) k_dropout<T, kWhole, false><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
+        else if (vec) k_dropout<T, kWhole, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
+        else k_dropout<T, kSingle, true><<<grid, kThreads, 0, (cudaStream_t)stream>>>((const T *)x, (T *)y, chunks, (uint32_t)dim, by, x_stride, y_stride, d);
     });
     AG_CUDA(cudaGetLastError());
     return AG_OK;
@@ -883,12 +937,15 @@ extern "C" int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream) 
     a.w_f32 = n->weight_dtype == AG_F32; a.plain = n->encode_only; a.eps = n->eps; a.inv_dim = 1.0f / (float)n->dim;
     const uint32_t e = elem_size(n->dtype);
     const bool vec = a.dim % kChunk == 0 && vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.y, a.y_stride, e) && vec_rows(a.h, a.h_stride, e);
+    const bool pairs = a.dim % 2 == 0 && pair_rows(a.weight, 0, elem_size(n->weight_dtype)) && pair_rows(a.x, a.x_stride, e) && pair_rows(a.res, a.res_stride, e) &&
+                       pair_rows(a.y, a.y_stride, e) && pair_rows(a.h, a.h_stride, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         cudaStream_t st = (cudaStream_t)stream;
-        if (a.codes) err = vec ? launch_norm<T, true, true>(a, n->dtype, st) : launch_norm<T, false, true>(a, n->dtype, st);
-        else err = vec ? launch_norm<T, true, false>(a, n->dtype, st) : launch_norm<T, false, false>(a, n->dtype, st);
+        err = with_mode<T>(vec, pairs, [&](auto mode) {
+            return a.codes ? launch_norm<T, decltype(mode)::value, true>(a, n->dtype, st) : launch_norm<T, decltype(mode)::value, false>(a, n->dtype, st);
+        });
     });
     AG_CUDA(err);
     return AG_OK;
@@ -931,10 +988,12 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
     const uint32_t e = elem_size(n->dtype);
     const bool vec = a.dim % kChunk == 0 && vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
                      vec_rows(a.dx, a.dim, e) && vec_rows(a.dres, a.dim, e);
+    const bool pairs = a.dim % 2 == 0 && pair_rows(a.weight, 0, elem_size(n->weight_dtype)) && pair_rows(a.dy, a.dy_stride, e) && pair_rows(a.dh, a.dh_stride, e) &&
+                       pair_rows(a.h, a.h_stride, e) && pair_rows(a.dx, a.dim, e) && pair_rows(a.dres, a.dim, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        err = vec ? launch_back<T, true>(a, n->dtype, grid, (cudaStream_t)stream) : launch_back<T, false>(a, n->dtype, grid, (cudaStream_t)stream);
+        err = with_mode<T>(vec, pairs, [&](auto mode) { return launch_back<T, decltype(mode)::value>(a, n->dtype, grid, (cudaStream_t)stream); });
     });
     AG_CUDA(err);
     if (n->dw)

@@ -256,9 +256,10 @@ def test_norm_gradient_against_differences(ops):
         assert abs(want - got) < 1e-5 * float((wide(g) * d).abs().sum()) + 1e-6
 
 
-def test_norm_bits_repeat_and_layouts(ops):
-    x, w, res, _ = norm_case(3000, 301, torch.bfloat16, 0.1, True, torch.bfloat16)
-    dy = rand(6, 3000, 301, dtype=torch.bfloat16)
+@pytest.mark.parametrize("dim,left,pitch", [(301, 7, 333), (100, 6, 134), (96, 8, 128)])
+def test_norm_bits_repeat_and_layouts(ops, dim, left, pitch):
+    x, w, res, _ = norm_case(3000, dim, torch.bfloat16, 0.1, True, torch.bfloat16)
+    dy = rand(6, 3000, dim, dtype=torch.bfloat16)
 
     def all_of(x, res, dy):
         leaves = [t.detach().requires_grad_() for t in (x, w, res)]
@@ -266,10 +267,10 @@ def test_norm_bits_repeat_and_layouts(ops):
         return (y, h, *torch.autograd.grad((y, h), leaves, (dy, dy)))
 
     first = all_of(x, res, dy)
-    pad = torch.zeros(3, 3000, 333, dtype=torch.bfloat16, device="cuda")
+    pad = torch.zeros(3, 3000, pitch, dtype=torch.bfloat16, device="cuda")
     for i, t in enumerate((x, res, dy)):
-        pad[i, :, 7:308] = t
-    for again in (all_of(x, res, dy), all_of(*(pad[i, :, 7:308] for i in range(3))),
+        pad[i, :, left:left + dim] = t
+    for again in (all_of(x, res, dy), all_of(*(pad[i, :, left:left + dim] for i in range(3))),
                   all_of(*(t.t().contiguous().t() for t in (x, res, dy)))):
         for a, b in zip(first, again):
             assert torch.equal(a, b)
