@@ -109,7 +109,8 @@ class Norm(C.Structure):
 class NormGrad(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("dy", "dh", "h", "weight", "rstd", "dx", "dresidual", "dw", "scratch")] + \
                [(n, C.c_uint64) for n in ("scratch_bytes", "rows", "dim", "dy_stride", "dh_stride", "h_stride", "seed", "offset")] + \
-               [("p", C.c_double), ("dtype", C.c_int32), ("weight_dtype", C.c_int32)]
+               [("p", C.c_double), ("dtype", C.c_int32), ("weight_dtype", C.c_int32)] + \
+               [("x", C.c_void_p), ("residual", C.c_void_p), ("x_stride", C.c_uint64), ("residual_stride", C.c_uint64)]
 
 
 class Product(C.Structure):

@@ -170,7 +170,10 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     static variable_list forward(AutogradContext *ctx, const Tensor &x, const MaybeTensor &weight, const MaybeTensor &residual, double eps, double p,
                                  int64_t seed, int64_t offset) {
         NormOut out = run_norm(x, weight, residual, eps, p, (uint64_t)seed, (uint64_t)offset, true);
-        ctx->save_for_backward({out.h, has(weight) ? *weight : Tensor(), out.rstd});
+        // 16-bit rows: not the rounded h but what it is made of, if that is not x alone
+        const bool again = x.scalar_type() != at::kFloat && !out.h.is_same(x);
+        ctx->save_for_backward({again ? x : out.h, has(weight) ? *weight : Tensor(), out.rstd, again && has(residual) ? *residual : Tensor()});
+        ctx->saved_data["again"] = again;
         ctx->saved_data["p"] = p;
         ctx->saved_data["seed"] = seed;
         ctx->saved_data["offset"] = offset;
@@ -183,7 +186,8 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
         variable_list got(7);
         if (!grads[0].defined() && !grads[1].defined()) return got;
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &h = saved[0], &weight = saved[1], &rstd = saved[2];
+        const Tensor &h = saved[0], &weight = saved[1], &rstd = saved[2], &res = saved[3];  // h, or x where it is made again
+        const bool again = ctx->saved_data["again"].toBool();
         const double p = ctx->saved_data["p"].toDouble();
         const bool residual = ctx->saved_data["residual"].toBool();
         // what autograd counts is the tensors that there were
@@ -191,7 +195,11 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
                    need_res = residual && ctx->needs_input_grad(weight.defined() ? 2 : 1);
         const Rows r(h);
         ag_norm_grad n{};
-        n.h = r.t.data_ptr(); n.rstd = rstd.data_ptr<float>(); n.rows = r.rows; n.dim = r.dim; n.h_stride = r.pitch; n.p = p;
+        std::optional<Rows> rr;
+        (again ? n.x : n.h) = r.t.data_ptr();
+        (again ? n.x_stride : n.h_stride) = r.pitch;
+        if (res.defined()) { rr.emplace(res); n.residual = rr->t.data_ptr(); n.residual_stride = rr->pitch; }
+        n.rstd = rstd.data_ptr<float>(); n.rows = r.rows; n.dim = r.dim; n.p = p;
         n.seed = (uint64_t)ctx->saved_data["seed"].toInt(); n.offset = (uint64_t)ctx->saved_data["offset"].toInt();
         n.dtype = tag_of(h.scalar_type());
         std::optional<Rows> dy, dh;

@@ -273,6 +273,48 @@ __device__ __forceinline__ void drop_columns(const Drop &d, uint32_t row, uint32
     }
 }
 
+// Bit e: element e of a chunk stays.  bits > bar is the carry of bits + ~bar; the next addition takes it in.
+__device__ __forceinline__ uint32_t stay_bits(const uint4 &r, uint32_t not_bar) {
+    uint32_t m;
+    asm("{\n .reg .u32 t;\n"
+        " add.cc.u32 t, %4, %9;\n addc.u32 %0, 0, 0;\n"
+        " add.cc.u32 t, %8, %9;\n addc.u32 %0, %0, %0;\n"
+        " add.cc.u32 t, %3, %9;\n addc.u32 %0, %0, %0;\n"
+        " add.cc.u32 t, %7, %9;\n addc.u32 %0, %0, %0;\n"
+        " add.cc.u32 t, %2, %9;\n addc.u32 %0, %0, %0;\n"
+        " add.cc.u32 t, %6, %9;\n addc.u32 %0, %0, %0;\n"
+        " add.cc.u32 t, %1, %9;\n addc.u32 %0, %0, %0;\n"
+        " add.cc.u32 t, %5, %9;\n addc.u32 %0, %0, %0;\n}"
+        : "=&r"(m) : "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(r.x << 16), "r"(r.y << 16), "r"(r.z << 16), "r"(r.w << 16), "r"(not_bar));
+    return m;
+}
+
+// Which of a thread's eight columns stay, a bit each, where one mask is used twice: the lots are as in drop_columns.
+template <int MODE>
+__device__ __forceinline__ uint32_t stay_columns(const Drop &d, uint32_t row, uint32_t lane, uint32_t lanes, uint32_t step_chunk, uint4 *warp_lots) {
+    const uint4 r = lots_of(d, row, step_chunk + lane);
+    if (MODE == kWhole) return stay_bits(r, ~d.bar);
+    __syncwarp();
+    warp_lots[threadIdx.x & 31] = r;
+    __syncwarp();
+    const uint16_t *group = (const uint16_t *)(warp_lots + ((threadIdx.x & 31) - lane));
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kChunk / 2; ++i) {
+        const uint32_t lo = MODE == kPair ? ((const uint32_t *)group)[lane + i * lanes] << 16 : (uint32_t)group[lane + 2 * i * lanes] << 16,
+                       hi = MODE == kPair ? ((const uint32_t *)group)[lane + i * lanes] : (uint32_t)group[lane + (2 * i + 1) * lanes] << 16;
+        m |= (lo > d.bar ? 1u << 2 * i : 0u) | (hi > d.bar ? 2u << 2 * i : 0u);
+    }
+    return m;
+}
+__device__ __forceinline__ void drop_by_bits(const Drop &d, uint32_t stay, Chunk &v) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+        const float2 f = __fmul2_rn(v.p[i], both(d.scale));
+        v.p[i] = make_float2(stay >> 2 * i & 1 ? f.x : 0.f, stay >> (2 * i + 1) & 1 ? f.y : 0.f);
+    }
+}
+
 constexpr int kThreads = 256;
 
 // Two chunks a thread, a block's width apart; both loads are in flight before either is used.  38 411 x 256
@@ -297,22 +339,6 @@ k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_
         if (d.on) drop_chunk(d, lots_of(d, row[u], chunk[u]), v);
         store_chunk<T, MODE, RAGGED>(y + row[u] * y_stride, Columns<MODE>(0, 1, chunk[u]), dim, v);
     }
-}
-
-// Bit e: element e of a chunk stays.  bits > bar is the carry of bits + ~bar; the next addition takes it in.
-__device__ __forceinline__ uint32_t stay_bits(const uint4 &r, uint32_t not_bar) {
-    uint32_t m;
-    asm("{\n .reg .u32 t;\n"
-        " add.cc.u32 t, %4, %9;\n addc.u32 %0, 0, 0;\n"
-        " add.cc.u32 t, %8, %9;\n addc.u32 %0, %0, %0;\n"
-        " add.cc.u32 t, %3, %9;\n addc.u32 %0, %0, %0;\n"
-        " add.cc.u32 t, %7, %9;\n addc.u32 %0, %0, %0;\n"
-        " add.cc.u32 t, %2, %9;\n addc.u32 %0, %0, %0;\n"
-        " add.cc.u32 t, %6, %9;\n addc.u32 %0, %0, %0;\n"
-        " add.cc.u32 t, %1, %9;\n addc.u32 %0, %0, %0;\n"
-        " add.cc.u32 t, %5, %9;\n addc.u32 %0, %0, %0;\n}"
-        : "=&r"(m) : "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(r.x << 16), "r"(r.y << 16), "r"(r.z << 16), "r"(r.w << 16), "r"(not_bar));
-    return m;
 }
 
 // Contiguous rows whose length is no multiple of eight: the lots belong to chunks, the memory is walked
@@ -542,10 +568,11 @@ k_norm(const NormArgs a, uint32_t log2_lanes) {
 
 struct NormBackArgs {
     const void *dy, *dh, *h, *weight;
+    const void *x, *res;  // h null: what h is made of (16-bit rows)
     const float *rstd;
     void *dx, *dres;
     float *partial;  // [blocks, dim] sums of dy h rstd over a block's rows, or null
-    uint32_t rows, dy_stride, dh_stride, h_stride;
+    uint32_t rows, dy_stride, dh_stride, h_stride, x_stride, res_stride;
     uint32_t dim;
     int w_f32;
     float inv_dim;
@@ -555,13 +582,15 @@ struct NormBackArgs {
 // g = dy w; t = dh + rstd g - h rstd^3 / dim sum(g h): the gradient of h and of the residual; dx = dropout(t).
 // dw = sum over rows of dy h rstd: a thread's columns are the same in every row, so it keeps their
 // sums; a block adds its lane groups in order into its row of `partial`, and k_norm_dw adds those.
-// No atomics: the same bits every time on the same GPU.  h is read as it was stored, rounded to the rows' type: a
-// second read of x and residual would be exact and cost a pass over a tensor more.
+// No atomics: the same bits every time on the same GPU.  Everything is computed from the h of 32 bits that the forward
+// pass normalised: f32 rows (and x alone) hold it, for 16-bit rows it is made again from x and residual, which is
+// one tensor more to read than the rounded h where there is a residual.
 //
 // 16 384 x 4096 f16: 102 us (0.80 of the copy rate), 38 411 x 256 bf16 20 us (0.75), 20 011 x 602 f32 42 us (0.88).
 // Bound by instructions with 16 to 32 warps an SM: bringing the next row into shared memory meanwhile (cp.async) made
 // it slower (139 us where this took 122), leaving the ragged path out of the aligned kernel faster (122 to 102).
-template <typename T, int MODE, int C, bool BLOCK, int L>
+// AGAIN: h may have to be made again.  The mask is then needed twice and kept as bits; else it is made where dx is.
+template <typename T, int MODE, int C, bool BLOCK, int L, bool AGAIN>
 __global__ void __launch_bounds__(BLOCK ? 512 : kThreads, BLOCK ? (C == 1 ? 2 : 1) : C == 1 ? 4 : 2)
 k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
     const uint32_t lanes = C > 1 || BLOCK ? 32 : L ? L : 1u << log2_lanes;
@@ -578,26 +607,38 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
     for (uint32_t base = blockIdx.x * per_block; base < a.rows; base += gridDim.x * per_block, turn ^= 16) {  // rows + a grid's worth fit 32 bits
         const uint32_t row = base + (BLOCK ? 0 : threadIdx.x >> log2_lanes);
         const uint32_t dim = row < a.rows ? a.dim : 0;
-        const T *h_row = (const T *)a.h + (uint64_t)row * a.h_stride, *dy_row = (const T *)a.dy + (uint64_t)row * a.dy_stride,
+        const bool again = AGAIN && !a.h;
+        const T *h_row = again ? (const T *)a.x + (uint64_t)row * a.x_stride : (const T *)a.h + (uint64_t)row * a.h_stride,
+                *res_row = (const T *)a.res + (uint64_t)row * a.res_stride, *dy_row = (const T *)a.dy + (uint64_t)row * a.dy_stride,
                 *dh_row = (const T *)a.dh + (uint64_t)row * a.dh_stride;
-        Raw<T> ry[C], rh[C], rd[C];
+        Raw<T> ry[C], rh[C], rd[C], rr[C];
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const Columns<MODE> c(lane, lanes, j * width + group_chunk);
-            ry[j] = rh[j] = rd[j] = Raw<T>{};
+            ry[j] = rh[j] = rd[j] = rr[j] = Raw<T>{};
             if (c.first >= dim) continue;
             rh[j] = load_chunk<T, MODE>(h_row, c, dim);
+            if (again && a.res) rr[j] = load_chunk<T, MODE>(res_row, c, dim);
             if (a.dy) ry[j] = load_chunk<T, MODE>(dy_row, c, dim);
             if (a.dh) rd[j] = load_chunk<T, MODE>(dh_row, c, dim);
         }
         const float rstd = dim ? a.rstd[row] : 0.f;
         Chunk gw[C], h[C];  // dy w and h
+        uint32_t stay[C];
         float2 sum = both(0.f);
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-            const Columns<MODE> c(lane, lanes, j * width + group_chunk);
+            const uint32_t step = j * width + group_chunk;
+            const Columns<MODE> c(lane, lanes, step);
+            if (AGAIN && a.drop.on) stay[j] = stay_columns<MODE>(a.drop, row, lane, lanes, step, warp_lots);
             const Chunk g = unpack(ry[j]), w = c.first < dim ? load_weight<T, MODE>(a.weight, a.w_f32, c, dim) : filled(0.f);
             h[j] = unpack(rh[j]);
+            if (again) {
+                if (a.drop.on) drop_by_bits(a.drop, stay[j], h[j]);
+                const Chunk r = unpack(rr[j]);
+#pragma unroll
+                for (int i = 0; i < kPairs; ++i) if (a.res) h[j].p[i] = __fadd2_rn(h[j].p[i], r.p[i]);
+            }
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
                 dw[j].p[i] = __ffma2_rn(__fmul2_rn(g.p[i], h[j].p[i]), both(rstd), dw[j].p[i]);
@@ -616,7 +657,8 @@ k_norm_back(const NormBackArgs a, uint32_t log2_lanes) {
             for (int i = 0; i < kPairs; ++i) t.p[i] = __fadd2_rn(t.p[i], __ffma2_rn(gw[j].p[i], both(rstd), __fmul2_rn(h[j].p[i], both(coef))));
             if (a.dres && c.first < dim) store_chunk<T, MODE>(dres, c, dim, t);
             if (a.dx) {
-                if (a.drop.on) drop_columns<MODE>(a.drop, row, lane, lanes, step, warp_lots, t);
+                if (AGAIN && a.drop.on) drop_by_bits(a.drop, stay[j], t);
+                else if (a.drop.on) drop_columns<MODE>(a.drop, row, lane, lanes, step, warp_lots, t);
                 if (c.first < dim) store_chunk<T, MODE>(dx, c, dim, t);
             }
         }
@@ -747,13 +789,14 @@ int32_t check_pitches(const char *who, std::initializer_list<uint64_t> pitches) 
 // `chunks` chunks each.  Whole blocks: as few threads as hold the row in
 // `most` chunks each (64 bytes of f16 / bf16 or f32: a thread's loads are all in flight together, and the sum
 // waits for fewer warps), unless that leaves many of them idle; a chunk each where there are no more rows than
-// SMs, and the time is one row's latency, and in the backward pass over rows that are not aligned (registers).  16 384 rows of 4096 f16, forward: four chunks 52 us, two 64, one 66.
+// SMs, and the time is one row's latency, and in the backward pass over rows that are not aligned (registers); two where the backward
+// pass makes h again, as long as the row fits (registers: four spill).  16 384 rows of 4096 f16, forward: four chunks 52 us, two 64, one 66.
 struct Split {
     uint32_t lanes, threads;
     int chunks;
     uint32_t log2_lanes() const { uint32_t l = 0; while ((1u << l) < lanes) ++l; return lanes ? l : 5; }
 };
-Split split_row(uint64_t rows, uint32_t dim, int dtype, bool vec, bool backward) {
+Split split_row(uint64_t rows, uint32_t dim, int dtype, bool vec, bool backward, bool again = false) {
     const uint32_t n = (dim + kChunk - 1) / kChunk;
     Split s{1, kThreads, 1};
     if (!vec) s.lanes = 4;
@@ -763,7 +806,7 @@ Split split_row(uint64_t rows, uint32_t dim, int dtype, bool vec, bool backward)
         return s;
     }
     s.lanes = 0;
-    const int most = rows <= (uint64_t)kSMs || (!vec && backward) ? 1 : dtype == AG_F32 ? 2 : 4;
+    const int most = rows <= (uint64_t)kSMs || (!vec && backward) ? 1 : dtype == AG_F32 || again ? 2 : 4;
     uint32_t slots = 0xFFFFFFFFu;
     for (int c = most; c; c /= 2) {
         const uint32_t threads = (n + 32 * c - 1) / (32 * c) * 32;
@@ -809,39 +852,41 @@ uint32_t back_blocks(uint64_t rows, const Split &s, uint32_t per_sm) {
 }
 uint32_t back_blocks_bound(uint64_t rows, uint32_t dim, int dtype) {
     uint32_t most = 0;
-    for (const bool vec : {false, true}) {
-        const Split s = split_row(rows, dim, dtype, vec, true);
+    for (const int form : {0, 1, 3}) {
+        const Split s = split_row(rows, dim, dtype, form & 1, true, form & 2);
         most = std::max(most, back_blocks(rows, s, std::min(2048 / s.threads, 32u)));
     }
     return most;
 }
 
-template <typename T, int MODE, int C, bool BLOCK, int L = 0>
+template <typename T, int MODE, int C, bool BLOCK, int L = 0, bool AGAIN = sizeof(T) == 2>
 cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t &grid, cudaStream_t st) {
     const size_t shared = BLOCK || !a.partial ? 0 : (size_t)(s.threads / s.lanes) * a.dim * 4;
     static std::atomic<int> known[17];  // blocks of 32 i threads that an SM holds; registers decide, not the sums' shared memory
     int per_sm = known[s.threads / 32].load(std::memory_order_relaxed);
     if (per_sm == 0) {
-        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, MODE, C, BLOCK, L>, (int)s.threads, shared);
+        const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, k_norm_back<T, MODE, C, BLOCK, L, AGAIN>, (int)s.threads, shared);
         if (e != cudaSuccess) return e;
         per_sm = std::max(1, per_sm);
         known[s.threads / 32].store(per_sm, std::memory_order_relaxed);
     }
     grid = back_blocks(a.rows, s, per_sm);
-    k_norm_back<T, MODE, C, BLOCK, L><<<grid, s.threads, shared, st>>>(a, s.log2_lanes());
+    k_norm_back<T, MODE, C, BLOCK, L, AGAIN><<<grid, s.threads, shared, st>>>(a, s.log2_lanes());
     return cudaGetLastError();
 }
 
 template <typename T, int MODE>
 cudaError_t launch_back(const NormBackArgs &a, int dtype, uint32_t &grid, cudaStream_t st) {
-    const Split s = split_row(a.rows, a.dim, dtype, MODE == kWhole, true);
+    const Split s = split_row(a.rows, a.dim, dtype, MODE == kWhole, true, !a.h);
     if (s.lanes) {
         if (s.chunks == 1) return with_lanes<MODE>(s.lanes, [&](auto l) { return launch_back<T, MODE, 1, false, decltype(l)::value>(a, s, grid, st); });
         return launch_back<T, MODE, 2, false>(a, s, grid, st);
     }
     if (s.chunks == 1) return launch_back<T, MODE, 1, true>(a, s, grid, st);
     if (s.chunks == 2) return launch_back<T, MODE, 2, true>(a, s, grid, st);
-    return launch_back<T, MODE, 4, true>(a, s, grid, st);
+    if constexpr (sizeof(T) == 2)
+        if (!a.h) return launch_back<T, MODE, 4, true, 0, true>(a, s, grid, st);
+    return launch_back<T, MODE, 4, true, 0, false>(a, s, grid, st);  // without the registers that the other needs
 }
 
 }  // namespace
@@ -967,29 +1012,32 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
     if (n->dim > kMaxNormDim) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: at most %u columns, got %llu", kMaxNormDim, (unsigned long long)n->dim);
     if (n->weight && n->weight_dtype != n->dtype && n->weight_dtype != AG_F32)
         return fail(AG_ERR_VALUE, "ag_rows_norm_backward: the weights are f32 or of the rows' type");
-    AG_TRY(check_pitches("ag_rows_norm_backward", {n->dy_stride, n->dh_stride, n->h_stride}));
+    AG_TRY(check_pitches("ag_rows_norm_backward", {n->dy_stride, n->dh_stride, n->h_stride, n->x_stride, n->residual_stride}));
     NormBackArgs a{};
     AG_TRY(make_drop(n->p, n->seed, n->offset, &a.drop));
+    if (n->rows && ((!n->h && !n->x) || !n->rstd || (n->dw && !n->scratch))) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: null argument");
+    if (n->h && (n->x || n->residual)) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: either h or what it is made of");
+    if (n->x && n->dtype == AG_F32) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: rows of f32 come with their h");
     DeviceGuard guard(device);
     if (!guard.ok) return AG_ERR_CUDA;
     if (n->rows == 0) {
         if (n->dw) AG_CUDA(cudaMemsetAsync(n->dw, 0, n->dim * elem_size(n->weight_dtype), (cudaStream_t)stream));
         return AG_OK;
     }
-    if (!n->h || !n->rstd || (n->dw && !n->scratch)) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: null argument");
     uint32_t grid = back_blocks_bound(n->rows, (uint32_t)n->dim, n->dtype);
     if (n->dw && n->scratch_bytes < (uint64_t)grid * n->dim * 4)
         return fail(AG_ERR_VALUE, "ag_rows_norm_backward: %llu bytes of scratch, %llu are needed", (unsigned long long)n->scratch_bytes,
                     (unsigned long long)grid * n->dim * 4);
     a.dy = n->dy; a.dh = n->dh; a.h = n->h; a.weight = n->weight; a.rstd = n->rstd; a.dx = n->dx; a.dres = n->dresidual;
+    a.x = n->x; a.res = n->residual; a.x_stride = (uint32_t)n->x_stride; a.res_stride = (uint32_t)n->residual_stride;
     a.partial = n->dw ? (float *)n->scratch : nullptr;
     a.rows = (uint32_t)n->rows; a.dim = (uint32_t)n->dim; a.dy_stride = (uint32_t)n->dy_stride; a.dh_stride = (uint32_t)n->dh_stride; a.h_stride = (uint32_t)n->h_stride;
     a.w_f32 = n->weight_dtype == AG_F32; a.inv_dim = 1.0f / (float)n->dim;
     const uint32_t e = elem_size(n->dtype);
     const bool vec = a.dim % kChunk == 0 && vec_rows(a.weight, 0, elem_size(n->weight_dtype)) && vec_rows(a.dy, a.dy_stride, e) && vec_rows(a.dh, a.dh_stride, e) && vec_rows(a.h, a.h_stride, e) &&
-                     vec_rows(a.dx, a.dim, e) && vec_rows(a.dres, a.dim, e);
+                     vec_rows(a.x, a.x_stride, e) && vec_rows(a.res, a.res_stride, e) && vec_rows(a.dx, a.dim, e) && vec_rows(a.dres, a.dim, e);
     const bool pairs = a.dim % 2 == 0 && pair_rows(a.weight, 0, elem_size(n->weight_dtype)) && pair_rows(a.dy, a.dy_stride, e) && pair_rows(a.dh, a.dh_stride, e) &&
-                       pair_rows(a.h, a.h_stride, e) && pair_rows(a.dx, a.dim, e) && pair_rows(a.dres, a.dim, e);
+                       pair_rows(a.h, a.h_stride, e) && pair_rows(a.x, a.x_stride, e) && pair_rows(a.res, a.res_stride, e) && pair_rows(a.dx, a.dim, e) && pair_rows(a.dres, a.dim, e);
     cudaError_t err = cudaSuccess;
     with_type(n->dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -62,7 +62,9 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: 
 
     One pass over the rows: sum, statistics and product are held in float32 and rounded once.
     Without residual and dropout h is `x` itself.  `weight` is [dim], of x's type or float32; rows have at most 16384 columns.  The
-    gradients of x, weight and residual take one pass too; weight's is summed in a fixed order.
+    gradients of x, weight and residual take one pass too; weight's is summed in a fixed order.  They are those of the
+    unrounded h: for float16 and bfloat16 rows x and residual are kept for the backward pass (as autograd keeps any operator's
+    inputs: changed in place meanwhile, the backward pass is refused), for float32 h.
     `p`, `seed` and `offset` are `dropout`'s."""
     _check_key(seed, offset)
     return _ops.add_rms_norm(x, weight, residual, eps, p, seed, offset)

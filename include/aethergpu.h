@@ -723,7 +723,9 @@ int32_t ag_rows_norm(const ag_norm *n, int32_t device, void *stream);
 /* Gradients of the norm, from dy and dh (the gradients of y and h, either may be NULL), h and
  * rstd: dresidual = dh + d(norm); dx = dropout(dresidual) with the forward call's mask; dw, of
  * weight_dtype, the sum over the rows of dy h rstd.  Any of the three may be NULL; dx and
- * dresidual are contiguous.  dw needs scratch of ag_rows_norm_backward_scratch bytes, which
+ * dresidual are contiguous.  The forward call normalised h before it was rounded to the rows' type:
+ * for f16 and bf16 rows h may be NULL and x (with residual, or NULL) given instead, from which it is
+ * made again, unrounded.  dw needs scratch of ag_rows_norm_backward_scratch bytes, which
  * belongs to the call until it is done; its summation order is fixed. */
 typedef struct {
     const void *dy, *dh, *h, *weight;
@@ -734,6 +736,8 @@ typedef struct {
     uint64_t seed, offset;
     double p;
     int32_t dtype, weight_dtype;
+    const void *x, *residual; /* instead of h */
+    uint64_t x_stride, residual_stride;
 } ag_norm_grad;
 int32_t ag_rows_norm_backward_scratch(uint64_t rows, uint64_t dim, int32_t dtype, int32_t device,
                                       uint64_t *bytes);

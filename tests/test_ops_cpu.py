@@ -129,3 +129,17 @@ def test_formulas_agree_with_autograd_and_differences():
 def test_mask_of_all_and_nothing():
     assert bool((f.mask(3, 9, 0.0, 1, 0) == 1).all()) and bool((f.mask(3, 9, 1.0, 1, 0) == 0).all())
     assert np.array_equal(f.lots(4, 9, 1, 0)[2:], f.lots(2, 9, 1, 0, first_row=2))
+
+
+def _norm_back(**kw):
+    base = dict(dy=16, h=16, rstd=16, dx=16, rows=2, dim=8, dy_stride=8, h_stride=8, x_stride=8, residual_stride=8, dtype=1)
+    base.update(kw)
+    return _lib.lib().ag_rows_norm_backward(C.byref(_lib.NormGrad(**base)), 0, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(h=None), "null"), (dict(x=16), "either"), (dict(residual=16), "either"), (dict(h=None, x=16, dtype=0), "f32"),
+    (dict(h=None, x=16, x_stride=1 << 32), "apart"), (dict(h=None, x=16, residual=16, residual_stride=1 << 32), "apart")])
+def test_norm_gradient_refusals(kw, text):
+    with pytest.raises(ValueError, match=text):
+        _lib.check(_norm_back(**kw))
