@@ -76,7 +76,8 @@ class FeatureStore:
 
     @staticmethod
     def from_array(features, dtype: str = "f32", *, device: int | None = None) -> "FeatureStore":
-        """Encode f32 rows (numpy, or a CUDA float32 tensor) into `dtype` on the device.
+        """Encode f32 rows (numpy, or a CUDA float32 tensor) into `dtype` on the device (`device`, else the
+        tensor's own or the current one).  Waits for the tensor's current stream, on which its rows were written.
         `"i8"` is the reference's block-scaled int8 codec (one byte per element and one f32
         scale per 32 elements of a row, crates/aethergraph-core/src/internal/feature_codec.rs):
         lossy, a quarter of f32's bytes; gathers decode to exactly what the reference's
@@ -92,6 +93,12 @@ class FeatureStore:
             if features.dtype != torch.float32 or features.dim() != 2 or not features.is_contiguous():
                 raise ValueError("features tensor must be a contiguous 2-d float32 tensor")
             kind = _lib.AG_MEM_DEVICE if features.is_cuda else _lib.AG_MEM_HOST
+            if features.is_cuda:
+                if device is None:
+                    dev = features.get_device()
+                elif features.get_device() != dev:
+                    raise ValueError(f"features are on {features.device}, the store is to be on cuda:{dev}")
+                torch.cuda.current_stream(features.device).synchronize()
             _lib.check(_lib.lib().ag_features_from_f32(features.data_ptr(), features.shape[0], features.shape[1],
                                                        _lib.DTYPE_TAG[dtype], kind, dev, C.byref(out)))
             return FeatureStore(out.value)
