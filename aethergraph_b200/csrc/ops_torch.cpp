@@ -65,10 +65,18 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const Tensor &like) { r
 Tensor fresh_like(const Tensor &x) { return fresh(x.sizes(), x.scalar_type(), x); }
 void *stream_of(const Tensor &x) { return c10::cuda::getCurrentCUDAStream(x.get_device()).stream(); }
 bool has(const MaybeTensor &t) { return t.has_value() && t->defined(); }
+// Derivatives are reverse mode only.  A forward-mode tangent is not in the memory that a kernel is given, and
+// would be gone without a word.
+void no_tangent(const char *what, std::initializer_list<const Tensor *> tensors) {
+    for (const Tensor *t : tensors)
+        if (t && t->defined() && t->_fw_grad(0).defined()) refuse(what, " has no forward-mode derivative");
+}
+const Tensor *ptr(const MaybeTensor &t) { return has(t) ? &*t : nullptr; }
 void once(const char *what) {
     if (at::GradMode::is_enabled()) throw std::runtime_error(c10::str(what, " is differentiable once; call the backward pass without create_graph"));
 }
 void no_gradient(const char *what, std::initializer_list<const Tensor *> tensors) {
+    no_tangent(what, tensors);
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor *t : tensors)
         if (t && t->defined() && t->requires_grad()) refuse(what, " has no gradient; call it under torch.no_grad()");
@@ -99,12 +107,14 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout(const Tensor &x, double p, uint64_t seed, uint64_t offset) {
+    no_tangent("dropout", {&x});
     check_rows(x, "x");
     if (x.requires_grad() && at::GradMode::is_enabled()) return Dropout::apply(x, p, (int64_t)seed, (int64_t)offset);
     return run_dropout(x, p, seed, offset);
 }
 
 void dropout_(const Tensor &x, double p, uint64_t seed, uint64_t offset) {
+    no_tangent("dropout_", {&x});
     const int tag = check_rows(x, "x");
     if (x.requires_grad() && at::GradMode::is_enabled()) refuse("dropout_ is for rows that need no gradient; use dropout");
     const Rows r(x);
@@ -237,6 +247,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
 
 std::pair<Tensor, Tensor> add_rms_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &residual, double eps, double p, uint64_t seed,
                                        uint64_t offset) {
+    no_tangent("add_rms_norm", {&x, ptr(weight), ptr(residual)});
     check_norm(x, weight, residual);
     if (at::GradMode::is_enabled() && (x.requires_grad() || (has(weight) && weight->requires_grad()) || (has(residual) && residual->requires_grad()))) {
         const variable_list out = AddRmsNorm::apply(x, weight, residual, eps, p, (int64_t)seed, (int64_t)offset);
@@ -264,8 +275,8 @@ std::pair<Tensor, Tensor> to_f8(NormCall &c, const Tensor &x) {
 }
 
 std::tuple<Tensor, Tensor, Tensor> add_rms_norm_f8(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &residual, double eps) {
+    no_gradient("add_rms_norm_f8", {&x, ptr(weight), ptr(residual)});
     check_norm(x, weight, residual);
-    no_gradient("add_rms_norm_f8", {&x, has(weight) ? &*weight : nullptr, has(residual) ? &*residual : nullptr});
     NormCall c(x, weight, residual, eps);
     Tensor h = x;
     if (has(residual)) {
@@ -277,17 +288,17 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_f8(const Tensor &x, const MaybeT
 }
 
 std::pair<Tensor, Tensor> encode_f8(const Tensor &x) {
-    check_rows(x, "x");
     no_gradient("encode_f8", {&x});
+    check_rows(x, "x");
     NormCall c(x, std::nullopt, std::nullopt, 0.0);
     c.n.encode_only = 1;
     return to_f8(c, x);
 }
 
 std::pair<Tensor, Tensor> encode_weight_f8(const Tensor &w) {
+    no_gradient("encode_weight_f8", {&w});
     const int tag = check_rows(w, "w");
     if (w.dim() != 2) refuse("weights must be [out, dim], got shape ", w.sizes());
-    no_gradient("encode_weight_f8", {&w});
     const Rows r(w);
     Tensor codes = empty_codes(r.rows, r.dim, w), scales = empty_scales(blocks_of(r.rows), r.dim, w);
     check(ag_rows_encode_weight(r.t.data_ptr(), r.rows, r.dim, r.pitch, tag, codes.data_ptr(), f8_pitch(r.dim), scales.data_ptr<float>(), w.get_device(),
@@ -311,6 +322,8 @@ void check_f8(const Tensor &codes, const Tensor &scales, const char *what, int64
 struct Held { const void *codes; const float *scales; int64_t rows, dim, pitch; int device; };
 
 Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &ids, const MaybeTensor &bias, at::ScalarType dtype) {
+    no_tangent("a product of 8-bit rows", {&weight_scales});
+    no_gradient("a product of 8-bit rows", {ptr(bias)});
     check_f8(weight, weight_scales, "weight", kF8Block);
     const int64_t out_dim = weight.size(0);
     if (weight.get_device() != held.device || weight.size(1) != held.dim || out_dim == 0)
@@ -330,7 +343,6 @@ Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scal
         if (!bias->is_cuda() || bias->get_device() != held.device || bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != out_dim ||
             !bias->is_contiguous())
             refuse("bias must be contiguous float32 [", out_dim, "] on cuda:", held.device);
-        no_gradient("a product of 8-bit rows", {&*bias});
         p.bias = bias->data_ptr<float>();
     }
     Tensor out = fresh({(int64_t)p.rows, out_dim}, dtype, weight);
@@ -341,6 +353,7 @@ Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scal
 
 Tensor product_f8(const Tensor &codes, const Tensor &scales, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &ids, const MaybeTensor &bias,
                   at::ScalarType dtype) {
+    no_tangent("a product of 8-bit rows", {&scales});
     check_f8(codes, scales, "codes", 1);
     return product({codes.data_ptr(), scales.data_ptr<float>(), codes.size(0), codes.size(1), codes.stride(0), (int)codes.get_device()}, weight, weight_scales,
                    ids, bias, dtype);

@@ -9,8 +9,8 @@ The rows are CUDA tensors of float32, float16 or bfloat16 whose last dimension i
 row; leading dimensions are flattened.  Calls run on the current stream of the rows' device,
 wait for nothing and may be captured into a CUDA graph (a backward pass, as with any PyTorch operator,
 only while no autograd graph of the same leaves made on another stream is alive).  `dropout`
-and `add_rms_norm` have gradients (once differentiable); the 8-bit operators are for
-inference and have none.
+and `add_rms_norm` have gradients (reverse mode, once: a backward pass with create_graph=True is refused, and so
+are inputs with a forward-mode tangent); the 8-bit operators are for inference and have none.
 
 8-bit rows are a pair (codes, scales): torch.float8_e4m3fn codes [rows, dim], whose row pitch
 is a multiple of 16 bytes, and float32 scales [rows, ceil(dim / 128)], value = code * scale.

@@ -143,3 +143,20 @@ def _norm_back(**kw):
 def test_norm_gradient_refusals(kw, text):
     with pytest.raises(ValueError, match=text):
         _lib.check(_norm_back(**kw))
+
+
+def _tangent_calls(x, w, plain):
+    """Calls with a tangent in one of their arguments; `plain`: one without."""
+    return [lambda: ops.dropout(x, 0.5, 1), lambda: ops.dropout_(x, 0.5, 1), lambda: ops.add_rms_norm(x), lambda: ops.add_rms_norm(plain, w),
+            lambda: ops.add_rms_norm(plain, None, x), lambda: ops.add_rms_norm_f8(x), lambda: ops.add_rms_norm_f8(plain, w),
+            lambda: ops.add_rms_norm_f8(plain, None, x), lambda: ops.encode_f8(x), lambda: ops.encode_weight_f8(x),
+            lambda: ops.product_f8(plain, x, plain, plain)]
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_forward_mode_tangents_are_refused(no_grad):
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(not no_grad):
+        x, w = (torch.autograd.forward_ad.make_dual(torch.ones(*s), torch.ones(*s)) for s in ((4, 16), (16,)))
+        for call in _tangent_calls(x, w, torch.ones(4, 16)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
