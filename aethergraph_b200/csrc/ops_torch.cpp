@@ -4,6 +4,7 @@
 // spends 120 us of host time written in Python, most of it in the autograd engine's thread.
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -34,7 +35,13 @@ int tag_of(at::ScalarType t) {
 
 std::string say(const Tensor &t) { return t.defined() ? c10::str(t.sizes(), " ", t.scalar_type(), " on ", t.device()) : "nothing"; }
 
+// A traced program would keep this call's results as constants: nothing here goes through PyTorch's dispatcher.
+void no_trace(const char *what) {
+    if (torch::jit::tracer::isTracing()) throw std::runtime_error(c10::str(what, " cannot be traced by torch.jit.trace"));
+}
+
 int check_rows(const Tensor &x, const char *what) {
+    no_trace("a row operator");
     if (!x.is_cuda()) refuse(what, " must be a CUDA tensor");
     const int tag = tag_of(x.scalar_type());
     if (tag < 0) refuse(what, " must be float32, float16 or bfloat16, got ", x.scalar_type());
@@ -322,6 +329,7 @@ void check_f8(const Tensor &codes, const Tensor &scales, const char *what, int64
 struct Held { const void *codes; const float *scales; int64_t rows, dim, pitch; int device; };
 
 Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &ids, const MaybeTensor &bias, at::ScalarType dtype) {
+    no_trace("a product of 8-bit rows");
     no_tangent("a product of 8-bit rows", {&weight_scales});
     no_gradient("a product of 8-bit rows", {ptr(bias)});
     check_f8(weight, weight_scales, "weight", kF8Block);
@@ -353,6 +361,7 @@ Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scal
 
 Tensor product_f8(const Tensor &codes, const Tensor &scales, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &ids, const MaybeTensor &bias,
                   at::ScalarType dtype) {
+    no_trace("a product of 8-bit rows");
     no_tangent("a product of 8-bit rows", {&scales});
     check_f8(codes, scales, "codes", 1);
     return product({codes.data_ptr(), scales.data_ptr<float>(), codes.size(0), codes.size(1), codes.stride(0), (int)codes.get_device()}, weight, weight_scales,

@@ -11,6 +11,7 @@ wait for nothing and may be captured into a CUDA graph (a backward pass, as with
 only while no autograd graph of the same leaves made on another stream is alive).  `dropout`
 and `add_rms_norm` have gradients (reverse mode, once: a backward pass with create_graph=True is refused, and so
 are inputs with a forward-mode tangent); the 8-bit operators are for inference and have none.
+torch.jit.trace is refused: it would keep a call's results as constants.
 
 8-bit rows are a pair (codes, scales): torch.float8_e4m3fn codes [rows, dim], whose row pitch
 is a multiple of 16 bytes, and float32 scales [rows, ceil(dim / 128)], value = code * scale.

@@ -160,3 +160,11 @@ def test_forward_mode_tangents_are_refused(no_grad):
         for call in _tangent_calls(x, w, torch.ones(4, 16)):
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
+
+
+def test_tracing_is_refused():
+    x = torch.ones(4, 16)
+    for call in (lambda v: ops.dropout(v, 0.5, 1), lambda v: ops.dropout_(v, 0.5, 1), lambda v: ops.add_rms_norm(v)[0], lambda v: ops.add_rms_norm_f8(v)[0],
+                 lambda v: ops.encode_f8(v)[0], lambda v: ops.encode_weight_f8(v)[0], lambda v: ops.product_f8(v, v, v, v)):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, x, check_trace=False)
