@@ -934,6 +934,8 @@ extern "C" int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64
     if (rows == 0) return AG_OK;
     if (!x || !y) return fail(AG_ERR_VALUE, "ag_rows_dropout: null argument");
     if (y_stride < dim) return fail(AG_ERR_VALUE, "ag_rows_dropout: rows of the output overlap");
+    if (x == y && x_stride != y_stride && rows > 1)  // a row would be written over another that is still to be read
+        return fail(AG_ERR_VALUE, "ag_rows_dropout: in place, both pitches are the same: got %llu and %llu", (unsigned long long)x_stride, (unsigned long long)y_stride);
     DeviceGuard guard(device);
     if (!guard.ok) return AG_ERR_CUDA;
     const Divide by((uint32_t)((dim + kChunk - 1) / kChunk));

@@ -692,7 +692,7 @@ void ag_hetero_loader_free(ag_hetero_loader *l);
  * Philox4x32-10 with the counter (c / 8, r, offset's lower, upper 32 bits) and the key `seed`:
  * of the four words the one numbered (c % 8) / 2, its lower half for even c.  The mask is a
  * function of (seed, offset, r, c): it is never stored, and the gradient of a dropout is the
- * same call on the gradient.  x == y is allowed.  At most 0xF0000000 rows. */
+ * same call on the gradient.  x == y with the same pitch is allowed, no other overlap.  At most 0xF0000000 rows. */
 int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64_t dim, uint64_t x_stride,
                         uint64_t y_stride, int32_t dtype, double p, uint64_t seed, uint64_t offset,
                         int32_t device, void *stream);

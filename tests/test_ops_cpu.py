@@ -168,3 +168,10 @@ def test_tracing_is_refused():
                  lambda v: ops.encode_f8(v)[0], lambda v: ops.encode_weight_f8(v)[0], lambda v: ops.product_f8(v, v, v, v)):
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(call, x, check_trace=False)
+
+
+@pytest.mark.parametrize("p", [0.0, 0.5])
+def test_dropout_in_place_keeps_its_pitch(p):
+    for strides in ((16, 8), (8, 16), (0, 8)):
+        with pytest.raises(ValueError, match="in place"):
+            _lib.check(_lib.lib().ag_rows_dropout(256, 256, 4, 8, *strides, 0, p, 1, 0, 0, None))
