@@ -116,7 +116,7 @@ class NormGrad(C.Structure):
 class Product(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("codes", "scales", "weight", "weight_scales", "ids", "bias", "out")] + \
                [(n, C.c_uint64) for n in ("rows", "held", "dim", "out_dim", "code_stride", "weight_stride", "out_stride")] + \
-               [("ids_are_i64", C.c_int32), ("out_dtype", C.c_int32)]
+               [("ids_are_i64", C.c_int32), ("out_dtype", C.c_int32), ("store", C.c_void_p)]
 
 
 _P = C.c_void_p

@@ -1425,11 +1425,10 @@ extern "C" int32_t ag_features_check(const ag_features *f) {
     if (!f) return fail(AG_ERR_VALUE, "ag_features_check: null store");
     DeviceGuard guard(f->device);
     if (!guard.ok) return AG_ERR_CUDA;
-    uint32_t h = 0;
-    AG_CUDA(cudaDeviceSynchronize());
-    AG_CUDA(cudaMemcpy(&h, f->err, 4, cudaMemcpyDeviceToHost));
-    if (h) {
-        cudaMemset(f->err, 0, 4);
+    uint32_t bits = 0;
+    AG_TRY(take_error(f->err, &bits));
+    if (bits == kErrSpinTimeout) return fail(AG_ERR_CUDA, "a gather or product of the store gave up waiting; its output is incomplete");
+    if (bits) {
         return fail(AG_ERR_VALUE, "a gathered node id is out of bounds (num_nodes=%llu)", (unsigned long long)f->num_nodes);
     }
     return AG_OK;

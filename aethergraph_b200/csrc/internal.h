@@ -190,6 +190,8 @@ cudaError_t launch_encode_i8(const float *src, uint64_t rows, uint64_t dim, int8
 // f32 rows -> e4m3 codes at a pitch of row_pitch bytes + scales; *bad_dev is set when a value is not finite.
 cudaError_t launch_encode_f8(const float *src, uint64_t rows, uint64_t dim, uint64_t pitch, uint8_t *codes, float *scales,
                              uint32_t *bad_dev, cudaStream_t st);
+// Waits for the current device, reads the sticky error word and clears the bits it gives.
+int32_t take_error(uint32_t *word, uint32_t *bits);
 int gather_grid_blocks(uint64_t n, uint32_t row_bytes);
 void sampler_set_pipelined(ag_sampler *s);  // other chains run beside this handle's: it gathers on a stream of its own
 int32_t sampler_set_yielding_wait(ag_sampler *s, bool on);  // poll + yield instead of spinning in ag_sample_group_wait

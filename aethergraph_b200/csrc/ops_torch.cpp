@@ -325,8 +325,8 @@ void check_f8(const Tensor &codes, const Tensor &scales, const char *what, int64
         refuse(what, "' scales must be contiguous float32 [", want, ", ", blocks_of(dim), "] on ", codes.device());
 }
 
-// Where 8-bit rows lie: a pair of tensors, or a feature store's own memory.
-struct Held { const void *codes; const float *scales; int64_t rows, dim, pitch; int device; };
+// Where 8-bit rows lie: a pair of tensors, or a feature store.
+struct Held { const void *codes; const float *scales; int64_t rows, dim, pitch; int device; const ag_features *store; };
 
 Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &ids, const MaybeTensor &bias, at::ScalarType dtype) {
     no_trace("a product of 8-bit rows");
@@ -340,7 +340,7 @@ Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scal
     p.out_dtype = tag_of(dtype);
     if (p.out_dtype < 0) refuse("dtype must be float32, float16 or bfloat16, got ", dtype);
     p.codes = held.codes; p.scales = held.scales; p.weight = weight.data_ptr(); p.weight_scales = weight_scales.data_ptr<float>();
-    p.rows = p.held = held.rows; p.dim = held.dim; p.out_dim = out_dim; p.code_stride = held.pitch; p.weight_stride = weight.stride(0); p.out_stride = out_dim;
+    p.rows = p.held = held.rows; p.dim = held.dim; p.out_dim = out_dim; p.code_stride = held.pitch; p.store = held.store; p.weight_stride = weight.stride(0); p.out_stride = out_dim;
     if (has(ids)) {
         if (!ids->is_cuda() || ids->get_device() != held.device || ids->dim() != 1 || !ids->is_contiguous() ||
             (ids->scalar_type() != at::kLong && ids->scalar_type() != at::kInt))
@@ -364,20 +364,18 @@ Tensor product_f8(const Tensor &codes, const Tensor &scales, const Tensor &weigh
     no_trace("a product of 8-bit rows");
     no_tangent("a product of 8-bit rows", {&scales});
     check_f8(codes, scales, "codes", 1);
-    return product({codes.data_ptr(), scales.data_ptr<float>(), codes.size(0), codes.size(1), codes.stride(0), (int)codes.get_device()}, weight, weight_scales,
+    return product({codes.data_ptr(), scales.data_ptr<float>(), codes.size(0), codes.size(1), codes.stride(0), (int)codes.get_device(), nullptr}, weight, weight_scales,
                    ids, bias, dtype);
 }
 
 // `store`: an ag_features handle of 8-bit float rows.
 Tensor project(uintptr_t store, const Tensor &ids, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &bias, at::ScalarType dtype) {
     const ag_features *f = (const ag_features *)store;
-    Held h{};
-    uint64_t rows = 0, dim = 0, pitch = 0;
-    int32_t device = 0;
-    check(ag_features_f8_rows(f, &h.codes, &h.scales, &pitch));
-    check(ag_features_info(f, &rows, &dim, nullptr, &device, nullptr));
-    h.rows = rows; h.dim = dim; h.pitch = pitch; h.device = device;
-    return product(h, weight, weight_scales, ids, bias, dtype);
+    uint64_t rows = 0, dim = 0;
+    int32_t device = 0, kind = 0;
+    check(ag_features_info(f, &rows, &dim, &kind, &device, nullptr));
+    if (kind != AG_F8) refuse("the store does not hold 8-bit float rows");
+    return product({nullptr, nullptr, (int64_t)rows, (int64_t)dim, 0, device, f}, weight, weight_scales, ids, bias, dtype);
 }
 
 }  // namespace

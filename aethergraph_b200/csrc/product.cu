@@ -16,7 +16,7 @@ namespace ag {
 
 namespace {
 
-__device__ uint32_t g_rows_error;  // sticky error bits of this device's products (ag_rows_check)
+__device__ uint32_t g_rows_error;  // sticky error bits of this device's products that are no store's (ag_rows_check)
 
 struct ProductArgs {
     const uint8_t *codes, *weight;
@@ -24,17 +24,20 @@ struct ProductArgs {
     const void *ids;
     const float *bias;
     void *out;
+    uint32_t *error;  // the store's sticky error bits, or null
     uint64_t rows, held, code_stride, weight_stride, out_stride;
     uint32_t dim, out_dim, blocks;  // blocks: of 128 columns
     int ids64, out_dtype;
 };
+
+__device__ __forceinline__ void raise(const ProductArgs &a, uint32_t bits) { atomicOr(a.error ? a.error : &g_rows_error, bits); }
 
 // Row of the codes that output row m takes; `held` where its id names none.
 __device__ __forceinline__ uint64_t source_row(const ProductArgs &a, uint64_t m) {
     if (!a.ids) return m;
     const uint64_t id = a.ids64 ? (uint64_t)((const int64_t *)a.ids)[m] : (uint64_t)((const uint32_t *)a.ids)[m];
     if (id < a.held) return id;
-    atomicOr(&g_rows_error, kErrBadId);
+    raise(a, kErrBadId);
     return a.held;
 }
 
@@ -158,7 +161,7 @@ __device__ __forceinline__ bool mbar_try_once(uint32_t bar, uint32_t parity) {
 }
 // Waits for the barrier's phase; false when the block is dead or the time ran out (which marks it dead).
 // The clock is looked at now and then only.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *dead) {
+__device__ __forceinline__ bool mbar_wait(const ProductArgs &a, uint32_t bar, uint32_t parity, volatile uint32_t *dead) {
     if (mbar_try(bar, parity)) return true;
     const long long since = clock64();
     for (uint32_t i = 1;; ++i) {
@@ -167,7 +170,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         if (*dead) return false;
         if (clock64() - since > kWaitLimit) {
             *dead = 1;
-            atomicOr(&g_rows_error, kErrSpinTimeout);
+            raise(a, kErrSpinTimeout);
             return false;
         }
     }
@@ -364,7 +367,7 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     mine[lane + i * 32] = id[i] < a.held ? (uint32_t)id[i] : 0;
-                    if (id[i] >= a.held && m0 + first + lane + i * 32 < a.rows) atomicOr(&g_rows_error, kErrBadId);
+                    if (id[i] >= a.held && m0 + first + lane + i * 32 < a.rows) raise(a, kErrBadId);
                 }
                 __syncwarp();
                 load_ids(tile + gridDim.x);  // a tile ahead
@@ -373,7 +376,7 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             }
             for (uint32_t k = 0; k < steps; ++k, ++issued) {
                 const uint32_t s = issued % kStages;
-                alive = __all_sync(0xffffffffu, mbar_wait(empty + 8 * s, (issued / kStages & 1) ^ 1, dead));
+                alive = __all_sync(0xffffffffu, mbar_wait(a, empty + 8 * s, (issued / kStages & 1) ^ 1, dead));
                 if (!alive) break;
                 const uint32_t at = shared_at + s * stage_bytes(BN);
                 if (warp == 0 && elect_one()) {
@@ -413,7 +416,7 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         for (uint32_t n = warp >> 1; n < total; n += 2) {
             const uint32_t s = n % kStages, c = n % kAccStages;
             if (!__all_sync(0xffffffffu, ready)) {
-                alive = __all_sync(0xffffffffu, mbar_wait(acc_empty + 8 * c, (n / kAccStages & 1) ^ 1, dead) && mbar_wait(full + 8 * s, n / kStages & 1, dead));
+                alive = __all_sync(0xffffffffu, mbar_wait(a, acc_empty + 8 * c, (n / kAccStages & 1) ^ 1, dead) && mbar_wait(a, full + 8 * s, n / kStages & 1, dead));
                 if (!alive) break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -495,7 +498,7 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     if (k0 + j >= steps) break;
                     const uint32_t c = n % kAccStages;
                     if (!__all_sync(0xffffffffu, ready)) {
-                        alive = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * c, n / kAccStages & 1, dead));
+                        alive = __all_sync(0xffffffffu, mbar_wait(a, acc_full + 8 * c, n / kAccStages & 1, dead));
                         if (!alive) break;
                     }
                     ++n;
@@ -604,8 +607,17 @@ template <typename T> int32_t launch_tile(const ProductArgs &a, cudaStream_t st)
 
 using namespace ag;
 
-extern "C" int32_t ag_rows_product(const ag_product *p, int32_t device, void *stream) {
-    if (!p) return fail(AG_ERR_VALUE, "ag_rows_product: null argument");
+extern "C" int32_t ag_rows_product(const ag_product *call, int32_t device, void *stream) {
+    if (!call) return fail(AG_ERR_VALUE, "ag_rows_product: null argument");
+    ag_product own = *call;
+    ag_product *p = &own;
+    if (const ag_features *f = p->store) {
+        if (f->dtype != AG_F8) return fail(AG_ERR_VALUE, "ag_rows_product: the store does not hold 8-bit float rows");
+        if (f->device != device) return fail(AG_ERR_VALUE, "ag_rows_product: the store is on device %d, the call on %d", f->device, device);
+        if (p->codes || p->scales) return fail(AG_ERR_VALUE, "ag_rows_product: either a store or rows");
+        p->codes = f->payload; p->scales = f->scales; p->held = f->rows; p->code_stride = f->pitch;
+        if (f->dim != p->dim) return fail(AG_ERR_VALUE, "ag_rows_product: rows of %llu columns, weights of %llu", (unsigned long long)f->dim, (unsigned long long)p->dim);
+    }
     if (p->out_dtype < AG_F32 || p->out_dtype > AG_BF16) return fail(AG_ERR_VALUE, "ag_rows_product: the output is f32, f16 or bf16, got dtype tag %d", p->out_dtype);
     if (p->dim == 0 || p->dim > 0x7FFFFF00ull || p->code_stride > 0xFFFFFFF0ull || p->out_dim == 0 || p->out_dim >= (1ull << 31) || p->held >= (1ull << 31) || p->rows >= (1ull << 31))
         return fail(AG_ERR_VALUE, "ag_rows_product: %llu rows of %llu x %llu from %llu held rows are out of range", (unsigned long long)p->rows,
@@ -622,7 +634,7 @@ extern "C" int32_t ag_rows_product(const ag_product *p, int32_t device, void *st
     if (!guard.ok) return AG_ERR_CUDA;
     ProductArgs a{};
     a.codes = (const uint8_t *)p->codes; a.weight = (const uint8_t *)p->weight; a.scales = p->scales; a.weight_scales = p->weight_scales;
-    a.ids = p->ids; a.bias = p->bias; a.out = p->out; a.rows = p->rows; a.held = p->ids ? p->held : (1ull << 31);
+    a.ids = p->ids; a.bias = p->bias; a.out = p->out; a.error = p->store ? p->store->err : nullptr; a.rows = p->rows; a.held = p->ids ? p->held : (1ull << 31);
     a.code_stride = p->code_stride; a.weight_stride = p->weight_stride; a.out_stride = p->out_stride;
     a.dim = (uint32_t)p->dim; a.out_dim = (uint32_t)p->out_dim; a.blocks = (uint32_t)((p->dim + kF8Block - 1) / kF8Block);
     a.ids64 = p->ids_are_i64; a.out_dtype = p->out_dtype;
@@ -641,15 +653,32 @@ extern "C" int32_t ag_rows_product(const ag_product *p, int32_t device, void *st
     return AG_OK;
 }
 
+namespace ag {
+namespace {
+__global__ void k_clear_bits(uint32_t *word, uint32_t bits) { atomicAnd(word, ~bits); }
+}  // namespace
+
+// A run-out wait comes first and alone, the rest stays for the next call; only what is reported is cleared, so that
+// what other streams raise meanwhile is kept.
+int32_t take_error(uint32_t *word, uint32_t *bits) {
+    AG_CUDA(cudaDeviceSynchronize());
+    AG_CUDA(cudaMemcpy(bits, word, 4, cudaMemcpyDeviceToHost));
+    if (*bits & kErrSpinTimeout) *bits = kErrSpinTimeout;
+    if (*bits) {
+        k_clear_bits<<<1, 1>>>(word, *bits);
+        AG_CUDA(cudaGetLastError());
+        AG_CUDA(cudaStreamSynchronize(nullptr));
+    }
+    return AG_OK;
+}
+}  // namespace ag
+
 extern "C" int32_t ag_rows_check(int32_t device) {
     DeviceGuard guard(device);
     if (!guard.ok) return AG_ERR_CUDA;
-    uint32_t h = 0;
-    AG_CUDA(cudaDeviceSynchronize());
-    AG_CUDA(cudaMemcpyFromSymbol(&h, g_rows_error, 4));
-    if (!h) return AG_OK;
-    const uint32_t zero = 0;
-    AG_CUDA(cudaMemcpyToSymbol(g_rows_error, &zero, 4));
-    if (h & kErrSpinTimeout) return fail(AG_ERR_CUDA, "a product gave up waiting for its loads or multiplications; its output is incomplete");
-    return fail(AG_ERR_VALUE, "a row id of a product is out of bounds");
+    uint32_t *word = nullptr, bits = 0;
+    AG_CUDA(cudaGetSymbolAddress((void **)&word, g_rows_error));
+    AG_TRY(take_error(word, &bits));
+    if (bits == kErrSpinTimeout) return fail(AG_ERR_CUDA, "a product gave up waiting for its loads or multiplications; its output is incomplete");
+    return bits ? fail(AG_ERR_VALUE, "a row id of a product is out of bounds") : AG_OK;
 }

@@ -290,11 +290,9 @@ class FeatureStore:
         return n.value
 
     def check(self) -> None:
-        """Raise ValueError if a device gather (or, on the store's GPU, a product) since the last check saw
-        an out-of-range id."""
+        """Raise ValueError if a device gather or a product of this store since the last check saw an
+        out-of-range id."""
         _lib.check(_lib.lib().ag_features_check(self._h))
-        if self._dtype == _lib.AG_F8:
-            _lib.check(_lib.lib().ag_rows_check(self._device))
 
     def telemetry(self):
         return None

@@ -110,5 +110,6 @@ def product_f8(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, 
 
 
 def check(device: int | None = None) -> None:
-    """Raise ValueError if a product since the last check saw an id outside its rows (waits for the device)."""
+    """Raise ValueError if a `product_f8` on the device since the last check saw an id outside its rows (waits for the
+    device).  A store's products are checked by the store."""
     _lib.check(_lib.lib().ag_rows_check(torch.cuda.current_device() if device is None else int(device)))

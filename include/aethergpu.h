@@ -752,7 +752,8 @@ int32_t ag_rows_encode_weight(const void *w, uint64_t out, uint64_t dim, uint64_
  * bias[n] (f32, may be NULL), in f32, rounded once to out_dtype (f32, f16, bf16).  i = m, or
  * ids[m] (int64, or u32 ids where ids_are_i64 == 0): the rows of a feature store by id.  An id
  * outside [0, held) gives a zero row and raises a sticky error that ag_rows_check reports, per
- * device.  held, out_dim < 2^31. */
+ * device.  held, out_dim < 2^31.  With `store`, a store of 8-bit float rows, codes, scales, held and
+ * code_stride are the store's, and so is the error (ag_features_check). */
 typedef struct {
     const void *codes;
     const float *scales;
@@ -763,10 +764,11 @@ typedef struct {
     void *out;
     uint64_t rows, held, dim, out_dim, code_stride, weight_stride, out_stride;
     int32_t ids_are_i64, out_dtype;
+    const ag_features *store;
 } ag_product;
 int32_t ag_rows_product(const ag_product *p, int32_t device, void *stream);
-/* AG_ERR_VALUE if any product since the last check saw an id outside its rows
- * (synchronises the device). */
+/* AG_ERR_VALUE if any product without a store since the last check saw an id outside its rows,
+ * AG_ERR_CUDA if one gave up waiting (synchronises the device).  What is reported is cleared. */
 int32_t ag_rows_check(int32_t device);
 
 /* ------------------------------------------------------ synthetic inputs --
