@@ -5,6 +5,7 @@ local edge index, and the feature-row gather with fused f16/bf16 -> f32 upcast,
 as hand-written CUDA kernels (sm_100a) behind a C ABI (include/aethergpu.h) and
 the reference's Python sampler / feature-store / loader surface.
 """
+from . import ops
 from ._lib import GraphLoadError, SamplingError, release_kept_memory
 from .features import FeatureStore, save_features
 from .graph import CsrGraph, Graph, partition_aligned_batches
@@ -14,14 +15,6 @@ from .hetero import (HeteroCsrGraph, HeteroNeighborLoader, HeteroNeighborSampler
 from .sampler import NeighborSampler, ParallelBatchSampler, SampledSubgraph, Sampler, SamplingConfig
 
 __version__ = "0.1.0"
-
-
-def __getattr__(name):
-    if name == "ops":  # needs torch, which the rest of the package imports only where it is used
-        import importlib
-
-        return importlib.import_module(".ops", __name__)
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 __all__ = [
     "CsrGraph", "FeatureStore", "Graph", "GraphLoadError", "HeteroCsrGraph", "HeteroNeighborLoader",

@@ -18,6 +18,7 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using MaybeTensor = std::optional<Tensor>;
+using MaybeType = std::optional<at::ScalarType>;
 
 constexpr int64_t kF8Block = 128;  // columns per scale
 
@@ -328,7 +329,8 @@ void check_f8(const Tensor &codes, const Tensor &scales, const char *what, int64
 // Where 8-bit rows lie: a pair of tensors, or a feature store.
 struct Held { const void *codes; const float *scales; int64_t rows, dim, pitch; int device; const ag_features *store; };
 
-Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &ids, const MaybeTensor &bias, at::ScalarType dtype) {
+Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &ids, const MaybeTensor &bias, MaybeType type) {
+    const at::ScalarType dtype = type.value_or(at::kBFloat16);
     no_trace("a product of 8-bit rows");
     no_tangent("a product of 8-bit rows", {&weight_scales});
     no_gradient("a product of 8-bit rows", {ptr(bias)});
@@ -360,7 +362,7 @@ Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scal
 }
 
 Tensor product_f8(const Tensor &codes, const Tensor &scales, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &ids, const MaybeTensor &bias,
-                  at::ScalarType dtype) {
+                  MaybeType dtype) {
     no_trace("a product of 8-bit rows");
     no_tangent("a product of 8-bit rows", {&scales});
     check_f8(codes, scales, "codes", 1);
@@ -369,7 +371,7 @@ Tensor product_f8(const Tensor &codes, const Tensor &scales, const Tensor &weigh
 }
 
 // `store`: an ag_features handle of 8-bit float rows.
-Tensor project(uintptr_t store, const Tensor &ids, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &bias, at::ScalarType dtype) {
+Tensor project(uintptr_t store, const Tensor &ids, const Tensor &weight, const Tensor &weight_scales, const MaybeTensor &bias, MaybeType dtype) {
     const ag_features *f = (const ag_features *)store;
     uint64_t rows = 0, dim = 0;
     int32_t device = 0, kind = 0;

@@ -132,7 +132,7 @@ class FeatureStore:
 
         from . import ops
 
-        ops._ops.check_f8(codes, scales, "codes", 1)
+        ops._native().check_f8(codes, scales, "codes", 1)
         torch.cuda.current_stream(codes.device).synchronize()
         out = C.c_void_p()
         _lib.check(_lib.lib().ag_features_from_f8(codes.data_ptr() or None, scales.data_ptr() or None, codes.shape[0], codes.shape[1],
@@ -250,11 +250,9 @@ class FeatureStore:
         computes, without writing the decoded rows: a kernel reads the stored codes by id and multiplies
         them.  `ids` is a CUDA tensor (int64, or int32 holding u32 ids); one outside the store gives a
         zero row and an error that `check` raises."""
-        import torch
-
         from . import ops
 
-        return ops._ops.project(self._h.value, ids, weight, weight_scales, bias, torch.bfloat16 if dtype is None else dtype)
+        return ops._native().project(self._h.value, ids, weight, weight_scales, bias, dtype)
 
     def gather_stats(self) -> tuple[int, int, int]:
         """Sharded views: `(rows requested, rows loaded, rows loaded from the local copy of

@@ -19,19 +19,33 @@ is a multiple of 16 bytes, and float32 scales [rows, ceil(dim / 128)], value = c
 rows under the dtype "f8".
 
 The functions are those of `_ops` (csrc/ops_torch.cpp), which calls the kernels through the C
-ABI; like the rest of the package there is no fallback without it.
+ABI; like the rest of the package there is no fallback without it.  It is loaded, and torch with it, by the
+first call.
 """
 from __future__ import annotations
 
-import torch
+from typing import TYPE_CHECKING
 
 from . import _lib
 
-_lib.lib()  # said in the package's own words if it was never built
-from . import _ops  # noqa: E402  (needs torch and the library above)
+if TYPE_CHECKING:
+    import torch
 
 __all__ = ["add_rms_norm", "add_rms_norm_f8", "check", "decode_f8", "dropout", "dropout_", "encode_f8", "encode_weight_f8",
            "product_f8"]
+
+
+_loaded = None
+
+
+def _native():
+    global _loaded
+    if _loaded is None:
+        _lib.lib()  # said in the package's own words if it was never built
+        import torch  # noqa: F401  (the extension needs its libraries)
+
+        from . import _ops as _loaded
+    return _loaded
 
 
 def _check_key(seed: int, offset: int) -> None:
@@ -47,13 +61,13 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0) -> torch.Tens
     call, for every type and layout; give every use in a program an `offset` of its own.  The gradient makes the mask again
     instead of storing it.  A dropped element is 0 even where `x` is infinite or NaN."""
     _check_key(seed, offset)
-    return _ops.dropout(x, p, seed, offset)
+    return _native().dropout(x, p, seed, offset)
 
 
 def dropout_(x: torch.Tensor, p: float, seed: int, offset: int = 0) -> torch.Tensor:
     """`dropout` in place, for rows that no gradient is asked of (a batch's own `x`)."""
     _check_key(seed, offset)
-    _ops.dropout_(x, p, seed, offset)
+    _native().dropout_(x, p, seed, offset)
     return x
 
 
@@ -68,30 +82,32 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: 
     inputs: changed in place meanwhile, the backward pass is refused), for float32 h.
     `p`, `seed` and `offset` are `dropout`'s."""
     _check_key(seed, offset)
-    return _ops.add_rms_norm(x, weight, residual, eps, p, seed, offset)
+    return _native().add_rms_norm(x, weight, residual, eps, p, seed, offset)
 
 
 def add_rms_norm_f8(x: torch.Tensor, weight: torch.Tensor | None = None, residual: torch.Tensor | None = None, *,
                     eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(codes, scales, h): `add_rms_norm` with y as 8-bit rows, encoded where it is computed.  For
     inference: no dropout, no gradient."""
-    return _ops.add_rms_norm_f8(x, weight, residual, eps)
+    return _native().add_rms_norm_f8(x, weight, residual, eps)
 
 
 def encode_f8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales): rows, of at most 16384 columns, in 8 bits.  A block's scale puts its largest magnitude on 448; a block
     that holds an infinity or NaN reads as NaN throughout."""
-    return _ops.encode_f8(x)
+    return _native().encode_f8(x)
 
 
 def encode_weight_f8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """(codes, scales) of weights [out, dim]: one scale per 128 x 128 block, float32
     [ceil(out / 128), ceil(dim / 128)]."""
-    return _ops.encode_weight_f8(w)
+    return _native().encode_weight_f8(w)
 
 
 def decode_f8(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """8-bit rows as float32 [rows, dim] (exact: code * scale, one multiplication)."""
+    import torch
+
     from .features import FeatureStore
 
     store = FeatureStore.from_f8(codes, scales)
@@ -100,16 +116,18 @@ def decode_f8(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 def product_f8(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, *,
                ids: torch.Tensor | None = None, bias: torch.Tensor | None = None,
-               dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """rows @ weight.T + bias of 8-bit rows and 8-bit weights, [rows, out] in `dtype`.
+               dtype: torch.dtype | None = None) -> torch.Tensor:
+    """rows @ weight.T + bias of 8-bit rows and 8-bit weights, [rows, out] in `dtype` (bfloat16 by default).
 
     With `ids` (int64, or int32 holding u32 ids) output row i is that of 8-bit row ids[i]; an id outside them
     gives a zero row and an error that `check` raises.  Every block of 128 columns is summed,
     multiplied by its two scales and added up in float32.  `bias` is float32 [out]."""
-    return _ops.product_f8(codes, scales, weight, weight_scales, ids, bias, dtype)
+    return _native().product_f8(codes, scales, weight, weight_scales, ids, bias, dtype)
 
 
 def check(device: int | None = None) -> None:
     """Raise ValueError if a `product_f8` on the device since the last check saw an id outside its rows (waits for the
     device).  A store's products are checked by the store."""
+    import torch
+
     _lib.check(_lib.lib().ag_rows_check(torch.cuda.current_device() if device is None else int(device)))

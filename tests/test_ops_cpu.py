@@ -1,5 +1,8 @@
 """Row operators without a GPU: the random bits' definition, refusals before anything is launched."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -175,3 +178,15 @@ def test_dropout_in_place_keeps_its_pitch(p):
     for strides in ((16, 8), (8, 16), (0, 8)):
         with pytest.raises(ValueError, match="in place"):
             _lib.check(_lib.lib().ag_rows_dropout(256, 256, 4, 8, *strides, 0, p, 1, 0, 0, None))
+
+
+def test_the_package_needs_no_torch_until_it_is_used():
+    """A star import, `ops` among its names, without torch and without the extension; the first call asks for both."""
+    code = ("import sys; sys.modules['torch'] = None; sys.modules['aethergraph_b200._ops'] = None\n"
+            "from aethergraph_b200 import *\n"
+            "import aethergraph_b200 as ag\n"
+            "assert ops is ag.ops and Graph is ag.Graph\n"
+            "try: ops.dropout(None, 0.5, 1)\n"
+            "except ImportError: print('asked')\n")
+    got = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True)
+    assert got.returncode == 0 and got.stdout.strip() == "asked", got.stderr
