@@ -18,6 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaethergpu.so")
 OPS = os.path.join(HERE, "_ops.so")
+OPS_TORCH = os.path.join(HERE, "_ops.torch")  # the PyTorch that _ops.so was built against
 SOURCES = ["api.cu", "gather.cu", "sampler.cu", "synth.cu", "loader.cu", "noalloc.cu", "hetero.cu", "hop.cu", "shard.cu",
            "hetero_loader.cu", "rewrite.cu", "hot.cu", "peer_block.cu", "reorder.cu", "workspace.cu",
            "rows.cu", "product.cu"]
@@ -34,8 +35,17 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found; libaethergpu.so cannot be built")
 
 
+def _torch_version() -> str:
+    """Without importing it."""
+    from importlib.metadata import version
+
+    return version("torch")
+
+
 def _stale() -> bool:
     if not os.path.exists(LIB) or not os.path.exists(OPS):
+        return True
+    if not os.path.exists(OPS_TORCH) or open(OPS_TORCH).read() != _torch_version():
         return True
     t = min(os.path.getmtime(LIB), os.path.getmtime(OPS))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
@@ -96,6 +106,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError("_ops.so: compilation failed\n" + r.stdout.decode(errors="replace")[-4000:])
     os.replace(OPS + ".tmp", OPS)
+    with open(OPS_TORCH, "w") as f:
+        f.write(_torch_version())
     return LIB
 
 
