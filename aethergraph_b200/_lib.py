@@ -233,6 +233,7 @@ SIGNATURES = {
     "ag_rows_norm_backward_scratch": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, _U64P]),
     "ag_rows_norm_backward": (C.c_int32, [_P, C.c_int32, _P]),
     "ag_rows_encode_weight": (C.c_int32, [_P, C.c_uint64, C.c_uint64, C.c_uint64, C.c_int32, _P, C.c_uint64, _P, C.c_int32, _P]),
+    "ag_rows_decode": (C.c_int32, [_P, _P, C.c_uint64, C.c_uint64, C.c_uint64, _P, C.c_int32, _P]),
     "ag_rows_product": (C.c_int32, [_P, C.c_int32, _P]),
     "ag_rows_check": (C.c_int32, [C.c_int32]),
     "ag_synth_rmat_graph": (C.c_int32, [C.c_uint64, C.c_uint64, C.c_float, C.c_float, C.c_float, C.c_uint64,

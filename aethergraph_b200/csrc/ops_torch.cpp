@@ -326,6 +326,16 @@ void check_f8(const Tensor &codes, const Tensor &scales, const char *what, int64
         refuse(what, "' scales must be contiguous float32 [", want, ", ", blocks_of(dim), "] on ", codes.device());
 }
 
+Tensor decode_f8(const Tensor &codes, const Tensor &scales) {
+    no_trace("decode_f8");
+    no_tangent("decode_f8", {&scales});
+    check_f8(codes, scales, "codes", 1);
+    Tensor out = fresh({codes.size(0), codes.size(1)}, at::kFloat, codes);
+    check(ag_rows_decode(codes.data_ptr(), scales.data_ptr<float>(), codes.size(0), codes.size(1), codes.stride(0), out.data_ptr<float>(), codes.get_device(),
+                         stream_of(codes)));
+    return out;
+}
+
 // Where 8-bit rows lie: a pair of tensors, or a feature store.
 struct Held { const void *codes; const float *scales; int64_t rows, dim, pitch; int device; const ag_features *store; };
 
@@ -390,6 +400,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("add_rms_norm_f8", &add_rms_norm_f8, release);
     m.def("encode_f8", &encode_f8, release);
     m.def("encode_weight_f8", &encode_weight_f8, release);
+    m.def("decode_f8", &decode_f8, release);
     m.def("check_f8", &check_f8, release);
     m.def("product_f8", &product_f8, release);
     m.def("project", &project, release);

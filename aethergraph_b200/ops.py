@@ -106,12 +106,7 @@ def encode_weight_f8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def decode_f8(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """8-bit rows as float32 [rows, dim] (exact: code * scale, one multiplication)."""
-    import torch
-
-    from .features import FeatureStore
-
-    store = FeatureStore.from_f8(codes, scales)
-    return store.gather(torch.arange(codes.shape[0], device=codes.device))
+    return _native().decode_f8(codes, scales)
 
 
 def product_f8(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor, *,

@@ -747,6 +747,9 @@ int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, void *strea
 int32_t ag_rows_encode_weight(const void *w, uint64_t out, uint64_t dim, uint64_t stride,
                               int32_t dtype, void *codes, uint64_t code_stride, float *scales,
                               int32_t device, void *stream);
+/* 8-bit rows back to f32 rows, one after the other: code * scale. */
+int32_t ag_rows_decode(const void *codes, const float *scales, uint64_t rows, uint64_t dim,
+                       uint64_t code_stride, float *out, int32_t device, void *stream);
 /* Product of 8-bit rows with 8-bit weights: out[m, n] = sum over the blocks of 128 columns of
  * scales[i, block] * weight_scales[n / 128, block] * (codes[i] . weight[n] within the block), plus
  * bias[n] (f32, may be NULL), in f32, rounded once to out_dtype (f32, f16, bf16).  i = m, or

@@ -190,3 +190,12 @@ def test_the_package_needs_no_torch_until_it_is_used():
             "except ImportError: print('asked')\n")
     got = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True)
     assert got.returncode == 0 and got.stdout.strip() == "asked", got.stderr
+
+
+def test_decode_refusals():
+    for args in ((None, 16, 4, 16, 16, 16), (16, None, 4, 16, 16, 16), (16, 16, 4, 16, 16, None), (16, 16, 4, 0, 16, 16), (16, 16, 4, 16, 24, 16), (16, 16, 4, 32, 16, 16),
+                 (8, 16, 4, 16, 16, 16), (16, 16, 4, 16, 1 << 32, 16)):
+        with pytest.raises(ValueError):
+            _lib.check(_lib.lib().ag_rows_decode(*args, 0, None))
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        ops.decode_f8(torch.zeros(4, 16), torch.zeros(4, 1))
