@@ -311,6 +311,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
                const __grid_constant__ TileArgs t) {
     constexpr int kStages = load_stages(BN, sizeof(T)), kHalf = BN / 2;
+    // A wait by parity knows a phase from the next but not from the one after: a warp that issues step n may look for
+    // it in stage n % kStages only when step n - kStages is known to have landed.  What shows that is its
+    // accumulator, drained of step n - kAccStages: steps are loaded and drained in order.
+    static_assert(kStages >= kAccStages, "the drained accumulator is of a step no older than the stage's last");
     extern __shared__ uint8_t raw_shared[];
     uint8_t *shared = (uint8_t *)(((uintptr_t)raw_shared + 1023) & ~(uintptr_t)1023);  // the swizzle's period
     uint64_t *bars = (uint64_t *)(shared + kStages * stage_bytes(BN) + out_bytes(BN, sizeof(T)));
