@@ -65,24 +65,23 @@ __device__ __forceinline__ void load_codes(const uint8_t *row, uint32_t c, uint3
     }
 }
 
-constexpr int kDotThreads = 256, kDotRows = 4;
-// Beyond this the tensor-core tiles are faster: 1024 x 1024 1, 2, 4, 8 rows 3.6, 4.2, 5.3, 5.8 us this way,
+constexpr int kDotThreads = 256;
+// Beyond this many rows the tensor-core tiles are faster: 1024 x 1024 1, 2, 4, 8 rows 3.6, 4.2, 5.3, 5.8 us this way,
 // 5.1, 5.1, 5.0, 5.2 the other; 2048 x 1024 4.8, 5.8, 7.8, 8.2 and 6.5, 6.5, 6.8, 6.8; 256 x 256 3.1, 3.2, 3.9, 3.8 and 4.0, 3.8, 3.8, 4.1.
-constexpr uint64_t kFewRows = 3;
+constexpr int kFewRows = 3;
 
-// Few rows: a warp per column of the output and up to kDotRows rows, a lane 16 codes a turn, which lie in one scale
+// Few rows: a warp per column of the output, a lane 16 codes a turn, which lie in one scale
 // block.  The weights are all there is to read; 1 x 1024 x 1024: 3.6 us, of which launch and one dependent load are most.
 __global__ void __launch_bounds__(kDotThreads)
 k_product_dot(ProductArgs a) {
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t n = blockIdx.x * (kDotThreads / 32) + (threadIdx.x >> 5);
-    const uint64_t m0 = (uint64_t)blockIdx.y * kDotRows;
     if (n >= a.out_dim) return;
-    uint64_t src[kDotRows];
-    float acc[kDotRows];
+    uint64_t src[kFewRows];
+    float acc[kFewRows];
 #pragma unroll
-    for (int r = 0; r < kDotRows; ++r) {
-        src[r] = m0 + r < a.rows ? source_row(a, m0 + r) : a.held;
+    for (int r = 0; r < kFewRows; ++r) {
+        src[r] = r < a.rows ? source_row(a, r) : a.held;
         acc[r] = 0.f;
     }
     for (uint32_t c = lane * 16; c < a.dim; c += 512) {
@@ -90,7 +89,7 @@ k_product_dot(ProductArgs a) {
         load_codes(a.weight + (uint64_t)n * a.weight_stride, c, a.dim, w);
         const float ws = a.weight_scales[(uint64_t)(n / kF8Block) * a.blocks + c / kF8Block];
 #pragma unroll
-        for (int r = 0; r < kDotRows; ++r) {
+        for (int r = 0; r < kFewRows; ++r) {
             if (src[r] == a.held) continue;
             float v[16], dot = 0.f;
             load_codes(a.codes + src[r] * a.code_stride, c, a.dim, v);
@@ -100,9 +99,9 @@ k_product_dot(ProductArgs a) {
         }
     }
 #pragma unroll
-    for (int r = 0; r < kDotRows; ++r) {
+    for (int r = 0; r < kFewRows; ++r) {
         for (int o = 16; o > 0; o /= 2) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
-        if (lane == 0 && m0 + r < a.rows) store_out(a, m0 + r, n, src[r] == a.held ? 0.f : acc[r] + (a.bias ? a.bias[n] : 0.f));
+        if (lane == 0 && r < a.rows) store_out(a, r, n, src[r] == a.held ? 0.f : acc[r] + (a.bias ? a.bias[n] : 0.f));
     }
 }
 
@@ -644,8 +643,7 @@ extern "C" int32_t ag_rows_product(const ag_product *call, int32_t device, void 
     a.ids64 = p->ids_are_i64; a.out_dtype = p->out_dtype;
     cudaStream_t st = (cudaStream_t)stream;
     if (a.rows <= kFewRows) {
-        const dim3 grid((a.out_dim + kDotThreads / 32 - 1) / (kDotThreads / 32), (uint32_t)((a.rows + kDotRows - 1) / kDotRows));
-        k_product_dot<<<grid, kDotThreads, 0, st>>>(a);
+        k_product_dot<<<(a.out_dim + kDotThreads / 32 - 1) / (kDotThreads / 32), kDotThreads, 0, st>>>(a);
     } else if (a.out_dtype == AG_F32) {
         AG_TRY(launch_tile<float>(a, st));
     } else if (a.out_dtype == AG_F16) {
