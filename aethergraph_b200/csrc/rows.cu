@@ -1012,7 +1012,7 @@ extern "C" int32_t ag_rows_norm_backward(const ag_norm_grad *n, int32_t device, 
     if (!n) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: null argument");
     AG_TRY(check_rows("ag_rows_norm_backward", n->rows, n->dim, n->dtype));
     if (n->dim > kMaxNormDim) return fail(AG_ERR_VALUE, "ag_rows_norm_backward: at most %u columns, got %llu", kMaxNormDim, (unsigned long long)n->dim);
-    if (n->weight && n->weight_dtype != n->dtype && n->weight_dtype != AG_F32)
+    if ((n->weight || n->dw) && n->weight_dtype != n->dtype && n->weight_dtype != AG_F32)
         return fail(AG_ERR_VALUE, "ag_rows_norm_backward: the weights are f32 or of the rows' type");
     AG_TRY(check_pitches("ag_rows_norm_backward", {n->dy_stride, n->dh_stride, n->h_stride, n->x_stride, n->residual_stride}));
     NormBackArgs a{};

@@ -142,7 +142,8 @@ def _norm_back(**kw):
 
 @pytest.mark.parametrize("kw,text", [
     (dict(h=None), "null"), (dict(x=16), "either"), (dict(residual=16), "either"), (dict(h=None, x=16, dtype=0), "f32"),
-    (dict(h=None, x=16, x_stride=1 << 32), "apart"), (dict(h=None, x=16, residual=16, residual_stride=1 << 32), "apart")])
+    (dict(weight=16, weight_dtype=2), "weights"),
+    (dict(dw=16, scratch=16, scratch_bytes=1 << 40, weight_dtype=3), "weights"), (dict(h=None, x=16, x_stride=1 << 32), "apart"), (dict(h=None, x=16, residual=16, residual_stride=1 << 32), "apart")])
 def test_norm_gradient_refusals(kw, text):
     with pytest.raises(ValueError, match=text):
         _lib.check(_norm_back(**kw))
