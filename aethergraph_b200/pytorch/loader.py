@@ -169,7 +169,7 @@ class FeatureDropout:
         return float(p)
 
     def __call__(self, x, batch_idx: int, node_type: int = 0):
-        if self._p == 0.0 or x is None:
+        if self._p == 0.0 or x is None or x.numel() == 0:
             return x
         from .. import ops
 

@@ -200,3 +200,14 @@ def test_decode_refusals():
             _lib.check(_lib.lib().ag_rows_decode(*args, 0, None))
     with pytest.raises(ValueError, match="CUDA tensor"):
         ops.decode_f8(torch.zeros(4, 16), torch.zeros(4, 1))
+
+
+def test_feature_dropout_of_nothing():
+    """A node type without features, without rows in this batch, or with rows of no columns."""
+    from aethergraph_b200.pytorch.loader import FeatureDropout
+
+    drop = FeatureDropout(0.5, 1)
+    assert drop(None, 0) is None
+    for shape in ((0, 8), (5, 0), (0, 0)):
+        x = torch.empty(shape)
+        assert drop(x, 0) is x
