@@ -50,11 +50,14 @@ int check_rows(const Tensor &x, const char *what) {
     return tag;
 }
 
+// The imaginary part of a conjugate keeps its values with the other sign.
+Tensor plain(const Tensor &x) { return x.is_neg() ? x.resolve_neg() : x; }
+
 // A tensor as rows of consecutive columns; copied only where it is laid out otherwise.
 struct Rows {
     Tensor t;
     int64_t rows, dim, pitch;
-    explicit Rows(const Tensor &x) : t(x), dim(x.size(-1)) {
+    explicit Rows(const Tensor &x) : t(plain(x)), dim(x.size(-1)) {
         if (!t.is_contiguous()) {
             if (t.dim() == 2 && (t.stride(1) == 1 || dim == 1) && t.stride(0) >= 0) {
                 rows = t.size(0);
@@ -160,7 +163,7 @@ struct NormCall {
             n.residual = res->t.data_ptr(); n.residual_stride = res->pitch;
         }
         if (has(weight)) {
-            w = weight->contiguous();
+            w = plain(*weight).contiguous();
             n.weight = w.data_ptr(); n.weight_dtype = tag_of(w.scalar_type());
         }
     }
@@ -237,7 +240,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
         }
         Tensor w, scratch;
         if (weight.defined()) {
-            w = weight.contiguous();
+            w = plain(weight).contiguous();
             n.weight = w.data_ptr(); n.weight_dtype = tag_of(w.scalar_type());
             if (need_w && !dy) {  // h alone was used: the weights have no part in it
                 got[1] = at::zeros_like(w);
@@ -322,7 +325,7 @@ void check_f8(const Tensor &codes, const Tensor &scales, const char *what, int64
         refuse(what, " must start on 16 bytes, with consecutive columns and a row pitch that is a multiple of 16 bytes");
     const int64_t want = (rows + rows_per_scale - 1) / rows_per_scale;
     if (!scales.is_cuda() || scales.get_device() != codes.get_device() || scales.scalar_type() != at::kFloat || scales.dim() != 2 || scales.size(0) != want ||
-        scales.size(1) != blocks_of(dim) || !scales.is_contiguous())
+        scales.size(1) != blocks_of(dim) || !scales.is_contiguous() || scales.is_neg())
         refuse(what, "' scales must be contiguous float32 [", want, ", ", blocks_of(dim), "] on ", codes.device());
 }
 
@@ -349,6 +352,7 @@ Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scal
     if (weight.get_device() != held.device || weight.size(1) != held.dim || out_dim == 0)
         refuse("weight must be [out, ", held.dim, "] on cuda:", held.device, ", got ", say(weight));
     ag_product p{};
+    Tensor plain_bias;
     p.out_dtype = tag_of(dtype);
     if (p.out_dtype < 0) refuse("dtype must be float32, float16 or bfloat16, got ", dtype);
     p.codes = held.codes; p.scales = held.scales; p.weight = weight.data_ptr(); p.weight_scales = weight_scales.data_ptr<float>();
@@ -363,7 +367,8 @@ Tensor product(const Held &held, const Tensor &weight, const Tensor &weight_scal
         if (!bias->is_cuda() || bias->get_device() != held.device || bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != out_dim ||
             !bias->is_contiguous())
             refuse("bias must be contiguous float32 [", out_dim, "] on cuda:", held.device);
-        p.bias = bias->data_ptr<float>();
+        plain_bias = plain(*bias);
+        p.bias = plain_bias.data_ptr<float>();
     }
     Tensor out = fresh({(int64_t)p.rows, out_dim}, dtype, weight);
     p.out = out.data_ptr();
