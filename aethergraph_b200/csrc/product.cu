@@ -406,8 +406,13 @@ k_product_tile(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             asm volatile("cp.async.wait_all;" ::: "memory");
             while (landed < issued) report();  // of a dead block too: the loads' barriers end
         }
-        if (!alive && warp == 0)
-            for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_drain(full + 8 * (i % kStages), i / kStages & 1);
+        // What arrives on the block's barriers by itself does so before the block ends: the last stages' commits or, where
+        // a wait has run out (here or in the warps that multiply), the loads.
+        if (warp == 0)
+            for (uint32_t i = issued > kStages ? issued - kStages : 0; i < issued; ++i) {
+                alive = alive && mbar_wait(a, empty + 8 * (i % kStages), i / kStages & 1, dead);
+                if (!alive) mbar_drain(full + 8 * (i % kStages), i / kStages & 1);
+            }
     } else if (warp & 1 && warp < 4) {
         // The whole warp walks the loop, so that addresses stay in uniform registers, and one lane issues.
         constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);  // e4m3 x e4m3 -> f32
