@@ -193,7 +193,8 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
         NormOut out = run_norm(x, weight, residual, eps, p, (uint64_t)seed, (uint64_t)offset, true);
         // 16-bit rows: not the rounded h but what it is made of, if that is not x alone
         const bool again = x.scalar_type() != at::kFloat && !out.h.is_same(x);
-        ctx->save_for_backward({again ? x : out.h, has(weight) ? *weight : Tensor(), out.rstd, again && has(residual) ? *residual : Tensor()});
+        auto kept = [](const Tensor &t) { return t.is_inference() ? t.clone() : t; };  // autograd keeps no tensor of inference mode
+        ctx->save_for_backward({again ? kept(x) : out.h, has(weight) ? *weight : Tensor(), out.rstd, again && has(residual) ? kept(*residual) : Tensor()});
         ctx->saved_data["again"] = again;
         ctx->saved_data["p"] = p;
         ctx->saved_data["seed"] = seed;

@@ -75,3 +75,15 @@ def test_what_the_gradients_are_made_of_is_watched(ops):  # noqa: F811
     want = torch.autograd.grad(ops.add_rms_norm(x, w, res, p=0.5, seed=1)[0].sum(), w)[0]
     for a, b in ((wide_x[:, 8:72], res), (x, res.t().contiguous().t()), (wide_x[:, 8:72].unflatten(0, (2, 4)), res.view(2, 4, 64))):
         assert torch.equal(torch.autograd.grad(ops.add_rms_norm(a, w, b, p=0.5, seed=1)[0].sum(), w)[0], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_inference_mode(ops, dtype):  # noqa: F811
+    """Branch or residual from a part of the model that runs in inference mode."""
+    x, w, res, _ = norm_case(8, 64, dtype, 0.0, True, dtype)
+    w.requires_grad_()
+    want = torch.autograd.grad(ops.add_rms_norm(x, w, res, p=0.5, seed=1)[0].sum(), w)[0]
+    with torch.inference_mode():
+        x2, res2 = x.clone(), res.clone()
+    for a, b in ((x2, res), (x, res2), (x2, res2)):
+        assert torch.equal(torch.autograd.grad(ops.add_rms_norm(a, w, b, p=0.5, seed=1)[0].sum(), w)[0], want)
