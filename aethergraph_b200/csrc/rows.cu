@@ -318,8 +318,8 @@ __device__ __forceinline__ void drop_by_bits(const Drop &d, uint32_t stay, Chunk
 constexpr int kThreads = 256;
 
 // Two chunks a thread, a block's width apart; both loads are in flight before either is used.  38 411 x 256
-// bf16: 10.6 us (0.57 of the copy rate), bound by instructions, of which the generator's ten rounds are
-// the largest part.
+// bf16: 10.6 us (0.57 of the copy rate), bound by instructions: of 156 a chunk the generator's ten rounds are
+// less than half, the rest is addresses, conversion, selects and packing.
 template <typename T, int MODE, bool RAGGED>
 __global__ void __launch_bounds__(kThreads)
 k_dropout(const T *x, T *y, uint64_t total, uint32_t dim, Divide chunks, uint64_t x_stride, uint64_t y_stride, Drop d) {
@@ -586,7 +586,9 @@ struct NormBackArgs {
 // pass normalised: f32 rows (and x alone) hold it, for 16-bit rows it is made again from x and residual, which is
 // one tensor more to read than the rounded h where there is a residual.
 //
-// 16 384 x 4096 f16: 102 us (0.80 of the copy rate), 38 411 x 256 bf16 20 us (0.75), 20 011 x 602 f32 42 us (0.88).
+// 16 384 x 4096 f16: 101 us (0.81 of the copy rate), 38 411 x 256 bf16 with residual and dropout 25 us (0.73), 20 011 x 602 f32
+// 42 us (0.88).  What is made again costs its bytes: 38 411 x 256 bf16 took 21 us from the rounded h, 16 384 x 4096 bf16 with
+// residual, forward and backward, 187 where it takes 207.
 // Bound by instructions with 16 to 32 warps an SM: bringing the next row into shared memory meanwhile (cp.async) made
 // it slower (139 us where this took 122), leaving the ragged path out of the aligned kernel faster (122 to 102).
 // AGAIN: h may have to be made again.  The mask is then needed twice and kept as bits; else it is made where dx is.
@@ -790,13 +792,14 @@ int32_t check_pitches(const char *who, std::initializer_list<uint64_t> pitches) 
 // `most` chunks each (64 bytes of f16 / bf16 or f32: a thread's loads are all in flight together, and the sum
 // waits for fewer warps), unless that leaves many of them idle; a chunk each where there are no more rows than
 // SMs, and the time is one row's latency, and in the backward pass over rows that are not aligned (registers); two where the backward
-// pass makes h again, as long as the row fits (registers: four spill).  16 384 rows of 4096 f16, forward: four chunks 52 us, two 64, one 66.
+// pass makes h again through a mask, as long as the row fits (registers).  16 384 rows of 4096 bf16 with residual, forward and
+// backward: two chunks 250 us, four 256; without dropout 219 and 207.  16 384 rows of 4096 f16, forward: four chunks 52 us, two 64, one 66.
 struct Split {
     uint32_t lanes, threads;
     int chunks;
     uint32_t log2_lanes() const { uint32_t l = 0; while ((1u << l) < lanes) ++l; return lanes ? l : 5; }
 };
-Split split_row(uint64_t rows, uint32_t dim, int dtype, bool vec, bool backward, bool again = false) {
+Split split_row(uint64_t rows, uint32_t dim, int dtype, bool vec, bool backward, bool mask_again = false) {
     const uint32_t n = (dim + kChunk - 1) / kChunk;
     Split s{1, kThreads, 1};
     if (!vec) s.lanes = 4;
@@ -806,7 +809,7 @@ Split split_row(uint64_t rows, uint32_t dim, int dtype, bool vec, bool backward,
         return s;
     }
     s.lanes = 0;
-    const int most = rows <= (uint64_t)kSMs || (!vec && backward) ? 1 : dtype == AG_F32 || again ? 2 : 4;
+    const int most = rows <= (uint64_t)kSMs || (!vec && backward) ? 1 : dtype == AG_F32 || mask_again ? 2 : 4;
     uint32_t slots = 0xFFFFFFFFu;
     for (int c = most; c; c /= 2) {
         const uint32_t threads = (n + 32 * c - 1) / (32 * c) * 32;
@@ -877,7 +880,7 @@ cudaError_t launch_back(const NormBackArgs &a, const Split &s, uint32_t &grid, c
 
 template <typename T, int MODE>
 cudaError_t launch_back(const NormBackArgs &a, int dtype, uint32_t &grid, cudaStream_t st) {
-    const Split s = split_row(a.rows, a.dim, dtype, MODE == kWhole, true, !a.h);
+    const Split s = split_row(a.rows, a.dim, dtype, MODE == kWhole, true, !a.h && a.drop.on);
     if (s.lanes) {
         if (s.chunks == 1) return with_lanes<MODE>(s.lanes, [&](auto l) { return launch_back<T, MODE, 1, false, decltype(l)::value>(a, s, grid, st); });
         return launch_back<T, MODE, 2, false>(a, s, grid, st);
