@@ -115,14 +115,15 @@ k_product_dot(ProductArgs a) {
 // of its number mod 4, so two warps share a quarter of the rows and split the columns).  Each
 // epilogue thread loads its own row's scales, four steps at a time, four steps ahead and across tiles.
 //
-// Measured: 131 072 x 2048 x 1024 to bf16 305 us (1.8 PFLOP/s, 1.1 of the measured bf16 rate of the library's
-// product).  Without the epilogue's work 230 us: a step's 32 KB pass through shared memory twice, on their
+// Measured: 131 072 x 2048 x 1024 to bf16 305 us alone, 313 - 325 back to back, up to 373 for a second and more under the
+// power cap (1.8 - 1.5 PFLOP/s; 1.1 - 0.9 of the measured bf16 rate of the library's product).  Without the epilogue's work 230 us: a step's 32 KB pass through shared memory twice, on their
 // way in and as operands, 512 clocks at 128 bytes where its multiplications take 256.  The rest is
 // TMEM reads and sums that do not hide behind them.  38 411 x 256 x 256 without ids 11.8 us, of them
-// about 4 the launch and the first tile's chain, then 1.6 us a round of 148 tiles: 4.5 TB/s.
+// about 4 the launch and the first tile's chain, then 1.6 us a round of 148 tiles: 4.5 TB/s, rows from L2.  By id 12.9 us
+// with the same ids in every call (rows in L2), 14.3 with others each time (rows of 2 M, from HBM).
 //
 // Every wait is bounded.  A role whose wait runs out marks the block dead and the sticky error
-// word; all roles then leave their loops, copies and multiplications in flight are waited for
+// word (the store's, or the device's); all roles then leave their loops, copies and multiplications in flight are waited for
 // (bounded too) and TMEM is freed.
 constexpr int kBM = 128, kBK = 128, kAccStages = 4, kTileThreads = 384;
 constexpr long long kWaitLimit = 4000000000ll;  // clocks, two seconds
