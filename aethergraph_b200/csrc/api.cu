@@ -1150,6 +1150,7 @@ extern "C" int32_t ag_features_save(const char *path, const float *features, uin
 extern "C" void ag_features_free(ag_features *f) {
     if (!f) return;
     DeviceGuard guard(f->device);
+    cudaDeviceSynchronize();  // gathers and products may still read the rows: unlike cudaFree, taking a mapping away waits for nobody
     if (f->owns_payload) {
         if (f->block) peer_block_free(f->block); else cudaFree(f->payload);
         cudaFree(f->scales);

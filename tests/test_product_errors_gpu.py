@@ -80,3 +80,37 @@ def test_a_store_in_other_types_has_no_product(ops):  # noqa: F811
     for dtype in ("f32", "bf16", "i8"):
         with pytest.raises(ValueError, match="8-bit float rows"):
             FeatureStore.from_array(rand(1, 4, 64), dtype).project(ids, *ops.encode_weight_f8(rand(2, 8, 64)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f8"])
+def test_a_store_that_goes_while_it_is_read(ops, dtype):  # noqa: F811
+    """The last reference to a store goes right after its calls, which wait behind other work."""
+    from aethergraph_b200 import FeatureStore
+
+    x = rand(1, 50_000, 128)
+    ids = torch.randint(0, 50_000, (100_000,), device="cuda")
+    w = ops.encode_weight_f8(rand(2, 64, 128))
+    kept = FeatureStore.from_array(x, dtype)
+    want = kept.gather(ids), kept.project(ids, *w) if dtype == "f8" else None
+    a = torch.randn(4096, 4096, device="cuda")
+    for _ in range(3):
+        store = FeatureStore.from_array(x, dtype)
+        for _ in range(30):
+            a = a @ a
+            a = a / a.abs().max()
+        got = store.gather(ids), store.project(ids, *w) if dtype == "f8" else None
+        del store
+        assert torch.equal(got[0], want[0]) and (dtype != "f8" or torch.equal(got[1], want[1]))
+
+
+def test_where_a_stores_rows_are(ops, stores):  # noqa: F811
+    """The rows of a store, for a product of the C ABI without the store."""
+    import ctypes as C
+
+    from aethergraph_b200 import FeatureStore, _lib
+
+    codes, scales = ops.encode_f8(rand(1, 6, 40))
+    store = FeatureStore.from_f8(codes, scales)
+    at, s, pitch = C.c_void_p(), C.c_void_p(), C.c_uint64()
+    _lib.check(_lib.lib().ag_features_f8_rows(store._h, C.byref(at), C.byref(s), C.byref(pitch)))
+    assert (at.value, s.value, pitch.value) == (codes.data_ptr(), scales.data_ptr(), codes.stride(0))
