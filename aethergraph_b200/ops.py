@@ -75,7 +75,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, residual: 
                  p: float = 0.0, seed: int = 0, offset: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
     """(y, h): h = residual + dropout(x), y = h / sqrt(mean(h**2) + eps) * weight, row by row.
 
-    One pass over the rows: sum, statistics and product are held in float32 and rounded once.
+    One pass over the rows: sum, statistics and product are held in float32 and rounded once; rows whose squares pass
+    float32 (magnitudes beyond about 1e19) come out as zeros.
     Without residual and dropout h is `x` itself.  `weight` is [dim], of x's type or float32; rows have at most 16384 columns.  The
     gradients of x, weight and residual take one pass too; weight's is summed in a fixed order.  They are those of the
     unrounded h: for float16 and bfloat16 rows x and residual are kept for the backward pass (as autograd keeps any operator's

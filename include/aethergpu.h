@@ -697,7 +697,8 @@ int32_t ag_rows_dropout(const void *x, void *y, uint64_t rows, uint64_t dim, uin
                         uint64_t y_stride, int32_t dtype, double p, uint64_t seed, uint64_t offset,
                         int32_t device, void *stream);
 /* h = residual + dropout(x);  y = h / sqrt(mean(h^2) + eps) * weight, the mean over the row's
- * columns (at most 16384), in f32 and rounded once to the rows' type.  Out come y, or codes and
+ * columns (at most 16384), in f32 and rounded once to the rows' type (rows whose squares pass f32 give
+ * zeros).  Out come y, or codes and
  * scales (8-bit rows, below), and where not NULL h and 1 / sqrt(..) per row (f32, what the
  * backward pass needs).  residual and weight may be NULL.  encode_only: no norm, x itself
  * becomes 8-bit rows.
